@@ -4,6 +4,7 @@
 #include "../../include/fal_b200.h"
 
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -1095,6 +1096,219 @@ int fal_cache_append(const void* k_new, const void* v_new, void* k_cache, void* 
   p.batch = batch; p.heads_kv = heads_kv; p.rows = rows; p.capacity = capacity; p.head_dim = head_dim;
   cudaError_t e = fal::launch_cache_append(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? FAL_OK : cuda_fail(e);
+}
+
+// ---------------------------------------------------------------------------
+// Paged caches
+// ---------------------------------------------------------------------------
+static_assert(sizeof(fal_paged_append_args) == 368 && sizeof(fal_paged_attn_args) == 288,
+              "the Python binding packs these blocks");
+
+namespace {
+
+bool paged_strides_ok(const fal_strides& s, int per16) {
+  return s.batch % per16 == 0 && s.head % per16 == 0 && s.row % per16 == 0;
+}
+
+// (no CUDA call is made here)
+int paged_check(const fal_paged_cache& c) {
+  if (!c.k_pages || !c.v_pages || !c.block_table || !c.cache_seqlens) return FAL_ERR_INVALID_ARGUMENT;
+  if (c.dtype < FAL_PAGED_F16 || c.dtype > FAL_PAGED_E4M3) return FAL_ERR_INVALID_ARGUMENT;
+  if (c.batch <= 0 || c.batch > 65535 || c.heads_kv <= 0 || c.heads_kv > 32767 || c.num_pages <= 0 || c.pages_per_entry <= 0)
+    return FAL_ERR_INVALID_ARGUMENT;
+  if (c.page_size < 16 || c.page_size > fal::kPagedMostRows || (c.page_size & (c.page_size - 1)) != 0)
+    return FAL_ERR_INVALID_ARGUMENT;
+  if (static_cast<int64_t>(c.pages_per_entry) * c.page_size > (1 << 30)) return FAL_ERR_INVALID_ARGUMENT;
+  if (!head_dim_ok(c.head_dim)) return FAL_ERR_UNSUPPORTED_HEAD_DIM;
+  auto aligned16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; };
+  const int per16 = c.dtype == FAL_PAGED_F16 ? 8 : 16;
+  if (!aligned16(c.k_pages) || !aligned16(c.v_pages) || !paged_strides_ok(c.k_strides, per16) ||
+      !paged_strides_ok(c.v_strides, per16))
+    return FAL_ERR_INVALID_ARGUMENT;
+  if (c.dtype != FAL_PAGED_F16 &&
+      (!c.k_scales || !c.v_scales || !c.k_tail || !c.v_tail || !aligned16(c.k_tail) || !aligned16(c.v_tail) ||
+       !paged_strides_ok(c.k_tail_strides, 8) || !paged_strides_ok(c.v_tail_strides, 8)))
+    return FAL_ERR_INVALID_ARGUMENT;
+  return FAL_OK;
+}
+
+fal::PagedCache paged_cache(const fal_paged_cache& c) {
+  fal::PagedCache p{};
+  p.k_pages = c.k_pages; p.v_pages = c.v_pages; p.k_scales = c.k_scales; p.v_scales = c.v_scales;
+  p.k_tail = c.k_tail; p.v_tail = c.v_tail;
+  p.k_strides = to_rs(&c.k_strides); p.v_strides = to_rs(&c.v_strides);
+  p.k_tail_strides = to_rs(&c.k_tail_strides); p.v_tail_strides = to_rs(&c.v_tail_strides);
+  p.table = c.block_table; p.table_stride = c.table_stride; p.lens = c.cache_seqlens;
+  p.type = c.dtype; p.num_pages = c.num_pages; p.pages_per_entry = c.pages_per_entry;
+  p.batch = c.batch; p.heads_kv = c.heads_kv; p.head_dim = c.head_dim;
+  while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
+  return p;
+}
+
+// Query rows of a KV head up to which the split-K pass takes them, 8 or 16 to a CTA that streams the keys for itself.
+constexpr int64_t kPagedFewRows = 64;
+constexpr int64_t kPagedGatherBytes = int64_t{1} << 30;
+
+// How a call is cut up, and what it needs of the workspace.
+struct PagedPlan {
+  bool few_rows;
+  int split_shift, fine_splits, grid_splits, splits;  // few rows
+  int entries, heads;  // many: (entry, KV head) pairs whose rows are put in order at a time
+  size_t k_bytes, lse_bytes, split_bytes;
+  size_t total;
+};
+
+PagedPlan paged_plan(const fal_paged_attn_args& a) {
+  const fal_paged_cache& c = a.cache;
+  const int64_t capacity = static_cast<int64_t>(c.pages_per_entry) * c.page_size;
+  const int group = a.heads_q / c.heads_kv;
+  const int64_t rows = static_cast<int64_t>(a.rows) * group;
+  const int dim = kernel_head_dim(c.head_dim);
+  PagedPlan p{};
+  p.few_rows = rows <= kPagedFewRows;
+  if (p.few_rows) {
+    const bool half = c.dtype == FAL_PAGED_F16;
+    const int per_cta = fal::paged_rows_per_cta(static_cast<int>(rows), dim);
+    const int64_t units = c.batch * c.heads_kv * ((rows + per_cta - 1) / per_cta);
+    const int64_t sms = sm_count() > 0 ? sm_count() : 148;
+    p.split_shift = (half ? 10 : 11) + (c.batch * (((capacity - 1) >> 11) + 1) >= 192 ? 1 : 0);
+    while (((capacity - 1) >> p.split_shift) + 1 > 1024) ++p.split_shift;
+    const int64_t most = ((capacity - 1) >> fal::kDecodeFinestShift) + 1;
+    int64_t fine = sms * (dim == 64 ? 4 : dim == 256 ? 1 : half ? 2 : 3) / units;
+    const int64_t fit = static_cast<int64_t>(kDecodeFineBytes / decode_partial_bytes(c.batch * a.rows, a.heads_q, 1, dim));
+    if (fine > fit) fine = fit;
+    if (fine > most) fine = most;
+    p.fine_splits = static_cast<int>(fine);
+    p.grid_splits = static_cast<int>(((capacity - 1) >> p.split_shift) + 1);
+    if (p.grid_splits < p.fine_splits) p.grid_splits = p.fine_splits;
+    p.splits = p.grid_splits + (half ? 0 : 1);
+    p.total = decode_partial_bytes(c.batch * a.rows, a.heads_q, p.splits, dim);
+    return p;
+  }
+  const int64_t unit = capacity * c.head_dim * 4;  // K and V
+  p.heads = static_cast<int>(kPagedGatherBytes / unit < c.heads_kv ? kPagedGatherBytes / unit : c.heads_kv);
+  if (p.heads < 1) p.heads = 1;
+  p.entries = 1;
+  if (p.heads == c.heads_kv) {
+    const int64_t e = kPagedGatherBytes / (unit * c.heads_kv);
+    p.entries = static_cast<int>(e < 1 ? 1 : e < c.batch ? e : c.batch);
+  }
+  p.k_bytes = static_cast<size_t>(p.entries) * p.heads * capacity * c.head_dim * 2;
+  p.lse_bytes = round_up(static_cast<int64_t>(p.entries) * p.heads * group * a.rows * 4, 256);
+  p.split_bytes = fal_fwd_kvcache_workspace_bytes(p.entries, p.heads * group, a.rows, static_cast<int>(capacity), c.head_dim);
+  p.total = 2 * p.k_bytes + p.lse_bytes + p.split_bytes;
+  return p;
+}
+
+int paged_attn_check(const fal_paged_attn_args& a) {
+  const int rc = paged_check(a.cache);
+  if (rc != FAL_OK) return rc;
+  if (!a.q || !a.o || a.rows <= 0 || a.heads_q <= 0 || a.heads_q % a.cache.heads_kv != 0 || !(a.softmax_scale > 0.f))
+    return FAL_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15u) != 0 || !paged_strides_ok(a.q_strides, 8))
+    return FAL_ERR_INVALID_ARGUMENT;
+  if (static_cast<int64_t>(a.cache.batch) * a.rows * a.heads_q > 0x7fffffff) return FAL_ERR_INVALID_ARGUMENT;
+  return FAL_OK;
+}
+
+}  // namespace
+
+int fal_paged_append_run(const fal_paged_append_args* a) {
+  if (!a) return FAL_ERR_INVALID_ARGUMENT;
+  int rc = paged_check(a->cache);
+  if (rc != FAL_OK) return rc;
+  const fal_paged_cache& c = a->cache;
+  if (!a->k || !a->v || !a->new_seqlens || a->rows <= 0 || a->heads_q < 0 || (a->q == nullptr) != (a->heads_q == 0) ||
+      (a->q == nullptr) != (a->q_out == nullptr))
+    return FAL_ERR_INVALID_ARGUMENT;
+  auto aligned16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; };
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->rotary_cos) ||
+      !aligned16(a->rotary_sin) || !paged_strides_ok(a->k_new_strides, 8) || !paged_strides_ok(a->v_new_strides, 8) ||
+      (a->q != nullptr && !paged_strides_ok(a->q_strides, 8)))
+    return FAL_ERR_INVALID_ARGUMENT;
+  if ((a->rotary_cos == nullptr) != (a->rotary_sin == nullptr)) return FAL_ERR_INVALID_ARGUMENT;
+  if (a->rotary_cos != nullptr &&
+      (a->rotary_dim <= 0 || a->rotary_dim % 16 != 0 || a->rotary_dim > c.head_dim ||
+       a->rotary_positions < static_cast<int64_t>(c.pages_per_entry) * c.page_size))
+    return FAL_ERR_INVALID_ARGUMENT;
+  if (static_cast<int64_t>(c.batch) * a->rows > 0x7fffffff || a->heads_q > (1 << 19)) return FAL_ERR_INVALID_ARGUMENT;
+  rc = check_device();
+  if (rc != FAL_OK) return rc;
+  fal::PagedAppendParams p{};
+  p.c = paged_cache(c);
+  p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out;
+  p.q_strides = to_rs(&a->q_strides); p.k_new_strides = to_rs(&a->k_new_strides); p.v_new_strides = to_rs(&a->v_new_strides);
+  p.cos = a->rotary_cos; p.sin = a->rotary_sin; p.half_tables = a->rotary_half; p.positions = a->rotary_positions;
+  p.rotary_dim = a->rotary_cos != nullptr ? a->rotary_dim : 0;
+  p.interleaved = a->rotary_interleaved;
+  p.heads_q = a->heads_q; p.rows = a->rows; p.new_lens = a->new_seqlens; p.status = a->status;
+  const cudaError_t e = fal::launch_paged_append(p, static_cast<cudaStream_t>(a->stream));
+  return e == cudaSuccess ? FAL_OK : cuda_fail(e);
+}
+
+size_t fal_paged_attn_workspace_bytes(const fal_paged_attn_args* a) {
+  // (the pointers of the workspace itself and of what the call writes may still be missing)
+  if (!a || a->cache.batch <= 0 || a->cache.heads_kv <= 0 || a->cache.page_size <= 0 || a->cache.pages_per_entry <= 0 ||
+      static_cast<int64_t>(a->cache.pages_per_entry) * a->cache.page_size > (1 << 30) || a->heads_q < a->cache.heads_kv ||
+      a->rows <= 0 || !head_dim_ok(a->cache.head_dim) || static_cast<int64_t>(a->cache.batch) * a->rows * a->heads_q > 0x7fffffff)
+    return 0;
+  return paged_plan(*a).total;
+}
+
+int fal_paged_attn_run(const fal_paged_attn_args* a) {
+  if (!a) return FAL_ERR_INVALID_ARGUMENT;
+  int rc = paged_attn_check(*a);
+  if (rc != FAL_OK) return rc;
+  const PagedPlan plan = paged_plan(*a);
+  if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return FAL_ERR_INVALID_ARGUMENT;
+  if (a->workspace_bytes < plan.total) return FAL_ERR_WORKSPACE_TOO_SMALL;
+  rc = check_device();
+  if (rc != FAL_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+  const fal_paged_cache& c = a->cache;
+  if (plan.few_rows) {
+    fal::PagedAttnParams p{};
+    p.c = paged_cache(c);
+    p.q = a->q; p.q_strides = to_rs(&a->q_strides); p.o = a->o;
+    p.heads_q = a->heads_q; p.rows = a->rows; p.kernel_dim = kernel_head_dim(c.head_dim);
+    p.split_shift = plan.split_shift; p.fine_splits = plan.fine_splits;
+    p.grid_splits = plan.grid_splits; p.splits = plan.splits;
+    p.part_o = static_cast<float*>(a->workspace);
+    p.part_ml = p.part_o + static_cast<int64_t>(c.batch) * a->rows * a->heads_q * p.splits * p.kernel_dim;
+    p.scale = a->softmax_scale; p.status = a->status;
+    const cudaError_t e = fal::launch_paged_attn(p, st);
+    return e == cudaSuccess ? FAL_OK : cuda_fail(e);
+  }
+
+  const int capacity = c.pages_per_entry * c.page_size;
+  const int group = a->heads_q / c.heads_kv;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  fal::PagedGatherParams g{};
+  g.c = paged_cache(c);
+  g.k_out = ws;
+  g.v_out = ws + plan.k_bytes;
+  g.status = a->status;
+  float* lse = reinterpret_cast<float*>(ws + 2 * plan.k_bytes);
+  void* split = plan.split_bytes != 0 ? ws + 2 * plan.k_bytes + plan.lse_bytes : nullptr;
+  const fal_strides o_strides = {static_cast<int64_t>(a->rows) * a->heads_q * c.head_dim, c.head_dim,
+                                 static_cast<int64_t>(a->heads_q) * c.head_dim};
+  for (g.b0 = 0; g.b0 < c.batch; g.b0 += plan.entries) {
+    g.entries = c.batch - g.b0 < plan.entries ? c.batch - g.b0 : plan.entries;
+    for (g.h0 = 0; g.h0 < c.heads_kv; g.h0 += plan.heads) {
+      g.heads = c.heads_kv - g.h0 < plan.heads ? c.heads_kv - g.h0 : plan.heads;
+      const cudaError_t e = fal::launch_paged_gather(g, st);
+      if (e != cudaSuccess) return cuda_fail(e);
+      const fal_strides kv = {static_cast<int64_t>(g.heads) * capacity * c.head_dim,
+                              static_cast<int64_t>(capacity) * c.head_dim, c.head_dim};
+      const __half* q = static_cast<const __half*>(a->q) + g.b0 * a->q_strides.batch + g.h0 * group * a->q_strides.head;
+      __half* o = static_cast<__half*>(a->o) + g.b0 * o_strides.batch + g.h0 * group * o_strides.head;
+      rc = fwd_batched(q, g.k_out, g.v_out, o, lse, c.cache_seqlens + g.b0, g.entries, g.heads * group, g.heads, a->rows,
+                       capacity, c.head_dim, &a->q_strides, &kv, &kv, &o_strides, a->softmax_scale,
+                       FAL_CAUSAL_BOTTOM_RIGHT, a->status, a->stream, split, plan.split_bytes);
+      if (rc != FAL_OK) return rc;
+    }
+  }
+  return FAL_OK;
 }
 
 int fal_set_fwd_variant(int variant) {

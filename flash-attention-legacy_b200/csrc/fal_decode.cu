@@ -31,6 +31,7 @@
 // of the cache: the entry's row pointers start there and its length shrinks.
 #include <type_traits>
 
+#include "fal_combine.cuh"
 #include "fal_common.h"
 #include "fal_launch.h"
 #include "sm100_ptx.cuh"
@@ -45,19 +46,6 @@ constexpr int kSliceKeys = 16;  // keys per warp step
 constexpr int kDecStages = 3;   // per-warp pipeline depth
 constexpr float kNegInfD = -INFINITY;
 
-__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool valid) {
-  const uint32_t n = valid ? 16u : 0u;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
                                             uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -70,16 +58,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, u
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
                : "r"(addr));
 }
-// D (fp32, 16x8) += A (fp16, 16x16) * B (fp16, 16x8)
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // ---------------------------------------------------------------------------
 // Append + split-K pass + merge by the last CTA to arrive.
 // ---------------------------------------------------------------------------
@@ -400,31 +378,15 @@ fal_decode_splitk_kernel(const DecodeParams p) {
 // (4 095); 256 x 32 of 128, 1 split 36.5 / 30.0; 8 x 32 of 64, 9 splits 8.2 / 8.0; 1 x 32 of 128, 16 splits 9.1 / 10.8;
 // 4 x 32 of 128, 32 splits 93.1 / 101.3; 1 x 8 of 64, 64 splits 8.8 / 13.2.
 // It is launched while the split-K grid still runs and waits here for that grid's results.
-constexpr int kCombineThreads = 128;
 constexpr int kCombineWarpBytes = 2048;  // of partials of a row, up to which one warp merges them;
 constexpr int kCombineManyRows = 256;    // twice as many in a grid of this many rows
-
-// (m, l) <- the merge with another running maximum and sum (log2 domain).
-__device__ __forceinline__ void merge_stats(float& m, float& l, float m2, float l2) {
-  const float m_new = fmaxf(m, m2);
-  const float m_use = (m_new == kNegInfD) ? 0.f : m_new;
-  l = l * fast_exp2(m - m_use) + l2 * fast_exp2(m2 - m_use);
-  m = m_new;
-}
 
 template <int D, int WARPS>
 __global__ void __launch_bounds__(kCombineThreads)
 fal_decode_combine_kernel(const DecodeParams p) {
-  static_assert(WARPS == 1 || WARPS * 32 == kCombineThreads, "a row per warp or per block");
   constexpr int kRows = kCombineThreads / (32 * WARPS);      // (batch, head) rows per block
-  constexpr int kThreads = 32 * WARPS;                       // threads per row
-  constexpr int kLanes = D / 4 < kThreads ? D / 4 : kThreads;  // threads per partial row
-  constexpr int kVecs = D / (4 * kLanes);                    // 16-byte pieces of it per thread
-  constexpr int kGroups = kThreads / kLanes;                 // partial rows in flight
-  __shared__ float2 warp_ml[WARPS];
-  __shared__ float4 part[kGroups][kLanes];
-  const int tid = threadIdx.x % kThreads;
-  const int bh = blockIdx.x * kRows + threadIdx.x / kThreads;
+  const int tid = threadIdx.x % (32 * WARPS);
+  const int bh = blockIdx.x * kRows + threadIdx.x / (32 * WARPS);
   const bool row_ok = bh < p.batch * p.heads_q;
   int n = 0;
   if (row_ok) {
@@ -433,107 +395,8 @@ fal_decode_combine_kernel(const DecodeParams p) {
   }
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + static_cast<int64_t>(bh) * p.splits;
   const float4* po = reinterpret_cast<const float4*>(p.part_o) + static_cast<int64_t>(bh) * p.splits * (D / 4);
-  // (The lengths were not written by the split-K grid, and whatever wrote them ended before that grid let this one start.)
-  grid_dependency_wait();
-  if (!row_ok) return;  // (whole warps; a block of one row has that row)
-
-  // The first partial rows of this thread are fetched with the statistics, not behind them: one round trip to L2 for three.
-  constexpr int kAhead = 4;
-  const int lane = tid % kLanes;
-  const int grp = tid / kLanes;
-  float mx[kAhead];
-  float4 px[kAhead][kVecs];
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) {
-    const int i = grp + k * kGroups;
-    mx[k] = kNegInfD;
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) px[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (i < n) {
-      mx[k] = ml[i].x;
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) px[k][v] = po[static_cast<int64_t>(i) * (D / 4) + v * kLanes + lane];
-    }
-  }
-  float m = kNegInfD, l = 0.f;
-  for (int i = tid; i < n; i += kThreads) {
-    const float2 x = ml[i];
-    merge_stats(m, l, x.x, x.y);
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, off);
-    const float l2 = __shfl_xor_sync(0xffffffffu, l, off);
-    merge_stats(m, l, m2, l2);
-  }
-  if constexpr (WARPS > 1) {
-    if ((tid & 31) == 0) warp_ml[tid >> 5] = make_float2(m, l);
-    __syncthreads();
-    m = warp_ml[0].x;
-    l = warp_ml[0].y;
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) merge_stats(m, l, warp_ml[w].x, warp_ml[w].y);
-  }
-  const float muse = (m == kNegInfD) ? 0.f : m;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-
-  float4 o[kVecs];
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add_weighted = [&](float4& a, float w, const float4& x) {
-    a.x += w * x.x;
-    a.y += w * x.y;
-    a.z += w * x.z;
-    a.w += w * x.w;
-  };
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) {
-    if (grp + k * kGroups < n) {
-      const float w = fast_exp2(mx[k] - muse);
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) add_weighted(o[v], w, px[k][v]);
-    }
-  }
-#pragma unroll 4
-  for (int i = grp + kAhead * kGroups; i < n; i += kGroups) {
-    const float w = fast_exp2(ml[i].x - muse);
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) add_weighted(o[v], w, po[static_cast<int64_t>(i) * (D / 4) + v * kLanes + lane]);
-  }
-  auto add = [&](float4& a, const float4& x) {
-    a.x += x.x;
-    a.y += x.y;
-    a.z += x.z;
-    a.w += x.w;
-  };
-  if constexpr (WARPS > 1) {
-    static_assert(kVecs == 1, "one piece per thread");
-    part[grp][lane] = o[0];
-    __syncthreads();
-    if (grp == 0) {
-#pragma unroll
-      for (int g = 1; g < kGroups; ++g) add(o[0], part[g][lane]);
-    }
-  } else {
-#pragma unroll
-    for (int off = kLanes; off < 32; off <<= 1) {  // (one piece per thread then)
-      const float4 x = make_float4(__shfl_xor_sync(0xffffffffu, o[0].x, off), __shfl_xor_sync(0xffffffffu, o[0].y, off),
-                                   __shfl_xor_sync(0xffffffffu, o[0].z, off), __shfl_xor_sync(0xffffffffu, o[0].w, off));
-      add(o[0], x);
-    }
-  }
   __half* out_row = static_cast<__half*>(p.o) + static_cast<int64_t>(bh) * p.head_dim_real;
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const int col = (v * kLanes + lane) * 4;
-    if (grp == 0 && col < p.head_dim_real) {
-      uint2 out;
-      out.x = pack_half2(o[v].x * inv, o[v].y * inv);
-      out.y = pack_half2(o[v].z * inv, o[v].w * inv);
-      *reinterpret_cast<uint2*>(out_row + col) = out;
-    }
-  }
-  if (p.lse != nullptr && tid == 0) p.lse[bh] = (l > 0.f) ? (m + log2f(l)) * 0.6931471805599453f : kNegInfD;
+  combine_row<D, WARPS>(tid, row_ok, n, ml, po, out_row, p.head_dim_real, p.lse != nullptr ? p.lse + bh : nullptr);
 }
 
 // ---------------------------------------------------------------------------

@@ -189,4 +189,81 @@ cudaError_t decode_static_scratch(float** ptr);
 cudaError_t launch_decode_splitk(const DecodeParams& p, cudaStream_t stream);
 cudaError_t launch_decode_combine(const DecodeParams& p, cudaStream_t stream);
 
+// Paged caches (fal_paged.cu): position p of entry b is row p % page of page table[b, p / page].  8-bit pages hold codes
+// with one fp32 scale per page and KV head; the rows of an entry's last, unfinished page are fp16 rows of its tail.
+constexpr int kPagedMostRows = 256;  // of a page
+enum PagedType : int { kPagedF16 = 0, kPagedS8 = 1, kPagedE4M3 = 2 };
+struct PagedCache {
+  void* k_pages;
+  void* v_pages;
+  float* k_scales;       // [num_pages, heads_kv], 8-bit pages only (as all of the next four)
+  float* v_scales;
+  void* k_tail;          // [batch, head, row] fp16
+  void* v_tail;
+  RowStrides k_strides, v_strides;            // page / head / row, in elements
+  RowStrides k_tail_strides, v_tail_strides;  // entry / head / row
+  const int32_t* table;  // [batch, pages_per_entry], rows table_stride apart
+  int64_t table_stride;
+  const int32_t* lens;   // [batch]
+  int type;
+  int num_pages;
+  int page_shift;        // log2 of the rows of a page
+  int pages_per_entry;
+  int batch;
+  int heads_kv;
+  int head_dim;          // the tensors' head_dim
+};
+
+// New rows: q and k rotated by their positions, k and v to their places in the cache.
+struct PagedAppendParams {
+  PagedCache c;          // (lens: before the append)
+  const void* q;         // optional
+  const void* k;
+  const void* v;
+  void* q_out;           // [batch, rows, heads_q, head_dim]
+  RowStrides q_strides, k_new_strides, v_new_strides;  // entry / head / row
+  const void* cos;       // [positions, rotary_dim / 2] fp32 or fp16, or null: no rotation
+  const void* sin;
+  int half_tables;
+  int positions;
+  int rotary_dim;
+  int interleaved;       // pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2)
+  int heads_q;           // 0 without q
+  int rows;
+  int32_t* new_lens;     // [batch]
+  int* status;
+};
+cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream);
+
+// Attention of a few query rows per KV head over the pages: split-K pass and merge.
+struct PagedAttnParams {
+  PagedCache c;
+  const void* q;         // [batch, rows, heads_q, head_dim] fp16 through strides (entry / head / row)
+  RowStrides q_strides;
+  void* o;               // [batch, rows, heads_q, head_dim] fp16, contiguous
+  float* part_o;         // workspace [batch, rows, heads_q, splits, kernel head_dim]
+  float* part_ml;        // workspace [batch, rows, heads_q, splits, 2]
+  int heads_q;
+  int rows;              // query i sees the keys up to position len - rows + i
+  int kernel_dim;        // 64, 128 or 256
+  int split_shift, fine_splits;  // as for decode
+  int grid_splits;       // splits of the pages that an entry can have
+  int splits;            // partials per row: grid_splits, and one more for the tail of 8-bit caches
+  float scale;
+  int* status;
+};
+// Query rows that one CTA takes.
+int paged_rows_per_cta(int rows, int kernel_dim);
+cudaError_t launch_paged_attn(const PagedAttnParams& p, cudaStream_t stream);
+
+// Entries b0 ... b0 + entries - 1 and KV heads h0 ... h0 + heads - 1 of a paged cache as fp16 rows in order.
+struct PagedGatherParams {
+  PagedCache c;
+  void* k_out;           // [entries, heads, capacity, head_dim]
+  void* v_out;
+  int b0, entries, h0, heads;
+  int* status;
+};
+cudaError_t launch_paged_gather(const PagedGatherParams& p, cudaStream_t stream);
+
 }  // namespace fal

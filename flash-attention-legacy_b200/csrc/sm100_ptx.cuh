@@ -20,7 +20,8 @@ namespace fal {
 enum DeviceStatus : int {
   kDevOk = 0,
   kDevWaitTimeout = 1000,     // + barrier id
-  kDevAppendOverflow = 2000,  // decode: a new token did not fit the cache (length >= capacity) and was dropped
+  kDevAppendOverflow = 2000,  // a new token did not fit the cache (length >= capacity, no page) and was dropped
+  kDevNoPage = 3000,          // a position within an entry's length has no page; its rows count as zeros
 };
 
 // Cycles a single mbarrier wait may take before it gives up (about one
@@ -346,6 +347,31 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
       "}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Asynchronous 16-byte copies and warp-level MMA (the kernels bound by HBM, which use tensor cores to save issue slots)
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool valid) {
+  const uint32_t n = valid ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// D (fp32, 16x8) += A (fp16, 16x16) * B (fp16, 16x8)
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Warpgroup-wide register reallocation (all four warps of a warpgroup must execute it).

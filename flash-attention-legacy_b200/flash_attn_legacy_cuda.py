@@ -91,6 +91,15 @@ for _name in ("fal_fwd_args_run", "fal_bwd_args_run", "fal_decode_args_run"):
     _fn = getattr(_lib, _name)
     _fn.restype = _i
     _fn.argtypes = [ctypes.c_char_p]
+# fal_paged_cache, then what the two calls add to it
+_PAGED_CACHE = "8Q13q8i"
+_PAGED_APPEND_ARGS = struct.Struct("@" + _PAGED_CACHE + "7Q9q6i2Q")
+_PAGED_ATTN_ARGS = struct.Struct("@" + _PAGED_CACHE + "2Q3q2ifi4Q")
+assert (_PAGED_APPEND_ARGS.size, _PAGED_ATTN_ARGS.size) == (368, 288)
+for _name in ("fal_paged_append_run", "fal_paged_attn_run", "fal_paged_attn_workspace_bytes"):
+    _fn = getattr(_lib, _name)
+    _fn.restype = ctypes.c_size_t if _name.endswith("bytes") else _i
+    _fn.argtypes = [ctypes.c_char_p]
 _lib.fal_fwd_kvcache_workspace_bytes.restype = ctypes.c_size_t
 _lib.fal_fwd_kvcache_workspace_bytes.argtypes = [_i] * 5
 _lib.fal_fwd_kvcache_split_run.restype = _i
@@ -197,7 +206,8 @@ def profile_read(kind):
     return total.value, n.value
 
 # One device status word per GPU (a 4-byte tensor created on first use); kernels set it non-zero if
-# an internal wait ran out (1000 + barrier id) or a decode append found its cache full (2000).
+# an internal wait ran out (1000 + barrier id), an append found its cache full or a page missing (2000), or attention
+# found a page missing (3000).
 _status = {}
 
 
@@ -735,6 +745,159 @@ def cache_append(k_new, v_new, k_cache, v_cache, cache_seqlens):
                                  cache_seqlens.data_ptr(), lens.data_ptr(), fits.data_ptr(), B, Hkv, rows, S, d,
                                  _stream(k_cache)))
     return lens, fits
+
+
+# ---------------------------------------------------------------------------------------------
+# Paged caches (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------------
+PAGE_SIZES = (16, 32, 64, 128, 256)
+_PAGED_TYPES = {torch.float16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+
+
+def _addressable(name, t, per16):
+    """Rows contiguous, 16-byte aligned, every longer dimension with a stride of its own."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16 != 0:
+        raise RuntimeError(f"{name} must have a contiguous last dimension and 16-byte aligned rows")
+    for s, n in zip(t.stride()[:-1], t.shape[:-1]):
+        if s % per16 != 0 or (s <= 0 and n > 1):
+            raise RuntimeError(f"{name} must have positive strides that keep rows 16-byte aligned")
+
+
+def _paged_cache(k_pages, v_pages, block_table, cache_seqlens, k_scales, v_scales, k_tail, v_tail, cache_layout, batch,
+                 head_dim):
+    """Checks the tensors of a paged cache; returns (the fal_paged_cache block's values, KV heads, capacity of an entry)."""
+    if cache_layout not in ("bshd", "bhsd"):
+        raise ValueError("cache_layout must be 'bshd' or 'bhsd'")
+    kind = _PAGED_TYPES.get(k_pages.dtype)
+    if kind is None or v_pages.dtype != k_pages.dtype:
+        raise RuntimeError("k_pages and v_pages must both be float16, int8 or float8_e4m3fn")
+    if not k_pages.is_cuda:
+        raise RuntimeError("k_pages must be on CUDA")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise RuntimeError("k_pages and v_pages must be 4D and of one shape")
+    seq, head = (1, 2) if cache_layout == "bshd" else (2, 1)
+    pages, page, heads = k_pages.shape[0], k_pages.shape[seq], k_pages.shape[head]
+    if page not in PAGE_SIZES:
+        raise RuntimeError(f"a page must hold 16, 32, 64, 128 or 256 rows, got {page}")
+    if k_pages.shape[3] != head_dim:
+        raise RuntimeError("the pages must have q's, k's and v's head_dim")
+    if pages == 0 or heads == 0:
+        raise RuntimeError("the cache must have pages and heads")
+    for name, t in (("block_table", block_table), ("cache_seqlens", cache_seqlens)):
+        if t.dtype != torch.int32:
+            raise RuntimeError(f"{name} must be int32")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] == 0 or (
+            block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise RuntimeError("block_table must be [B, pages per entry] with contiguous rows")
+    if cache_seqlens.shape != (batch,) or not cache_seqlens.is_contiguous():
+        raise RuntimeError("cache_seqlens must be contiguous [B]")
+    _addressable("k_pages", k_pages, 8 if kind == 0 else 16)
+    _addressable("v_pages", v_pages, 8 if kind == 0 else 16)
+    extras = (k_scales, v_scales, k_tail, v_tail)
+    if kind == 0:
+        if any(t is not None for t in extras):
+            raise RuntimeError("scales and tails belong to 8-bit pages")
+        more, tail_strides = (0, 0, 0, 0), (0,) * 6
+    else:
+        if any(t is None for t in extras):
+            raise RuntimeError("8-bit pages need k_scales, v_scales, k_tail and v_tail")
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if t.dtype != torch.float32 or t.shape != (pages, heads) or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be contiguous float32 [pages, H_kv]")
+        shape = (batch, *k_pages.shape[1:])
+        for name, t in (("k_tail", k_tail), ("v_tail", v_tail)):
+            if t.dtype != torch.float16 or t.shape != shape:
+                raise RuntimeError(f"{name} must be float16 {list(shape)}: a page of rows per entry")
+            _addressable(name, t, 8)
+        more = tuple(t.data_ptr() for t in extras)
+        tail_strides = tuple(t.stride(i) for t in (k_tail, v_tail) for i in (0, head, seq))
+    block = (k_pages.data_ptr(), v_pages.data_ptr(), *more, block_table.data_ptr(), cache_seqlens.data_ptr(),
+             *(t.stride(i) for t in (k_pages, v_pages) for i in (0, head, seq)), *tail_strides, block_table.stride(0),
+             kind, pages, page, block_table.shape[1], batch, heads, head_dim, 0)
+    return block, heads, block_table.shape[1] * page
+
+
+def paged_append(k, v, k_pages, v_pages, block_table, cache_seqlens, q=None, rotary_cos=None, rotary_sin=None,
+                 rotary_interleaved=False, k_scales=None, v_scales=None, k_tail=None, v_tail=None, cache_layout="bshd"):
+    """Writes k, v [B,L,Hkv,d] behind every entry's rows of a paged cache; returns (rotated q or None, new lengths).
+
+    See fal_paged_append_run in fal_b200.h.  q [B,L,Hq,d] and k are rotated on the way if the tables [positions,
+    rotary_dim / 2] (fp32 or fp16) are given.  A dropped row is reported by the device status word (2000).
+    """
+    for name, t in (("k", k), ("v", v), ("q", q)):
+        if t is not None:
+            _require_cuda_half(name, t, 4)
+            _addressable(name, t, 8)
+    B, L, heads, d = k.shape
+    if v.shape != k.shape:
+        raise RuntimeError("k and v must have the same shape")
+    if B == 0 or L == 0:
+        raise RuntimeError("k and v must have rows")
+    dev = _same_device(k, v, q, k_pages, v_pages, block_table, cache_seqlens, k_scales, v_scales, k_tail, v_tail,
+                       rotary_cos, rotary_sin)
+    block, hkv, capacity = _paged_cache(k_pages, v_pages, block_table, cache_seqlens, k_scales, v_scales, k_tail, v_tail,
+                                        cache_layout, B, d)
+    if heads != hkv:
+        raise RuntimeError("k and v must have the cache's heads")
+    caches = [t.untyped_storage().data_ptr() for t in (k_pages, v_pages, k_tail, v_tail) if t is not None]
+    if any(t is not None and t.untyped_storage().data_ptr() in caches for t in (q, k, v)):
+        raise RuntimeError("q, k and v must not share memory with the cache")
+    if not _rows_apart(k_pages, v_pages) or (k_tail is not None and not _rows_apart(k_tail, v_tail)):
+        raise RuntimeError("K and V must not share rows of the cache")
+    heads_q, q_strides, q_out = 0, (0, 0, 0), None
+    if q is not None:
+        if q.shape[0] != B or q.shape[1] != L or q.shape[3] != d or q.shape[2] == 0:
+            raise RuntimeError("q must be [B, L, H_q, d] with k's B, L and d")
+        heads_q, q_strides = q.shape[2], (q.stride(0), q.stride(2), q.stride(1))
+        q_out = torch.empty((B, L, heads_q, d), dtype=torch.float16, device=q.device)
+    if (rotary_cos is None) != (rotary_sin is None):
+        raise RuntimeError("rotary_cos and rotary_sin go together")
+    rotary_dim, half, positions = 0, 0, 0
+    if rotary_cos is not None:
+        if (rotary_cos.dtype not in (torch.float32, torch.float16) or rotary_sin.dtype != rotary_cos.dtype
+                or rotary_cos.dim() != 2 or rotary_sin.shape != rotary_cos.shape
+                or not rotary_cos.is_contiguous() or not rotary_sin.is_contiguous()):
+            raise RuntimeError("rotary_cos and rotary_sin must be contiguous float32 or float16 [positions, rotary_dim / 2]")
+        positions, rotary_dim, half = rotary_cos.shape[0], 2 * rotary_cos.shape[1], int(rotary_cos.dtype == torch.float16)
+        if rotary_dim % 16 != 0 or not 0 < rotary_dim <= d:
+            raise RuntimeError("rotary_dim must be a multiple of 16 up to head_dim")
+        if positions < capacity:
+            raise RuntimeError(f"the rotary tables must cover the {capacity} positions of the block table, got {positions}")
+    lens = torch.empty((B,), dtype=torch.int32, device=k.device)
+    _check(_lib.fal_paged_append_run(_PAGED_APPEND_ARGS.pack(
+        *block, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q is None else q_out.data_ptr(),
+        0 if rotary_cos is None else rotary_cos.data_ptr(), 0 if rotary_sin is None else rotary_sin.data_ptr(),
+        lens.data_ptr(), *q_strides, k.stride(0), k.stride(2), k.stride(1), v.stride(0), v.stride(2), v.stride(1),
+        heads_q, L, rotary_dim, int(bool(rotary_interleaved)), half, positions, _status_ptr(dev), _raw_stream(dev))))
+    return q_out, lens
+
+
+def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_scale, k_scales=None, v_scales=None,
+                    k_tail=None, v_tail=None, cache_layout="bshd"):
+    """q [B,L,Hq,d] against a paged cache that holds its L rows already -> [B,L,Hq,d]; see fal_paged_attn_run in fal_b200.h.
+
+    The workspace is allocated per call, so that calls on different streams and captured graphs do not share one.
+    """
+    _require_cuda_half("q", q, 4)
+    _addressable("q", q, 8)
+    dev = _same_device(q, k_pages, v_pages, block_table, cache_seqlens, k_scales, v_scales, k_tail, v_tail)
+    B, L, heads_q, d = q.shape
+    if B == 0 or L == 0 or heads_q == 0:
+        raise RuntimeError("q must have rows")
+    block, heads, _ = _paged_cache(k_pages, v_pages, block_table, cache_seqlens, k_scales, v_scales, k_tail, v_tail,
+                                   cache_layout, B, d)
+    if heads_q % heads != 0:
+        raise RuntimeError("H_q must be divisible by H_kv")
+    out = torch.empty((B, L, heads_q, d), dtype=torch.float16, device=q.device)
+
+    def args(workspace, nbytes):
+        return _PAGED_ATTN_ARGS.pack(*block, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(2), q.stride(1), heads_q, L,
+                                     _scale(softmax_scale), 0, workspace, nbytes, _status_ptr(dev), _raw_stream(dev))
+
+    nbytes = _lib.fal_paged_attn_workspace_bytes(args(0, 0))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _check(_lib.fal_paged_attn_run(args(ws.data_ptr(), nbytes)))
+    return out
 
 
 def decode_static(q, k_cache, v_cache, cache_seqlens, softmax_scale, out, k_new=None, v_new=None,

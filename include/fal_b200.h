@@ -364,6 +364,79 @@ FAL_API int fal_cache_append(const void* k_new, const void* v_new, void* k_cache
                int batch, int heads_kv, int rows, int capacity, int head_dim, void* stream);
 
 /*
+ * Paged key/value caches (no counterpart in the reference, whose hook's cache is written and grown by the framework around
+ * it, flash_attn_legacy/integrations.py:77-98).  Position p of entry b is row p % page_size of page
+ * block_table[b, p / page_size]; an entry holds cache_seqlens[b] positions of pages_per_entry * page_size at most.
+ *   dtype FAL_PAGED_F16: pages of fp16 rows.
+ *   dtype FAL_PAGED_S8 / FAL_PAGED_E4M3: pages of 8-bit codes, each page and KV head with a scale of its own,
+ *   k_scales / v_scales [num_pages, heads_kv] fp32: value = code * scale.  A page is written when it is full:
+ *   scale = a / m with the largest magnitude a of its rows of the head, m = 127 / 448, code = x m / a rounded to the
+ *   nearest whole number / e4m3 number, ties to even (scale NaN if the page holds an infinity or a NaN).  The rows of an
+ *   entry's last, unfinished page are fp16 rows of its tail: position p is row p % page_size of k_tail / v_tail [b].
+ * Page strides are in elements and name page, head and row; tail strides name entry, head and row.  Rows are contiguous and
+ * 16-byte aligned (strides of 8-bit pages are multiples of 16, of fp16 rows of 8).  page_size: 16, 32, 64, 128 or 256.
+ * A table entry that names no page (negative or >= num_pages) is an error only if the entry's length reaches it.
+ */
+enum fal_paged_type { FAL_PAGED_F16 = 0, FAL_PAGED_S8 = 1, FAL_PAGED_E4M3 = 2 };
+typedef struct fal_paged_cache {
+  void *k_pages, *v_pages;
+  float *k_scales, *v_scales;     /* 8-bit pages only */
+  void *k_tail, *v_tail;          /* 8-bit pages only */
+  const int32_t* block_table;     /* device, [batch, pages_per_entry], rows table_stride apart */
+  const int32_t* cache_seqlens;   /* device, [batch] */
+  fal_strides k_strides, v_strides, k_tail_strides, v_tail_strides;
+  int64_t table_stride;
+  int dtype, num_pages, page_size, pages_per_entry, batch, heads_kv, head_dim, reserved;
+} fal_paged_cache;
+
+/*
+ * Appends `rows` new rows per entry: row i of entry b goes to position cache_seqlens[b] + i.  With rotary tables
+ * (rotary_cos / rotary_sin [rotary_positions, rotary_dim / 2], fp32, or fp16 if rotary_half; rotary_positions at least
+ * pages_per_entry * page_size, rotary_dim a multiple of 16 up to head_dim) the first rotary_dim columns of k and of q
+ * are rotated by their position on the way, pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if rotary_interleaved,
+ * in 32 bits, rounded once; q_out [batch, rows, heads_q, head_dim] is contiguous.  q (and q_out, heads_q) is optional.
+ * new_seqlens[b] = cache_seqlens[b] + rows, the capacity at most.  An entry with a negative length is unused: nothing
+ * of it is stored and its length stays.  A row without a place (beyond the capacity, or without a page) is dropped, its
+ * query is 0, and *status becomes 2000.  Two entries must not share the page that new rows go to.
+ */
+typedef struct fal_paged_append_args {
+  fal_paged_cache cache;
+  const void *q, *k, *v;          /* [batch, rows, heads, head_dim] fp16 through strides (entry / head / row) */
+  void* q_out;
+  const void *rotary_cos, *rotary_sin; /* optional */
+  int32_t* new_seqlens;
+  fal_strides q_strides, k_new_strides, v_new_strides;
+  int heads_q, rows, rotary_dim, rotary_interleaved, rotary_half, rotary_positions;
+  int* status;
+  void* stream;
+} fal_paged_append_args;
+FAL_API int fal_paged_append_run(const fal_paged_append_args* args);
+
+/*
+ * Attention of `rows` query tokens per entry over a paged cache that holds their own rows already: query i of entry b
+ * sees positions up to cache_seqlens[b] - rows + i.  q [batch, rows, heads_q, head_dim] through strides (entry / head /
+ * row), o the same, contiguous.  A query that sees no position gives zeros; a position within the length that has no page
+ * counts as a row of zeros and *status becomes 3000.  workspace: fal_paged_attn_workspace_bytes (16-byte aligned, not
+ * shared by calls that overlap on the GPU).  Few rows run on a split-K pass over the pages, many on the forward kernel
+ * over the rows put in order in the workspace (as many entries and KV heads at a time as 1 GiB holds).
+ */
+typedef struct fal_paged_attn_args {
+  fal_paged_cache cache;
+  const void* q;
+  void* o;
+  fal_strides q_strides;
+  int heads_q, rows;
+  float softmax_scale;
+  int reserved;
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;
+  void* stream;
+} fal_paged_attn_args;
+FAL_API size_t fal_paged_attn_workspace_bytes(const fal_paged_attn_args* args);
+FAL_API int fal_paged_attn_run(const fal_paged_attn_args* args);
+
+/*
  * Decode for callers that must not allocate device memory (no counterpart in the
  * reference).  Some hosts of this library cannot call cudaMalloc at the point where
  * they decode: a serving loop that was handed a fixed memory budget at start-up, a

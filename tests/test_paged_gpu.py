@@ -1,0 +1,356 @@
+"""GPU: paged caches against plain models -- append with rotation bit for bit, attention over the pages to rounding."""
+import math
+
+import pytest
+import torch
+
+from paged_reference import Cache, assert_close, attention, rotate
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"fp16": torch.float16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+@pytest.fixture()
+def ext():
+    import flash_attn_legacy_cuda as m
+    m.reset_device_status()
+    yield m
+    m.reset_device_status()
+
+
+@pytest.fixture()
+def fal():
+    import flash_attn_legacy as m
+    return m
+
+
+def _rows(gen, *shape):
+    return torch.randn(*shape, generator=gen).half()
+
+
+def _tables(positions, rotary_dim):
+    half = rotary_dim // 2
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(half) / half)[None]
+    return angle.cos().float(), angle.sin().float()
+
+
+def _filled(gen, dtype, lens, page, hkv, d, extra=0, spare=2):
+    """A cache with lens[b] rows in entry b (negative: unused) and room for `extra` more."""
+    width = (max(max(lens), 0) + extra) // page + 2
+    pages = sum((max(n, 0) + extra + page - 1) // page for n in lens) + spare
+    cache = Cache(gen, dtype, pages, page, hkv, d, len(lens), width)
+    for e, n in enumerate(lens):
+        if n >= 0:
+            cache.reserve(e, n + extra)
+            cache.append(e, _rows(gen, n, hkv, d), _rows(gen, n, hkv, d))
+    return cache
+
+
+def _lens(lens):
+    return torch.tensor(lens, dtype=torch.int32).cuda()
+
+
+# Chunks that start and end on, before and behind a page border, whole pages, several pages, one row; entries that are empty,
+# that are full and that are unused; every head_dim; both rotations, all or half of the columns.
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hq,hkv,d,page,layout", [(4, 2, 128, 16, "bshd"), (2, 1, 64, 32, "bhsd"), (3, 3, 32, 64, "bshd"),
+                                                 (8, 2, 96, 16, "bhsd"), (2, 2, 256, 128, "bshd"), (5, 1, 128, 256, "bhsd")])
+@pytest.mark.parametrize("rows", [1, 5, 16, 33, 300])
+def test_append_writes_what_the_model_writes(ext, fal, dtype, hq, hkv, d, page, layout, rows):
+    gen = torch.Generator().manual_seed(d + rows)
+    lens = [0, 1, page - 1, page, 2 * page + 7, -1, 3 * page - rows % page]
+    cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d, extra=rows)
+    interleaved, rotary_dim = rows % 2 == 1, d if rows % 3 else d // 2
+    cos, sin = _tables(cache.table.shape[1] * page, rotary_dim)
+    if rows == 33:
+        cos, sin = cos.half(), sin.half()
+    got = cache.on_gpu(layout)
+    q, k, v = (_rows(gen, len(lens), rows, h, d) for h in (hq, hkv, hkv))
+    q_out, new = fal.paged_cache_append(k.cuda(), v.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens), q=q.cuda(),
+                                        rotary_cos=cos.cuda(), rotary_sin=sin.cuda(), rotary_interleaved=interleaved,
+                                        cache_layout=layout, **got)
+    for e, n in enumerate(lens):
+        if n >= 0:
+            cache.append(e, rotate(k[e], n, cos, sin, interleaved), v[e])
+            assert torch.equal(q_out[e].cpu(), rotate(q[e], n, cos, sin, interleaved))
+        else:
+            assert not q_out[e].any()
+    cache.check(got, layout)
+    assert new.tolist() == [n + rows if n >= 0 else n for n in lens]
+    assert ext.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_8_bit_pages_do_not_depend_on_how_the_rows_came_in(fal, dtype):
+    gen = torch.Generator().manual_seed(9)
+    page, hkv, d, total = 16, 2, 64, 75
+    k, v = _rows(gen, 2, total, hkv, d).cuda(), _rows(gen, 2, total, hkv, d).cuda()
+    ends = []
+    for steps in ([total], [1] * total, [3, 20, 1, 51], [16, 16, 43]):
+        cache = _filled(torch.Generator().manual_seed(4), DTYPES[dtype], [0, 0], page, hkv, d, extra=total)
+        got, lens, at = cache.on_gpu("bshd"), _lens([0, 0]), 0
+        for n in steps:
+            _, lens = fal.paged_cache_append(k[:, at:at + n], v[:, at:at + n], block_table=cache.table.cuda(), cache_seqlens=lens, **got)
+            at += n
+        left = total % page
+        got["k_tail"], got["v_tail"] = got["k_tail"][:, :left], got["v_tail"][:, :left]
+        ends.append([got[n].view(torch.uint8) for n in sorted(got) if not n.endswith("tail")] + [got["k_tail"], got["v_tail"]])
+    for other in ends[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(ends[0], other))
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_what_8_bit_pages_make_of_special_values(fal, dtype):
+    """Zeros, the smallest and the largest fp16 numbers, ties, an infinity, a NaN: one head each of one page."""
+    page, d = 16, 32
+    specials = [0.0, 2.0 ** -24, 65504.0, 1.0, math.inf, math.nan]
+    gen = torch.Generator().manual_seed(1)
+    k = (torch.rand(1, page, len(specials), d, generator=gen) - 0.5).half()
+    for h, x in enumerate(specials):
+        k[0, :, h] = 0 if x == 0 else (k[0, :, h] * (x if math.isfinite(x) else 1)).half()
+        k[0, 3, h, 5] = x
+        if x == 1.0:
+            k[0, 4, h, :8] = torch.tensor([0.5, -0.5, 63.5 / 127, 0.25, 1.3125 * 2 / 7, 0.75, -1.0, 2.0 ** -9]).half()
+    cache = Cache(gen, DTYPES[dtype], 2, page, len(specials), d, 1, 1)
+    cache.reserve(0, page)
+    got = cache.on_gpu("bshd")
+    fal.paged_cache_append(k.cuda(), k.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens([0]), **got)
+    cache.append(0, k[0], k[0])
+    for n in ("k_pages", "v_pages"):
+        assert torch.equal(got[n].cpu().view(torch.uint8), cache.tensors[n].view(torch.uint8))
+    scales, want = got["k_scales"].cpu(), cache.tensors["k_scales"]
+    assert torch.equal(scales.isnan(), want.isnan()) and torch.equal(scales.nan_to_num(), want.nan_to_num())
+    assert scales[cache.table[0, 0]].isnan().tolist() == [not math.isfinite(x) for x in specials]
+
+
+# Lengths around page, slice and split borders, empty and unused entries; one and several query tokens, up to where the
+# split-K pass hands over to the forward kernel and beyond; one, several and many query heads per KV head.
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hq,hkv,d,page,layout", [(8, 2, 128, 16, "bshd"), (16, 1, 64, 64, "bhsd"), (3, 3, 32, 32, "bshd"),
+                                                 (20, 1, 96, 16, "bhsd"), (4, 2, 256, 128, "bshd"), (6, 6, 128, 256, "bhsd")])
+@pytest.mark.parametrize("rows,lens", [(1, [1, 15, 16, 17, 255, 256, 257, 0, -1]), (1, [2049]), (1, [700, 9, 4100]),
+                                       (3, [3, 1, 16, 300, 0, -1, 35]), (16, [16, 40, 513, 7]), (130, [130, 200, 1000, 0, 64])])
+def test_attention_over_pages(ext, fal, dtype, hq, hkv, d, page, layout, rows, lens):
+    gen = torch.Generator().manual_seed(hq * d + rows)
+    cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d)
+    q = _rows(gen, len(lens), rows, hq, d)
+    scale = 1 / math.sqrt(d)
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens),
+                                          cache_layout=layout, **cache.on_gpu(layout)).cpu()
+    for e, n in enumerate(lens):
+        k, v = cache.dense(e, max(n, 0), as_half=rows * hq // hkv > 64)
+        want, mag = attention(q[e], k, v, scale)
+        assert_close(o[e], want, mag, n, v.abs().max().item() if n > 0 else 0.0)
+        first = max(rows - max(n, 0), 0)
+        assert not o[e, :first].any()  # queries before the first position
+    assert ext.device_status() == 0
+
+
+def test_a_run_of_steps_as_a_server_makes_them(ext, fal):
+    """A prompt, chunks and tokens, appended and attended to in one call each, against the whole text in 64 bits."""
+    for dtype in DTYPES:
+        gen = torch.Generator().manual_seed(11)
+        hq, hkv, d, page, total = 8, 2, 64, 32, 230
+        q, k, v = (_rows(gen, 2, total, h, d) for h in (hq, hkv, hkv))
+        cos, sin = _tables(256, d)
+        cache = _filled(gen, DTYPES[dtype], [0, 0], page, hkv, d, extra=256)
+        cache.table = cache.table[:, :8].contiguous()
+        got, lens = cache.on_gpu("bshd"), _lens([0, 0])
+        table, at = cache.table.cuda(), 0
+        for n in [150, 40, 1, 1, 5, 30, 1, 1, 1]:
+            args = [x[:, at:at + n].cuda() for x in (q, k, v)]
+            o = fal.flash_attn_with_paged_kvcache(args[0], block_table=table, cache_seqlens=lens, k=args[1], v=args[2],
+                                                  rotary_cos=cos.cuda(), rotary_sin=sin.cuda(), **got).cpu()
+            for e in range(2):
+                cache.append(e, rotate(k[e, at:at + n], at, cos, sin, False), v[e, at:at + n])
+                kd, vd = cache.dense(e, at + n, as_half=n * hq // hkv > 64)
+                want, mag = attention(rotate(q[e, at:at + n], at, cos, sin, False), kd, vd, 1 / math.sqrt(d))
+                assert_close(o[e], want, mag, at + n, vd.abs().max().item())
+            at += n
+            lens = lens + n
+        cache.check(got, "bshd")
+        assert ext.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_captured_steps_replayed_side_by_side(fal, dtype):
+    """Two graphs of one stream, replayed on two streams at once, lengths moved on inside: each as the same steps made eagerly."""
+    gen = torch.Generator().manual_seed(2)
+    hq, hkv, d, page, steps = 8, 2, 128, 16, 20
+    cos, sin = (t.cuda() for t in _tables(64 * page, d))
+    sides, graphs = [], []
+    for i in range(2):
+        lens = [500 + i, 9, 30]
+        cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d, extra=steps + 1)
+        s = {"got": cache.on_gpu("bshd"), "table": cache.table.cuda(), "lens": _lens(lens),
+             "in": [_rows(gen, 3, 1, h, d).cuda() for h in (hq, hkv, hkv)]}
+        s["eager"] = {"got": {n: t.clone() for n, t in s["got"].items()}, "lens": s["lens"].clone()}
+        sides.append(s)
+
+    def step(s, got, lens):
+        q, k, v = s["in"]
+        o = fal.flash_attn_with_paged_kvcache(q, block_table=s["table"], cache_seqlens=lens, k=k, v=v, rotary_cos=cos,
+                                              rotary_sin=sin, **got)
+        lens += 1
+        return o
+
+    want = []
+    for s in sides:
+        for _ in range(steps):
+            o = step(s, s["eager"]["got"], s["eager"]["lens"])
+        want.append(o)
+    capture = torch.cuda.Stream()
+    for s in sides:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=capture):
+            s["out"] = step(s, s["got"], s["lens"])
+        graphs.append(g)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(steps):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for s, o in zip(sides, want):
+        assert torch.equal(s["out"], o) and torch.equal(s["lens"], s["eager"]["lens"])
+        for n, t in s["got"].items():
+            assert torch.equal(t.view(torch.uint8), s["eager"]["got"][n].view(torch.uint8)), n
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_views_and_another_stream(fal, dtype):
+    """q, k, v as slices of one projection, a table that is part of a larger one, pages of one allocation, off the default stream."""
+    gen = torch.Generator().manual_seed(3)
+    hq, hkv, d, page, rows, lens = 4, 2, 64, 16, 6, [20, 45]
+    cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d, extra=rows)
+    plain = cache.on_gpu("bshd")
+    views = {n: t.clone() for n, t in plain.items()}  # (the append moves scales and tails on)
+    both = torch.stack([plain["k_pages"].view(torch.uint8), plain["v_pages"].view(torch.uint8)], dim=1).contiguous()
+    views["k_pages"], views["v_pages"] = both[:, 0].view(DTYPES[dtype]), both[:, 1].view(DTYPES[dtype])
+    x = _rows(gen, 2, rows, hq + 2 * hkv, d).cuda()
+    q, k, v = x[:, :, :hq], x[:, :, hq:hq + hkv], x[:, :, hq + hkv:]
+    wide = torch.full((4, cache.table.shape[1] + 5), -7, dtype=torch.int32).cuda()
+    wide[1:3, 2:-3] = cache.table.cuda()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        o = fal.flash_attn_with_paged_kvcache(q, block_table=wide[1:3, 2:-3], cache_seqlens=_lens(lens), k=k, v=v, **views)
+    stream.synchronize()
+    want = fal.flash_attn_with_paged_kvcache(q.contiguous(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens).long(),
+                                             k=k.contiguous(), v=v.contiguous(), **plain)
+    assert torch.equal(o, want)
+    for n in plain:
+        assert torch.equal(views[n].contiguous().view(torch.uint8), plain[n].view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_rows_without_a_place_are_dropped_and_reported(ext, fal, dtype):
+    """Entry 0 runs into the end of its table, entry 1 into a table entry that names no page, entry 2 into a page number that is too large."""
+    gen = torch.Generator().manual_seed(5)
+    hkv, d, page, rows = 2, 64, 16, 20
+    cache = _filled(gen, DTYPES[dtype], [40, 10, 10, 3], page, hkv, d, extra=rows)
+    cache.table = cache.table[:, :3].contiguous()  # 48 positions
+    cache.table[1, 1], cache.table[2, 1] = -1, 10 ** 6
+    got = cache.on_gpu("bshd")
+    k, v, q = (_rows(gen, 4, rows, hkv, d) for _ in range(3))
+    out, lens = fal.paged_cache_append(k.cuda(), v.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens([40, 10, 10, 3]), q=q.cuda(), **got)
+    assert ext.device_status() == 2000
+    assert lens.tolist() == [48, 30, 30, 23]
+    assert not out[0, 8:].any() and torch.equal(out[0, :8].cpu(), q[0, :8]) and torch.equal(out[1:].cpu(), q[1:])
+    cache.append(0, k[0, :8], v[0, :8])
+    cache.table[2, 1] = -1
+    for e in (1, 2, 3):
+        cache.append(e, k[e], v[e])
+    cache.check(got, "bshd")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_position_without_a_page_counts_as_zeros(ext, fal, dtype, rows):
+    gen = torch.Generator().manual_seed(6)
+    hq, hkv, d, page, lens = 4, 2, 64, 16, [100, 70]
+    cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d)
+    q = _rows(gen, 2, rows, hq, d)
+    table = cache.table.clone()
+    table[0, 2], table[1, 0] = -1, 4096
+    args = dict(cache_seqlens=_lens(lens), **cache.on_gpu("bshd"))
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=table.cuda(), **args).cpu()
+    assert ext.device_status() == 3000
+    for e, (n, gone) in enumerate(zip(lens, (2, 0))):
+        k, v = cache.dense(e, n, as_half=rows * hq // hkv > 64)
+        k[gone * page:(gone + 1) * page] = 0
+        v[gone * page:(gone + 1) * page] = 0
+        want, mag = attention(q[e], k, v, 1 / math.sqrt(d))
+        assert_close(o[e], want, mag, n, v.abs().max().item())
+
+
+def test_a_page_with_a_nan_shows_in_what_sees_it_only(fal):
+    gen = torch.Generator().manual_seed(7)
+    cache = _filled(gen, torch.int8, [64, 64], 16, 2, 64)
+    got = cache.on_gpu("bshd")
+    got["v_scales"][cache.table[1, 2].item(), 1] = math.nan
+    o = fal.flash_attn_with_paged_kvcache(_rows(gen, 2, 1, 4, 64).cuda(), block_table=cache.table.cuda(),
+                                          cache_seqlens=_lens([64, 64]), **got)
+    assert o.isnan().any(dim=-1)[:, 0].tolist() == [[False] * 4, [False, False, True, True]]
+
+
+def test_positions_beyond_32_bits_of_elements(fal):
+    """Pages whose elements lie more than 2^31 from the pool's start."""
+    gen = torch.Generator().manual_seed(8)
+    hkv, d, page = 8, 128, 256
+    pages = 2 ** 31 // (page * hkv * d) + 4
+    for dtype in (torch.float16, torch.int8):
+        small = _filled(gen, dtype, [600], page, hkv, d, extra=8, spare=0)
+        got = small.on_gpu("bshd")
+        large = {n: t.clone() for n, t in got.items()}
+        for n in ("k_pages", "v_pages"):
+            large[n] = torch.zeros((pages, page, hkv, d), dtype=dtype, device="cuda")
+            large[n][-3:] = got[n]
+            if dtype == torch.int8:
+                scales = torch.zeros((pages, hkv), device="cuda")
+                scales[-3:] = got[n[0] + "_scales"]
+                large[n[0] + "_scales"] = scales
+        q, k, v = (_rows(gen, 1, 3, h, d).cuda() for h in (16, hkv, hkv))
+        for rows in (3, 1):
+            args = dict(cache_seqlens=_lens([600]), k=k[:, :rows], v=v[:, :rows])
+            a = fal.flash_attn_with_paged_kvcache(q[:, :rows], block_table=small.table.cuda(), **args, **got)
+            far = torch.where(small.table >= 0, small.table + pages - 3, small.table).cuda()
+            b = fal.flash_attn_with_paged_kvcache(q[:, :rows], block_table=far, **args, **large)
+            assert torch.equal(a, b) and torch.equal(large["k_pages"][-3:].view(torch.uint8), got["k_pages"].view(torch.uint8))
+        del large
+
+
+def test_refusals(fal):
+    gen = torch.Generator().manual_seed(10)
+    good = _filled(gen, torch.int8, [20, 30], 16, 2, 64, extra=4)
+    got = good.on_gpu("bshd")
+    q, k, v = (_rows(gen, 2, 1, h, 64).cuda() for h in (4, 2, 2))
+    base = dict(block_table=good.table.cuda(), cache_seqlens=_lens([20, 30]), **got)
+    cos, sin = (t.cuda() for t in _tables(good.table.shape[1] * 16, 64))
+
+    def attend(**change):
+        return fal.flash_attn_with_paged_kvcache(**{"q": q, **base, **change})
+
+    attend()
+    attend(k=k, v=v, rotary_cos=cos, rotary_sin=sin)
+    wrong = [dict(k_tail=None), dict(k_scales=None), dict(k_scales=got["k_scales"].half()), dict(v_scales=got["v_scales"][:, :1]),
+             dict(k_tail=got["k_tail"][:1]), dict(v_tail=got["v_tail"].float()), dict(k_pages=got["k_pages"].half()),
+             dict(k_pages=got["k_pages"].view(torch.uint8), v_pages=got["v_pages"].view(torch.uint8)),
+             dict(v_pages=got["v_pages"][:-1]), dict(k_pages=got["k_pages"][:, :8], v_pages=got["v_pages"][:, :8]),
+             dict(block_table=base["block_table"][:1]), dict(block_table=base["block_table"].t()), dict(cache_seqlens=_lens([1, 2, 3])),
+             dict(q=q[:, :, :3]), dict(q=q[..., :32]), dict(softmax_scale=-1.0), dict(block_table=base["block_table"].cpu()),
+             dict(k=k, v=v[:, :, :1]), dict(k=k, v=v, rotary_cos=cos), dict(k=k, v=v, rotary_cos=cos[:20], rotary_sin=sin[:20]),
+             dict(k=k, v=v, rotary_cos=cos[:, :12].contiguous(), rotary_sin=sin[:, :12].contiguous()),
+             dict(k=k, v=v, rotary_cos=cos.double(), rotary_sin=sin.double()), dict(q=q.clone().requires_grad_()),
+             dict(k=k.clone().requires_grad_(), v=v), dict(q=q[:, :0]), dict(k=got["k_tail"][:, :1], v=v)]
+    for change in wrong:
+        with pytest.raises(RuntimeError):
+            attend(**change)
+    for change in (dict(q=q.float()), dict(rotary_cos=cos, rotary_sin=sin), dict(k=k), dict(v=v), dict(k=k.float(), v=v.float())):
+        with pytest.raises(AssertionError):
+            attend(**change)
+    with pytest.raises(ValueError):
+        attend(cache_layout="bhnd")
+    with torch.no_grad():
+        attend(q=q.clone().requires_grad_())
