@@ -38,6 +38,9 @@ struct Calls {
   int (*fwd_run)(const fal_fwd_args*);
   int (*decode_run)(const fal_decode_args*);
   size_t (*decode_workspace_bytes)(int, int, int, int);
+  int (*paged_append_run)(const fal_paged_append_args*);
+  int (*paged_attn_run)(const fal_paged_attn_args*);
+  size_t (*paged_attn_workspace_bytes)(const fal_paged_attn_args*);
   PyObject* workspaces;       // {(device, stream): uint8 tensor}
   size_t workspace_min;
   int* status[kMaxDevices];   // device status words, null until the binding has made one
@@ -236,6 +239,245 @@ PyObject* calls_decode(PyObject* self_obj, PyObject* const* args, Py_ssize_t nar
   END_HANDLE_TH_ERRORS
 }
 
+// ---- paged caches ----
+// The arguments of both calls behind q, k and v, in the order of the Python functions.
+enum PagedArg { kPages, kVPages, kTable, kLens, kCos, kSin, kInterleaved, kKScales, kVScales, kKTail, kVTail, kLayout, kPagedArgs };
+
+struct PagedTensors {
+  const at::Tensor *kp, *vp, *table, *lens, *ks = nullptr, *vs = nullptr, *kt = nullptr, *vt = nullptr;
+  const at::Tensor *cos = nullptr, *sin = nullptr;
+  int rotary_dim = 0;
+  bool interleaved = false;
+};
+
+bool addressable(const at::Tensor& t, int64_t per16) {
+  if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.stride(i) % per16 != 0 || (t.stride(i) <= 0 && t.size(i) != 1)) return false;
+  return true;
+}
+
+const void* storage(const at::Tensor* t) { return t == nullptr ? nullptr : t->storage().unsafeGetStorageImpl()->data(); }
+
+// The cache of a call for `batch` entries of `head_dim` columns: what the binding's checks accept, as its block.
+bool paged_cache(PyObject* const* args, int64_t batch, int64_t head_dim, PagedTensors& x, fal_paged_cache& c) {
+  if (!THPVariable_CheckExact(args[kPages])) return false;
+  const auto type = THPVariable_Unpack(args[kPages]).scalar_type();
+  c.dtype = type == at::kHalf ? FAL_PAGED_F16 : type == at::kChar ? FAL_PAGED_S8 : FAL_PAGED_E4M3;
+  if (c.dtype == FAL_PAGED_E4M3 && type != at::kFloat8_e4m3fn) return false;
+  x.kp = plain(args[kPages], type, 4);
+  x.vp = plain(args[kVPages], type, 4);
+  x.table = plain(args[kTable], at::kInt, 2);
+  x.lens = plain(args[kLens], at::kInt, 1);
+  const int layout = layout_of(args[kLayout], "bshd", "bhsd");
+  if (!x.kp || !x.vp || !x.table || !x.lens || layout < 0 || x.kp->sizes() != x.vp->sizes()) return false;
+  const int seq = layout == 0 ? 1 : 2, head = 3 - seq;
+  const at::Tensor &kp = *x.kp, &vp = *x.vp;
+  const int64_t pages = kp.size(0), page = kp.size(seq), heads = kp.size(head), width = x.table->size(1);
+  if (kp.size(3) != head_dim || !supported_head_dim(head_dim) || x.table->size(0) != batch || x.lens->size(0) != batch ||
+      !fits_int({pages, page, heads, width, batch}) || width * page > (1 << 30))
+    return false;
+  const int64_t per16 = c.dtype == FAL_PAGED_F16 ? 8 : 16;
+  if (!addressable(kp, per16) || !addressable(vp, per16) || storage(x.kp) == storage(x.vp)) return false;
+  if (c.dtype == FAL_PAGED_F16) {
+    for (int i : {kKScales, kVScales, kKTail, kVTail})
+      if (args[i] != Py_None) return false;
+  } else {
+    x.ks = plain(args[kKScales], at::kFloat, 2);
+    x.vs = plain(args[kVScales], at::kFloat, 2);
+    x.kt = plain(args[kKTail], at::kHalf, 4);
+    x.vt = plain(args[kVTail], at::kHalf, 4);
+    if (!x.ks || !x.vs || !x.kt || !x.vt) return false;
+    for (const at::Tensor* s : {x.ks, x.vs})
+      if (s->size(0) != pages || s->size(1) != heads || !s->is_contiguous()) return false;
+    for (const at::Tensor* s : {x.kt, x.vt})
+      if (s->size(0) != batch || s->size(1) != kp.size(1) || s->size(2) != kp.size(2) || s->size(3) != head_dim || !addressable(*s, 8))
+        return false;
+    if (storage(x.kt) == storage(x.vt)) return false;
+    c.k_scales = x.ks->mutable_data_ptr<float>();
+    c.v_scales = x.vs->mutable_data_ptr<float>();
+    c.k_tail = x.kt->data_ptr();
+    c.v_tail = x.vt->data_ptr();
+    c.k_tail_strides = {x.kt->stride(0), x.kt->stride(head), x.kt->stride(seq)};
+    c.v_tail_strides = {x.vt->stride(0), x.vt->stride(head), x.vt->stride(seq)};
+  }
+  for (const at::Tensor* s : {x.kp, x.vp, x.kt, x.vt, x.ks, x.vs})
+    if (s != nullptr && tracked(*s)) return false;
+  if (args[kCos] != Py_None || args[kSin] != Py_None) {
+    if (!THPVariable_CheckExact(args[kCos]) || !PyBool_Check(args[kInterleaved])) return false;
+    const auto table_type = THPVariable_Unpack(args[kCos]).scalar_type();
+    if (table_type != at::kFloat && table_type != at::kHalf) return false;
+    x.cos = plain(args[kCos], table_type, 2);
+    x.sin = plain(args[kSin], table_type, 2);
+    if (!x.cos || !x.sin || !x.cos->is_contiguous() || !x.sin->is_contiguous() || x.cos->sizes() != x.sin->sizes() ||
+        !fits_int({x.cos->size(0)}) || x.cos->size(1) > head_dim || x.cos->size(0) < width * page)
+      return false;
+    x.rotary_dim = static_cast<int>(2 * x.cos->size(1));
+    x.interleaved = args[kInterleaved] == Py_True;
+  }
+  const auto dev = kp.get_device();
+  for (const at::Tensor* s : {x.vp, x.table, x.lens, x.ks, x.vs, x.kt, x.vt, x.cos, x.sin})
+    if (s != nullptr && s->get_device() != dev) return false;
+  c.k_pages = kp.data_ptr();
+  c.v_pages = vp.data_ptr();
+  c.block_table = x.table->const_data_ptr<int32_t>();
+  c.cache_seqlens = x.lens->const_data_ptr<int32_t>();
+  c.k_strides = {kp.stride(0), kp.stride(head), kp.stride(seq)};
+  c.v_strides = {vp.stride(0), vp.stride(head), vp.stride(seq)};
+  c.table_stride = x.table->stride(0);
+  c.num_pages = static_cast<int>(pages);
+  c.page_size = static_cast<int>(page);
+  c.pages_per_entry = static_cast<int>(width);
+  c.batch = static_cast<int>(batch);
+  c.heads_kv = static_cast<int>(heads);
+  c.head_dim = static_cast<int>(head_dim);
+  return true;
+}
+
+// [B,L,H,d] fp16 of the calls' new tokens, in no memory of the cache.
+const at::Tensor* paged_rows(PyObject* obj, const PagedTensors& x) {
+  const at::Tensor* t = plain(obj, at::kHalf, 4);
+  if (t == nullptr || !addressable(*t, 8) || tracked(*t) || t->get_device() != x.kp->get_device() ||
+      !fits_int({t->size(0), t->size(1), t->size(2)}))
+    return nullptr;
+  for (const at::Tensor* s : {x.kp, x.vp, x.kt, x.vt})
+    if (s != nullptr && storage(s) == storage(t)) return nullptr;
+  return t;
+}
+
+fal_strides row_strides(const at::Tensor& t) { return {t.stride(0), t.stride(2), t.stride(1)}; }
+
+// Fills the append's block but for its outputs; q may be null.
+bool paged_append_block(const PagedTensors& x, const at::Tensor* q, const at::Tensor& k, const at::Tensor& v, fal_paged_append_args& a) {
+  if (k.sizes() != v.sizes() || k.size(0) != a.cache.batch || k.size(2) != a.cache.heads_kv || k.size(3) != a.cache.head_dim) return false;
+  if (q != nullptr) {
+    if (q->size(0) != k.size(0) || q->size(1) != k.size(1) || q->size(3) != k.size(3)) return false;
+    a.q = q->const_data_ptr();
+    a.q_strides = row_strides(*q);
+    a.heads_q = static_cast<int>(q->size(2));
+  }
+  a.k = k.const_data_ptr();
+  a.v = v.const_data_ptr();
+  a.k_new_strides = row_strides(k);
+  a.v_new_strides = row_strides(v);
+  a.rows = static_cast<int>(k.size(1));
+  if (x.cos != nullptr) {
+    a.rotary_cos = x.cos->const_data_ptr();
+    a.rotary_sin = x.sin->const_data_ptr();
+    a.rotary_dim = x.rotary_dim;
+    a.rotary_interleaved = x.interleaved ? 1 : 0;
+    a.rotary_half = x.cos->scalar_type() == at::kHalf ? 1 : 0;
+    a.rotary_positions = static_cast<int>(x.cos->size(0));
+  }
+  return true;
+}
+
+void paged_written(const PagedTensors& x) {
+  for (const at::Tensor* t : {x.kp, x.vp, x.ks, x.vs, x.kt, x.vt})
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+// paged_append(k, v, <paged arguments>, q) -> (rotated q or None, new lengths), or None
+PyObject* calls_paged_append(PyObject* self_obj, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Calls* self = reinterpret_cast<Calls*>(self_obj);
+  if (nargs != 3 + kPagedArgs || !ordinary_call()) Py_RETURN_NONE;
+  const at::Tensor* k = plain(args[0], at::kHalf, 4);
+  PagedTensors x;
+  fal_paged_append_args a{};
+  if (k == nullptr || !paged_cache(args + 2, k->size(0), k->size(3), x, a.cache)) Py_RETURN_NONE;
+  k = paged_rows(args[0], x);
+  const at::Tensor* v = paged_rows(args[1], x);
+  const at::Tensor* q = nullptr;
+  if (args[2 + kPagedArgs] != Py_None && (q = paged_rows(args[2 + kPagedArgs], x)) == nullptr) Py_RETURN_NONE;
+  if (!k || !v || !paged_append_block(x, q, *k, *v, a)) Py_RETURN_NONE;
+  const auto dev = k->get_device();
+  if (dev >= kMaxDevices || self->status[dev] == nullptr || c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  a.status = self->status[dev];
+  at::Tensor q_out, lens;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (q != nullptr) {
+      q_out = at::empty(q->sizes(), q->options());
+      a.q_out = q_out.data_ptr();
+    }
+    lens = at::empty({a.cache.batch}, x.lens->options());
+    a.new_seqlens = lens.mutable_data_ptr<int32_t>();
+    a.stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+    rc = self->paged_append_run(&a);
+    if (rc == 0) paged_written(x);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  THPObjectPtr first(q != nullptr ? THPVariable_Wrap(std::move(q_out)) : Py_NewRef(Py_None));
+  THPObjectPtr second(THPVariable_Wrap(std::move(lens)));
+  if (!first || !second) return nullptr;
+  return PyTuple_Pack(2, first.get(), second.get());
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attend(q, k, v, <paged arguments>, softmax_scale) -> out [B,L,Hq,d], or None; k, v: None, or appended first
+PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Calls* self = reinterpret_cast<Calls*>(self_obj);
+  if (nargs != 4 + kPagedArgs || !ordinary_call()) Py_RETURN_NONE;
+  const at::Tensor* q = plain(args[0], at::kHalf, 4);
+  PagedTensors x;
+  fal_paged_append_args a{};
+  fal_paged_attn_args r{};
+  if (q == nullptr || !paged_cache(args + 3, q->size(0), q->size(3), x, a.cache)) Py_RETURN_NONE;
+  q = paged_rows(args[0], x);
+  if (q == nullptr || q->size(2) % a.cache.heads_kv != 0 || !scale_of(args[3 + kPagedArgs], q->size(3), r.softmax_scale)) Py_RETURN_NONE;
+  const bool appends = args[1] != Py_None;
+  if (appends) {
+    const at::Tensor* k = paged_rows(args[1], x);
+    const at::Tensor* v = paged_rows(args[2], x);
+    if (!k || !v || k->size(1) != q->size(1) || !paged_append_block(x, x.cos != nullptr ? q : nullptr, *k, *v, a)) Py_RETURN_NONE;
+  } else if (args[2] != Py_None || x.cos != nullptr) {
+    Py_RETURN_NONE;
+  }
+  const auto dev = q->get_device();
+  if (dev >= kMaxDevices || self->status[dev] == nullptr || c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  r.cache = a.cache;
+  r.heads_q = static_cast<int>(q->size(2));
+  r.rows = static_cast<int>(q->size(1));
+  r.q = q->const_data_ptr();
+  r.q_strides = row_strides(*q);
+  a.status = r.status = self->status[dev];
+  at::Tensor o;
+  int rc = 0;
+  {
+    pybind11::gil_scoped_release no_gil;
+    at::Tensor lens, turned;
+    a.stream = r.stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+    o = at::empty(q->sizes(), q->options());
+    r.o = o.data_ptr();
+    r.workspace_bytes = self->paged_attn_workspace_bytes(&r);
+    const at::Tensor ws = at::empty({static_cast<int64_t>(r.workspace_bytes)}, q->options().dtype(at::kByte));
+    r.workspace = ws.data_ptr();
+    // (a call that the library refuses must not have appended anything: the general way makes it again)
+    if (r.workspace_bytes == 0) rc = FAL_ERR_INVALID_ARGUMENT;
+    if (rc == 0 && appends) {
+      lens = at::empty({a.cache.batch}, x.lens->options());
+      a.new_seqlens = lens.mutable_data_ptr<int32_t>();
+      if (x.cos != nullptr) {
+        turned = at::empty(q->sizes(), q->options());
+        a.q_out = turned.data_ptr();
+        r.q = a.q_out;
+        r.q_strides = row_strides(turned);
+      }
+      r.cache.cache_seqlens = a.new_seqlens;
+      if (!(r.softmax_scale > 0.f)) rc = FAL_ERR_INVALID_ARGUMENT;
+      else rc = self->paged_append_run(&a);
+      if (rc == 0) paged_written(x);
+    }
+    if (rc == 0) rc = self->paged_attn_run(&r);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_status(device index, address of its status word)
 PyObject* calls_set_status(PyObject* self_obj, PyObject* const* args, Py_ssize_t nargs) {
   const long dev = nargs == 2 ? PyLong_AsLong(args[0]) : -1;
@@ -245,16 +487,22 @@ PyObject* calls_set_status(PyObject* self_obj, PyObject* const* args, Py_ssize_t
   Py_RETURN_NONE;
 }
 
-// Calls(address of fal_fwd_args_run, of fal_decode_args_run, of fal_decode_workspace_bytes, workspaces, least bytes)
+// Calls(address of fal_fwd_args_run, of fal_decode_args_run, of fal_decode_workspace_bytes, workspaces, least bytes,
+//       address of fal_paged_append_run, of fal_paged_attn_run, of fal_paged_attn_workspace_bytes)
 PyObject* calls_new(PyTypeObject* type, PyObject* args, PyObject*) {
-  unsigned long long fwd, dec, bytes_fn, least;
+  unsigned long long fwd, dec, bytes_fn, least, paged_append, paged_attn, paged_bytes;
   PyObject* workspaces;
-  if (!PyArg_ParseTuple(args, "KKKO!K", &fwd, &dec, &bytes_fn, &PyDict_Type, &workspaces, &least)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKO!KKKK", &fwd, &dec, &bytes_fn, &PyDict_Type, &workspaces, &least, &paged_append, &paged_attn,
+                        &paged_bytes))
+    return nullptr;
   Calls* self = reinterpret_cast<Calls*>(type->tp_alloc(type, 0));  // (zeroed)
   if (self == nullptr) return nullptr;
   self->fwd_run = reinterpret_cast<decltype(self->fwd_run)>(fwd);
   self->decode_run = reinterpret_cast<decltype(self->decode_run)>(dec);
   self->decode_workspace_bytes = reinterpret_cast<decltype(self->decode_workspace_bytes)>(bytes_fn);
+  self->paged_append_run = reinterpret_cast<decltype(self->paged_append_run)>(paged_append);
+  self->paged_attn_run = reinterpret_cast<decltype(self->paged_attn_run)>(paged_attn);
+  self->paged_attn_workspace_bytes = reinterpret_cast<decltype(self->paged_attn_workspace_bytes)>(paged_bytes);
   self->workspaces = Py_NewRef(workspaces);
   self->workspace_min = least;
   return reinterpret_cast<PyObject*>(self);
@@ -273,6 +521,8 @@ PyCFunction fastcall(F f) {
 PyMethodDef calls_methods[] = {
     {"forward", fastcall(calls_forward), METH_FASTCALL, "flash_attention without gradients, or None"},
     {"decode", fastcall(calls_decode), METH_FASTCALL, "one decode step, or None"},
+    {"paged_append", fastcall(calls_paged_append), METH_FASTCALL, "rows into a paged cache, or None"},
+    {"paged_attend", fastcall(calls_paged_attend), METH_FASTCALL, "attention over a paged cache, rows appended first, or None"},
     {"set_status", fastcall(calls_set_status), METH_FASTCALL, "address of a device's status word"},
     {nullptr, nullptr, 0, nullptr}};
 
@@ -294,7 +544,9 @@ PyMODINIT_FUNC PyInit__fal_host() {
   // sizes of the argument blocks it was compiled with
   if (PyModule_AddObjectRef(m, "Calls", reinterpret_cast<PyObject*>(&calls_type)) < 0 ||
       PyModule_AddIntConstant(m, "FWD_ARGS_BYTES", sizeof(fal_fwd_args)) < 0 ||
-      PyModule_AddIntConstant(m, "DECODE_ARGS_BYTES", sizeof(fal_decode_args)) < 0) {
+      PyModule_AddIntConstant(m, "DECODE_ARGS_BYTES", sizeof(fal_decode_args)) < 0 ||
+      PyModule_AddIntConstant(m, "PAGED_APPEND_ARGS_BYTES", sizeof(fal_paged_append_args)) < 0 ||
+      PyModule_AddIntConstant(m, "PAGED_ATTN_ARGS_BYTES", sizeof(fal_paged_attn_args)) < 0) {
     Py_DECREF(m);
     return nullptr;
   }

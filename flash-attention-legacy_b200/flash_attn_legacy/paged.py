@@ -64,6 +64,11 @@ def paged_cache_append(
     page) are dropped, their queries become 0, and the device status word 2000.  Pages that new rows go to must not be
     shared between entries.
     """
+    # the ordinary call in one native function; None: any other
+    out = flash_attn_legacy_cuda.paged_append_plain(k, v, k_pages, v_pages, block_table, cache_seqlens, rotary_cos, rotary_sin,
+                                                    rotary_interleaved, k_scales, v_scales, k_tail, v_tail, cache_layout, q)
+    if out is not None:
+        return out
     assert k.dim() == 4 and v.dim() == 4, "k and v must be [B, L, H_kv, d]"
     assert k.dtype == torch.float16 and v.dtype == torch.float16, f"k and v must be float16, got {k.dtype}, {v.dtype}"
     assert q is None or q.dtype == torch.float16, f"Q must be float16, got {q.dtype}"
@@ -109,6 +114,11 @@ def flash_attn_with_paged_kvcache(
     more run on the forward kernel, over the pages put in order in a workspace as large as the block table allows for (up to
     1 GiB at a time): pass a view of the table's first columns where entries are much shorter than it.
     """
+    out = flash_attn_legacy_cuda.paged_attend_plain(q, k, v, k_pages, v_pages, block_table, cache_seqlens, rotary_cos, rotary_sin,
+                                                    rotary_interleaved, k_scales, v_scales, k_tail, v_tail, cache_layout,
+                                                    softmax_scale)
+    if out is not None:
+        return out
     assert q.dim() == 4, "q must be [B, L, H_q, d]"
     assert q.dtype == torch.float16, f"Q must be float16, got {q.dtype}"
     d = q.shape[-1]
@@ -116,14 +126,17 @@ def flash_attn_with_paged_kvcache(
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(d)
     block_table, cache_seqlens = block_table.to(torch.int32), cache_seqlens.to(torch.int32)
+    q, append = _kernel_ready(q), None
     if k is not None:
         assert v is not None and q.shape[:2] == k.shape[:2], "k, v must be [B, L, H_kv, d]"
-        turned, cache_seqlens = paged_cache_append(
-            k, v, k_pages, v_pages, block_table, cache_seqlens, q if rotary_cos is not None else None, rotary_cos, rotary_sin,
-            rotary_interleaved, k_scales, v_scales, k_tail, v_tail, cache_layout)
-        q = turned if turned is not None else q
+
+        def append():
+            turned, lens = paged_cache_append(
+                k, v, k_pages, v_pages, block_table, cache_seqlens, q if rotary_cos is not None else None, rotary_cos, rotary_sin,
+                rotary_interleaved, k_scales, v_scales, k_tail, v_tail, cache_layout)
+            return turned if turned is not None else q, lens
     else:
         assert v is None and rotary_cos is None and rotary_sin is None, "v and the rotary tables go with k"
-        _inference_only(q, k_pages, v_pages, k_tail, v_tail)
-    return flash_attn_legacy_cuda.paged_attention(_kernel_ready(q), k_pages, v_pages, block_table, cache_seqlens,
-                                                  softmax_scale, k_scales, v_scales, k_tail, v_tail, cache_layout)
+    _inference_only(q, k_pages, v_pages, k_tail, v_tail)
+    return flash_attn_legacy_cuda.paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_scale, k_scales,
+                                                  v_scales, k_tail, v_tail, cache_layout, append)

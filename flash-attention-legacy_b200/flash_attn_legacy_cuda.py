@@ -147,10 +147,12 @@ def _load_host():
         module = _load("_fal_host", importlib.machinery.ExtensionFileLoader, path)
     except ImportError:
         return None
-    if (module.FWD_ARGS_BYTES, module.DECODE_ARGS_BYTES) != (_FWD_ARGS.size, _DECODE_ARGS.size):
+    sizes = [getattr(module, n, 0) for n in ("FWD_ARGS_BYTES", "DECODE_ARGS_BYTES", "PAGED_APPEND_ARGS_BYTES", "PAGED_ATTN_ARGS_BYTES")]
+    if sizes != [_FWD_ARGS.size, _DECODE_ARGS.size, _PAGED_APPEND_ARGS.size, _PAGED_ATTN_ARGS.size]:
         return None  # built with another header than this binding is written for
-    address = [ctypes.cast(f, _vp).value for f in (_fwd_run, _decode_run, _lib.fal_decode_workspace_bytes)]
-    return module.Calls(*address, _decode_ws, _DECODE_WS_MIN)
+    address = [ctypes.cast(f, _vp).value for f in (_fwd_run, _decode_run, _lib.fal_decode_workspace_bytes, _lib.fal_paged_append_run,
+                                                   _lib.fal_paged_attn_run, _lib.fal_paged_attn_workspace_bytes)]
+    return module.Calls(*address[:3], _decode_ws, _DECODE_WS_MIN, *address[3:])
 
 
 def _general(*args):
@@ -165,6 +167,8 @@ _host = _load_host()
 # Each answers None for whatever is not an ordinary call: make it through the functions below.
 forward_plain = _general if _host is None else _host.forward
 decode_plain = _general if _host is None else _host.decode
+paged_append_plain = _general if _host is None else _host.paged_append
+paged_attend_plain = _general if _host is None else _host.paged_attend
 
 KERNEL_FWD, KERNEL_BWD, KERNEL_DECODE_SPLITK = 0, 1, 2
 
@@ -873,9 +877,11 @@ def paged_append(k, v, k_pages, v_pages, block_table, cache_seqlens, q=None, rot
 
 
 def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_scale, k_scales=None, v_scales=None,
-                    k_tail=None, v_tail=None, cache_layout="bshd"):
+                    k_tail=None, v_tail=None, cache_layout="bshd", append=None):
     """q [B,L,Hq,d] against a paged cache that holds its L rows already -> [B,L,Hq,d]; see fal_paged_attn_run in fal_b200.h.
 
+    `append`, if given, is called once everything else has been checked, and returns the queries (of q's shape) and the
+    lengths to go on with.
     The workspace is allocated per call, so that calls on different streams and captured graphs do not share one.
     """
     _require_cuda_half("q", q, 4)
@@ -888,14 +894,22 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_sca
                                    cache_layout, B, d)
     if heads_q % heads != 0:
         raise RuntimeError("H_q must be divisible by H_kv")
+    softmax_scale = _scale(softmax_scale)
+    if not softmax_scale > 0:
+        raise RuntimeError("softmax_scale must be positive")
+    if B * L * heads_q >= 1 << 31:
+        raise RuntimeError("q has too many rows")
     out = torch.empty((B, L, heads_q, d), dtype=torch.float16, device=q.device)
 
     def args(workspace, nbytes):
         return _PAGED_ATTN_ARGS.pack(*block, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(2), q.stride(1), heads_q, L,
-                                     _scale(softmax_scale), 0, workspace, nbytes, _status_ptr(dev), _raw_stream(dev))
+                                     softmax_scale, 0, workspace, nbytes, _status_ptr(dev), _raw_stream(dev))
 
     nbytes = _lib.fal_paged_attn_workspace_bytes(args(0, 0))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    if append is not None:
+        q, cache_seqlens = append()
+        block = (*block[:7], cache_seqlens.data_ptr(), *block[8:])
     _check(_lib.fal_paged_attn_run(args(ws.data_ptr(), nbytes)))
     return out
 

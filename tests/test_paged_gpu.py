@@ -354,3 +354,40 @@ def test_refusals(fal):
         attend(cache_layout="bhnd")
     with torch.no_grad():
         attend(q=q.clone().requires_grad_())
+    # a refused call has not appended anything
+    before = {n: t.clone() for n, t in got.items()}
+    for change in (dict(softmax_scale=0.0), dict(q=q[:, :, :3].contiguous())):
+        with pytest.raises(RuntimeError):
+            attend(k=k, v=v, **change)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.view(torch.uint8), before[n].view(torch.uint8)) for n, t in got.items())
+
+
+def test_both_host_paths_give_the_same(ext, fal, monkeypatch):
+    """The native function takes these calls, and Python makes them to the same bits where there is none."""
+    gen = torch.Generator().manual_seed(12)
+    if ext._host is None:
+        pytest.skip("no native host path was built")
+    ext.device_status()
+    for dtype in DTYPES:
+        ends = []
+        for native in (True, False):
+            gen = torch.Generator().manual_seed(12)
+            cache = _filled(gen, DTYPES[dtype], [30, 7], 16, 2, 64, extra=9)
+            got = cache.on_gpu("bhsd")
+            q, k, v = (_rows(gen, 2, 9, h, 64).cuda() for h in (4, 2, 2))
+            cos, sin = (t.cuda() for t in _tables(cache.table.shape[1] * 16, 32))
+            calls = []
+            for n in ("paged_append_plain", "paged_attend_plain"):
+                real = getattr(ext._host, n[:-6])
+                monkeypatch.setattr(ext, n, (lambda *a, real=real: calls.append(real(*a)) or calls[-1]) if native else ext._general)
+            versions = {n: t._version for n, t in got.items()}
+            o = fal.flash_attn_with_paged_kvcache(q[:, :4], block_table=cache.table.cuda(), cache_seqlens=_lens([30, 7]), k=k[:, :4], v=v[:, :4],
+                                                  rotary_cos=cos, rotary_sin=sin, rotary_interleaved=True, softmax_scale=0.2, cache_layout="bhsd", **got)
+            turned, lens = fal.paged_cache_append(k[:, 4:], v[:, 4:], block_table=cache.table.cuda(), cache_seqlens=_lens([34, 11]), q=q[:, 4:],
+                                                  rotary_cos=cos, rotary_sin=sin, cache_layout="bhsd", **got)
+            o2 = fal.flash_attn_with_paged_kvcache(turned, block_table=cache.table.cuda(), cache_seqlens=lens, cache_layout="bhsd", **got)
+            assert len(calls) == (3 if native else 0) and all(c is not None for c in calls)
+            assert all(t._version > versions[n] for n, t in got.items())
+            ends.append([o, turned, lens, o2, *(t.view(torch.uint8) for t in got.values())])
+        assert all(torch.equal(a, b) for a, b in zip(*ends))
