@@ -1145,15 +1145,53 @@ fal::PagedCache paged_cache(const fal_paged_cache& c) {
   return p;
 }
 
+// The pages as [page, head, row, head_dim], boxes as launch_paged_attn wants them.
+int make_paged_map(CUtensorMap* map, const void* base, const fal_paged_cache& c, const fal_strides& s) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (enc == nullptr) return FAL_ERR_TENSOR_MAP;
+  const bool half = c.dtype == FAL_PAGED_F16;
+  const cuuint64_t bytes = half ? 2 : 1;
+  const cuuint32_t row_bytes = static_cast<cuuint32_t>(kernel_head_dim(c.head_dim) * bytes);
+  const cuuint32_t box_bytes = row_bytes < 128 ? row_bytes : 128;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                              static_cast<cuuint64_t>(c.heads_kv), static_cast<cuuint64_t>(c.num_pages)};
+  if (s.row <= 0 || (c.heads_kv > 1 && s.head <= 0) || (c.num_pages > 1 && s.batch <= 0)) return FAL_ERR_INVALID_ARGUMENT;
+  // (a dimension of extent 1 is never stepped along: any valid stride will do)
+  auto fix = [&](int64_t x) { return static_cast<cuuint64_t>(x > 0 ? x : c.head_dim) * bytes; };
+  const cuuint64_t strides[3] = {fix(s.row), fix(s.head), fix(s.batch)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_bytes / bytes), fal::kPagedBoxRows, 1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims,
+                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    g_last_cuda_error = 100000 + static_cast<int>(r);
+    return FAL_ERR_TENSOR_MAP;
+  }
+  return FAL_OK;
+}
+
 // Query rows of a KV head up to which the split-K pass takes them, 8 or 16 to a CTA that streams the keys for itself.
 constexpr int64_t kPagedFewRows = 64;
 constexpr int64_t kPagedGatherBytes = int64_t{1} << 30;
 
+constexpr int64_t kPagedUnknownSlots = 148 * 24;  // without a GPU to ask
+
+fal::PagedAttnParams paged_attn_params(const fal_paged_attn_args& a) {
+  fal::PagedAttnParams p{};
+  p.c = paged_cache(a.cache);
+  p.q = a.q; p.q_strides = to_rs(&a.q_strides); p.o = a.o;
+  p.heads_q = a.heads_q; p.rows = a.rows; p.kernel_dim = kernel_head_dim(a.cache.head_dim);
+  p.part_o = static_cast<float*>(a.workspace);
+  p.scale = a.softmax_scale; p.status = a.status;
+  return p;
+}
+
 // How a call is cut up, and what it needs of the workspace.
 struct PagedPlan {
   bool few_rows;
-  int split_shift, fine_splits, grid_splits, splits;  // few rows
-  int entries, heads;  // many: (entry, KV head) pairs whose rows are put in order at a time
+  int entries, heads;  // many rows: (entry, KV head) pairs whose rows are put in order at a time
   size_t k_bytes, lse_bytes, split_bytes;
   size_t total;
 };
@@ -1167,22 +1205,12 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
   PagedPlan p{};
   p.few_rows = rows <= kPagedFewRows;
   if (p.few_rows) {
-    const bool half = c.dtype == FAL_PAGED_F16;
+    fal::PagedAttnParams k = paged_attn_params(a);
+    const cudaError_t e = fal::paged_attn_plan(k);
+    if (e == cudaErrorInvalidValue) return p;  // too many units for one grid: nothing that a workspace helps
+    if (e != cudaSuccess) k.slots = kPagedUnknownSlots;
     const int per_cta = fal::paged_rows_per_cta(static_cast<int>(rows), dim);
-    const int64_t units = c.batch * c.heads_kv * ((rows + per_cta - 1) / per_cta);
-    const int64_t sms = sm_count() > 0 ? sm_count() : 148;
-    p.split_shift = (half ? 10 : 11) + (c.batch * (((capacity - 1) >> 11) + 1) >= 192 ? 1 : 0);
-    while (((capacity - 1) >> p.split_shift) + 1 > 1024) ++p.split_shift;
-    const int64_t most = ((capacity - 1) >> fal::kDecodeFinestShift) + 1;
-    int64_t fine = sms * (dim == 64 ? 4 : dim == 256 ? 1 : half ? 2 : 3) / units;
-    const int64_t fit = static_cast<int64_t>(kDecodeFineBytes / decode_partial_bytes(c.batch * a.rows, a.heads_q, 1, dim));
-    if (fine > fit) fine = fit;
-    if (fine > most) fine = most;
-    p.fine_splits = static_cast<int>(fine);
-    p.grid_splits = static_cast<int>(((capacity - 1) >> p.split_shift) + 1);
-    if (p.grid_splits < p.fine_splits) p.grid_splits = p.fine_splits;
-    p.splits = p.grid_splits + (half ? 0 : 1);
-    p.total = decode_partial_bytes(c.batch * a.rows, a.heads_q, p.splits, dim);
+    p.total = static_cast<size_t>(k.slots) * per_cta * (dim + 2) * sizeof(float) + 16;
     return p;
   }
   const int64_t unit = capacity * c.head_dim * 4;  // K and V
@@ -1260,6 +1288,7 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
   int rc = paged_attn_check(*a);
   if (rc != FAL_OK) return rc;
   const PagedPlan plan = paged_plan(*a);
+  if (plan.total == 0) return FAL_ERR_INVALID_ARGUMENT;
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return FAL_ERR_INVALID_ARGUMENT;
   if (a->workspace_bytes < plan.total) return FAL_ERR_WORKSPACE_TOO_SMALL;
   rc = check_device();
@@ -1267,16 +1296,11 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
   cudaStream_t st = static_cast<cudaStream_t>(a->stream);
   const fal_paged_cache& c = a->cache;
   if (plan.few_rows) {
-    fal::PagedAttnParams p{};
-    p.c = paged_cache(c);
-    p.q = a->q; p.q_strides = to_rs(&a->q_strides); p.o = a->o;
-    p.heads_q = a->heads_q; p.rows = a->rows; p.kernel_dim = kernel_head_dim(c.head_dim);
-    p.split_shift = plan.split_shift; p.fine_splits = plan.fine_splits;
-    p.grid_splits = plan.grid_splits; p.splits = plan.splits;
-    p.part_o = static_cast<float*>(a->workspace);
-    p.part_ml = p.part_o + static_cast<int64_t>(c.batch) * a->rows * a->heads_q * p.splits * p.kernel_dim;
-    p.scale = a->softmax_scale; p.status = a->status;
-    const cudaError_t e = fal::launch_paged_attn(p, st);
+    fal::PagedAttnParams p = paged_attn_params(*a);
+    CUtensorMap maps[2];
+    if ((rc = make_paged_map(&maps[0], c.k_pages, c, c.k_strides)) || (rc = make_paged_map(&maps[1], c.v_pages, c, c.v_strides)))
+      return rc;
+    const cudaError_t e = fal::launch_paged_attn(p, maps, st);
     return e == cudaSuccess ? FAL_OK : cuda_fail(e);
   }
 

@@ -17,10 +17,10 @@ __device__ __forceinline__ void merge_stats(float& m, float& l, float m2, float 
 }
 
 // Called by all threads of a block of kCombineThreads, WARPS warps to a row; tid: the thread's index among its row's.
-// Waits for the grids before this one, then merges partials 0 ... n - 1 (statistics ml, rows po of D / 4 pieces) into
-// head_dim_real columns at out_row.
-template <int D, int WARPS>
-__device__ __forceinline__ void combine_row(int tid, bool row_ok, int n, const float2* ml, const float4* po, __half* out_row,
+// Waits for the grids before this one, then merges n partials into head_dim_real columns at out_row: the i-th has its
+// statistics at ml[index(i)] and its row at po[index(i) * D / 4].
+template <int D, int WARPS, class Index>
+__device__ __forceinline__ void combine_row(int tid, bool row_ok, int n, const float2* ml, const float4* po, Index index, __half* out_row,
                                             int head_dim_real, float* lse) {
   static_assert(WARPS == 1 || WARPS * 32 == kCombineThreads, "a row per warp or per block");
   constexpr int kThreads = 32 * WARPS;                       // threads per row
@@ -46,14 +46,15 @@ __device__ __forceinline__ void combine_row(int tid, bool row_ok, int n, const f
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) px[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < n) {
-      mx[k] = ml[i].x;
+      const int64_t at = index(i);
+      mx[k] = ml[at].x;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) px[k][v] = po[static_cast<int64_t>(i) * (D / 4) + v * kLanes + lane];
+      for (int v = 0; v < kVecs; ++v) px[k][v] = po[at * (D / 4) + v * kLanes + lane];
     }
   }
   float m = -INFINITY, l = 0.f;
   for (int i = tid; i < n; i += kThreads) {
-    const float2 x = ml[i];
+    const float2 x = ml[index(i)];
     merge_stats(m, l, x.x, x.y);
   }
 #pragma unroll
@@ -92,9 +93,10 @@ __device__ __forceinline__ void combine_row(int tid, bool row_ok, int n, const f
   }
 #pragma unroll 4
   for (int i = grp + kAhead * kGroups; i < n; i += kGroups) {
-    const float w = fast_exp2(ml[i].x - muse);
+    const int64_t at = index(i);
+    const float w = fast_exp2(ml[at].x - muse);
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) add_weighted(o[v], w, po[static_cast<int64_t>(i) * (D / 4) + v * kLanes + lane]);
+    for (int v = 0; v < kVecs; ++v) add_weighted(o[v], w, po[at * (D / 4) + v * kLanes + lane]);
   }
   auto add = [&](float4& a, const float4& x) {
     a.x += x.x;

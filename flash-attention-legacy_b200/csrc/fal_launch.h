@@ -241,20 +241,23 @@ struct PagedAttnParams {
   const void* q;         // [batch, rows, heads_q, head_dim] fp16 through strides (entry / head / row)
   RowStrides q_strides;
   void* o;               // [batch, rows, heads_q, head_dim] fp16, contiguous
-  float* part_o;         // workspace [batch, rows, heads_q, splits, kernel head_dim]
-  float* part_ml;        // workspace [batch, rows, heads_q, splits, 2]
+  float* part_o;         // workspace [slots, rows per CTA, kernel head_dim]
+  float* part_ml;        // workspace [slots, rows per CTA, 2], behind part_o
   int heads_q;
   int rows;              // query i sees the keys up to position len - rows + i
   int kernel_dim;        // 64, 128 or 256
-  int split_shift, fine_splits;  // as for decode
-  int grid_splits;       // splits of the pages that an entry can have
-  int splits;            // partials per row: grid_splits, and one more for the tail of 8-bit caches
+  int parts;             // CTAs that all entries' keys are cut for
+  int64_t slots;         // CTAs whose results can go to the workspace
   float scale;
   int* status;
 };
 // Query rows that one CTA takes.
 int paged_rows_per_cta(int rows, int kernel_dim);
-cudaError_t launch_paged_attn(const PagedAttnParams& p, cudaStream_t stream);
+cudaError_t paged_attn_plan(PagedAttnParams& p);  // sets p.parts and p.slots, from the shapes and types in p
+// maps: of the K and of the V pages, (head_dim, row, head, page) with boxes of kPagedBoxRows rows x 128 bytes (64 where the
+// kernel's rows are that short), permuted as wide.
+constexpr int kPagedBoxRows = 16;
+cudaError_t launch_paged_attn(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream);
 
 // Entries b0 ... b0 + entries - 1 and KV heads h0 ... h0 + heads - 1 of a paged cache as fp16 rows in order.
 struct PagedGatherParams {

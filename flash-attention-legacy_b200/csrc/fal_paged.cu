@@ -9,6 +9,7 @@
 // token or as chunks, and no page is rounded again when a larger value arrives.  x m is exact in 32 bits (11 + 7 bits) and
 // its quotient by a, rounded once, is on the same side of every rounding border as the exact one: the border is a multiple
 // of 2^-5 of the code's leading bit at least 2^-16 away relative to it, or the quotient is exactly the border.
+#include <algorithm>
 #include <type_traits>
 
 #include "fal_combine.cuh"
@@ -308,15 +309,23 @@ cudaError_t launch_seal(const PagedAppendParams& p, cudaStream_t stream) {
 // ---------------------------------------------------------------------------
 // Bound by HBM: every K and V row is read once for all query rows of its KV head.  The products are mma.sync m16n8k16 with
 // 16 keys (scores) or 16 columns of V (output) as the M rows and 8 query rows as N: S^T = K Q^T, O^T = V^T P^T.  Query rows
-// are (token, head of the group) pairs, 8 NT to a CTA.  K and V fragments are read from shared memory as the lanes' own 16
-// bytes, without ldmatrix: a contraction may take its columns in any order, so lane t of four takes the columns 16 t' ...
-// of a key row that are next to each other, and Q is laid out to match; lane g of eight takes D / 8 neighbouring columns of V.
+// are (token, head of the group) pairs, 8 NT to a CTA.  A warp fetches 16-key slices of K and V by TMA (boxes of 16 rows of a
+// page) into a ring of its own.  Fragments are read from shared memory as the lanes' own 16 bytes, without ldmatrix: a
+// contraction may take its terms in any order, so lane t of four takes 16 bytes of a key row that are next to each other,
+// and Q is laid out to match; lane g of eight takes 16 neighbouring bytes of a V row.
 // 8-bit codes become fp16 in registers (exact), the scales enter in 32 bits: K's with the softmax scale, V's where the
 // product of a 16-key slice is added to the output.  P^T of the scores' layout becomes the second product's operand by
-// movmatrix.
+// movmatrix; its column sums, as one more product with ones, are the softmax sum and remove what int8's widening adds.
+//
+// An (entry, KV head, chunk of 8 NT query rows) is a unit; its keys count in steps of 64, a 16-key slice for each of four
+// warps.  Entries are cut into parts of one length that the GPU works out from all lengths, so that all units together
+// make a few CTAs for every place on the GPU, whatever the lengths are; the units of one part are CTAs next to each other,
+// because their rows are next to each other in memory where a page holds all heads of a position.  Parts of a cut entry go
+// to the workspace and a second kernel merges them; a CTA that has all keys of its unit writes the result itself.
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kPagedSlice = 16;
+constexpr int kPagedStep = kPagedWarps * kPagedSlice;  // keys
 
 template <class T>
 struct Elem {
@@ -328,14 +337,19 @@ struct Elem<__half> {
   static constexpr bool kScaled = false;
   static constexpr int kBytes = 2;
 };
+constexpr float kS8Bias = 1152.f;  // what widen_biased adds to a code
 
 // Four 8-bit codes as two pairs of fp16.
-__device__ __forceinline__ void widen(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ void widen_biased(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
   // 1024 + u, u = code + 128, as fp16 is 0x6400 + u
   const uint32_t u = w ^ 0x80808080u;
-  const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(l), "r"(0x64806480u));
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(h), "r"(0x64806480u));
+  lo = __byte_perm(u, 0x64646464u, 0x4140);
+  hi = __byte_perm(u, 0x64646464u, 0x4342);
+}
+__device__ __forceinline__ void widen(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
+  widen_biased(static_cast<const S8*>(nullptr), w, lo, hi);
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x64806480u));
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x64806480u));
 }
 __device__ __forceinline__ void widen(const E4M3*, uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t"
@@ -347,325 +361,533 @@ __device__ __forceinline__ void widen(const E4M3*, uint32_t w, uint32_t& lo, uin
       : "=r"(lo), "=r"(hi)
       : "r"(w));
 }
+__device__ __forceinline__ void widen_biased(const E4M3* type, uint32_t w, uint32_t& lo, uint32_t& hi) { widen(type, w, lo, hi); }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void cp_async_4_zfill(uint32_t dst, const void* src, bool valid) {
-  const uint32_t n = valid ? 4u : 0u;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void cp_async_16_bytes(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-
-__device__ __forceinline__ void lds16(uint32_t addr, uint32_t (&w)[4]) {
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-               : "r"(addr));
+// D = A * B + C of mma_16816, C and D apart
+__device__ __forceinline__ void mma_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-__device__ __forceinline__ void lds8(uint32_t addr, uint32_t (&w)[2]) {
+__device__ __forceinline__ void lds16(uint32_t addr, uint32_t* w) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+}
+__device__ __forceinline__ void lds8(uint32_t addr, uint32_t* w) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
 }
 
-// Rows of D elements in shared memory, 16-byte chunks permuted so that eight lanes of a 16-byte load hit different
-// banks: for K they are two rows of four chunks, for V four rows (2 t) of one or two lanes' columns.
+// A slice of 16 rows of a page in shared memory as TMA leaves it: blocks of 16 rows x 128 bytes (64-byte rows: one of 64),
+// the 16-byte chunks of a row exclusive-or'ed with the row's number (64-byte rows: half of it).  The eight lanes that a
+// 16-byte load serves at a time hit different banks if they are, for K, rows 4 apart, and for V, rows 0 ... 3 and chunks 4
+// apart (64-byte rows: rows of both parities).  So row i of the first product's operand is key key_of(i), and lane g takes
+// chunk chunk_of(g) of the V rows.
 template <int D, class T>
 struct PagedTile {
   static constexpr int kRowBytes = D * Elem<T>::kBytes;
-  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kBlockRow = kRowBytes < 128 ? kRowBytes : 128;
+  static constexpr int kBlocks = kRowBytes / kBlockRow;
+  static constexpr int kBlockBytes = kPagedSlice * kBlockRow;
   static constexpr int kSliceBytes = kPagedSlice * kRowBytes;  // K or V
-  static constexpr int kLaneBytes = kRowBytes / 8;             // of a V row
-  static __device__ __forceinline__ int k_chunk(int row, int ch) { return kChunks >= 8 ? ch ^ ((row & 1) << 2) : ch; }
-  static __device__ __forceinline__ int v_chunk(int row, int ch) {
-    const int t = (row >> 1) & 3;
-    if (kLaneBytes == 8 || kLaneBytes == 64) return ch ^ t;
-    if (kLaneBytes == 16) return ch ^ (t << 1);
-    return ch ^ ((t & 1) | ((t & 2) << 1));
+  static constexpr int kLaneCols = kBlockRow / 8 / Elem<T>::kBytes;  // of a block's V row that a lane takes
+  static constexpr bool kNarrow = kBlockRow == 64;
+  static __device__ __forceinline__ int key_of(int i) {  // i: 0 ... 7; 8 ... 15 are 8 further
+    return kNarrow ? i ^ ((i >> 1) & 1) : ((i & 1) << 2) | (i >> 1);
   }
+  static __device__ __forceinline__ int chunk_of(int g) { return ((g & 1) << 2) | (g >> 1); }
+  // Shared address in the K slice of row key_of(g), chunk t; in the V slice of row key_of(2 t), the lane's columns.
+  static __device__ __forceinline__ uint32_t k_read(int g, int t) {
+    const int row = key_of(g);
+    return row * kBlockRow + (t ^ (kNarrow ? row >> 1 : row)) * 16;
+  }
+  static __device__ __forceinline__ uint32_t v_read(int g, int t) {
+    const int row = key_of(2 * t);
+    if (kNarrow) return row * kBlockRow + ((g >> 1) ^ (row >> 1)) * 16 + (g & 1) * 8;
+    return row * kBlockRow + (chunk_of(g) ^ row) * 16;
+  }
+  // From there to row key_of(2 t + 1).
+  static __device__ __forceinline__ uint32_t v_next(uint32_t at) { return kNarrow ? at ^ 64u : (at ^ 64u) + 4 * kBlockRow; }
+  // First of the two columns that a lane has of output tile j.
+  static __device__ __forceinline__ int column(int g, int j) {
+    const int block = j / (kLaneCols / 2);
+    return block * 8 * kLaneCols + (kNarrow ? g : chunk_of(g)) * kLaneCols + j % (kLaneCols / 2) * 2;
+  }
+};
+
+// A slice of an 8-bit cache's tail: 16 fp16 rows, copied by the lanes (rows behind the end are zeros), chunks permuted for K
+// as above with two chunks a lane.  Lanes take the columns that they take of the pages.
+template <int D, class T>
+struct PagedTailTile {
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kLoads = kPagedSlice * kChunks / 32;
+  static constexpr int kCopyRows = 32 / kChunks;
+  static_assert(kCopyRows >= 1, "a row is at most 512 bytes");
+  static __device__ __forceinline__ uint32_t place(int row, int ch) { return row * kRowBytes + (ch ^ (row & 7)) * 16; }
 };
 
 template <int D, class T>
 struct PagedSmem {
-  static constexpr int kStages = Elem<T>::kScaled ? 4 : 3;
-  static constexpr int kRingBytes = kStages * 2 * PagedTile<D, T>::kSliceBytes;  // per warp
-  static constexpr int kScaleBytes = kStages * 8;
-  static constexpr int kTailStages = kRingBytes / (2 * PagedTile<D, __half>::kSliceBytes);
-  static_assert(kTailStages >= 1, "a slice of the tail fits");
-  static constexpr int kScaleOffset = kPagedWarps * kRingBytes;
-  static constexpr int kPipeBytes = kScaleOffset + kPagedWarps * kScaleBytes;
-  static constexpr int merge_bytes(int rows) { return kPagedWarps * rows * (D + 2) * 4; }
-  static constexpr int bytes(int rows) { return kPipeBytes > merge_bytes(rows) ? kPipeBytes : merge_bytes(rows); }
+  static constexpr bool kScaled = Elem<T>::kScaled;
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStageBytes = 2 * PagedTile<D, T>::kSliceBytes;  // K and V; or one of a slice of the tail
+  static constexpr int kRingBytes = kStages * kStageBytes;  // per warp
+  static constexpr int kPipeBytes = kPagedWarps * kRingBytes;
+  static constexpr int kPitch = D + 4;  // floats of a row of a warp's result
+  static constexpr int merge_bytes(int rows) { return kPagedWarps * rows * (kPitch + 2) * 4; }
+  static constexpr int kAlign = 1024;   // of TMA's permuted blocks
+  static constexpr int bytes(int rows) { return (kPipeBytes > merge_bytes(rows) ? kPipeBytes : merge_bytes(rows)) + kAlign; }
 };
 
-// log2 of the positions per split of an entry with `len` positions in pages.
-__device__ __forceinline__ int paged_split_shift(const PagedAttnParams& p, int len) {
-  int shift = kDecodeFinestShift;
-  while (shift < p.split_shift && ((len - 1) >> shift) + 1 > p.fine_splits) ++shift;
-  return shift;
-}
-// Positions of an entry of n that are in pages.
+// ---- the deal ----
 __device__ __forceinline__ int paged_len_in_pages(const PagedCache& c, int n) {
   return c.type == kPagedF16 ? n : n >> c.page_shift << c.page_shift;
 }
+// Steps of one unit of an entry with n positions: those of its pages, then those of its tail.
+__device__ __forceinline__ int paged_steps(const PagedCache& c, int n) {
+  const int in_pages = paged_len_in_pages(c, n);
+  return (in_pages + kPagedStep - 1) / kPagedStep + (n - in_pages + kPagedStep - 1) / kPagedStep;
+}
 
+// Sums over the block's threads up to this one, and over all of them.
+struct PagedSums {
+  uint64_t warp_sum[kPagedWarps];
+};
+__device__ __forceinline__ uint64_t paged_block_sum(PagedSums& sums, uint64_t mine, uint64_t& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint64_t x = __shfl_up_sync(0xffffffffu, mine, off);
+    if (lane >= off) mine += x;
+  }
+  __syncthreads();  // (the last sums have been read)
+  if (lane == 31) sums.warp_sum[warp] = mine;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kPagedWarps; ++w) {
+    if (w < warp) mine += sums.warp_sum[w];
+    all += sums.warp_sum[w];
+  }
+  return mine;
+}
+
+// A part is at least kPagedMinSteps long, and otherwise as long as makes `p.parts` CTAs of all units: kPagedWaves for every place.
+constexpr int kPagedMinSteps = 4;
+#ifndef FAL_PAGED_WAVES
+#define FAL_PAGED_WAVES 2
+#endif
+constexpr int kPagedWaves = FAL_PAGED_WAVES;
+
+// How an entry is cut.
+struct PagedCut {
+  int n;          // positions
+  int steps;      // of a unit
+  int parts;
+  int64_t group;  // parts of the entries before it
+  int64_t slot;   // the same, of those that are cut (their results go to the workspace)
+};
+// Finds the entry `b` (if b >= 0), or else the one that has part `group` of all entries' parts (b is set).  False: there is none.
+// Called by all threads of a block.
+__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, const PagedAttnParams& p, int64_t heads, int64_t group, int& b,
+                                           PagedCut& shared_cut, int& shared_b) {
+  const PagedCache& c = p.c;
+  const int last = (c.batch - 1) / kPagedThreads * kPagedThreads;
+  int64_t total = 0;
+  int n = 0;
+  for (int base = last; base >= 0; base -= kPagedThreads) {
+    const int e = base + threadIdx.x;
+    n = e < c.batch ? paged_len(c, e) : 0;
+    uint64_t all;
+    paged_block_sum(sums, paged_steps(c, n), all);
+    total += all;
+  }
+  const int64_t length = max((total * heads + p.parts - 1) / p.parts, static_cast<int64_t>(kPagedMinSteps));
+  uint64_t before = 0;  // parts in the low half, parts of cut entries in the high half
+  for (int base = 0; base <= last; base += kPagedThreads) {
+    const int e = base + threadIdx.x;
+    if (base > 0) n = e < c.batch ? paged_len(c, e) : 0;
+    const int steps = paged_steps(c, n);
+    const uint64_t parts = (steps + length - 1) / length;
+    uint64_t all;
+    const uint64_t upto = before + paged_block_sum(sums, parts | (parts > 1 ? parts << 32 : 0), all);
+    const uint64_t from = upto - (parts | (parts > 1 ? parts << 32 : 0));
+    const bool here = b >= 0 ? b >= base && b < base + kPagedThreads
+                             : group < static_cast<int64_t>((before + all) & 0xffffffffu);
+    if (here) {
+      const int64_t first = static_cast<int64_t>(from & 0xffffffffu);
+      if (b >= 0 ? e == b : group >= first && group < first + static_cast<int64_t>(parts)) {
+        shared_cut = PagedCut{n, steps, static_cast<int>(parts), first, static_cast<int64_t>(from >> 32)};
+        shared_b = e;
+      }
+      __syncthreads();
+      cut_out = shared_cut;
+      b = shared_b;
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
+// ---- one piece of a unit ----
 template <int D, int NT>
 struct PagedState {
   uint32_t q[D / 16][2][NT];
+  uint32_t p[NT][2];  // the weights of the slice in hand, as the second product's operand
+  float sum[NT][4];   // of those weights, times kSumFactor
   float o[NT][D / 16][4];
-  float m[NT][2];  // running maximum, log2 domain
-  float l[NT][2];  // this lane's part of the sum
+  float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far
+  float most[NT][2];  // what an exponent may be before the reference moves: 8, or -infinity before the first key
+  float l[NT][2];     // times kSumFactor
+  float c2;
+  int limit[NT][2];  // first key that a query row does not see
+  int min_limit;
 };
 
-// Where a warp finds its keys: pages through the table (T as stored), or the tail (fp16).
+// The column sums of the weights come from a product with this number in every place: int8 wants them times what
+// widen_biased adds, to take it off again.
 template <class T>
-struct PagedSource {
-  const uint8_t* k;  // of the KV head
-  const uint8_t* v;
-  int64_t k_page, v_page, k_row, v_row;  // bytes
-  const int32_t* table;  // of the entry; null for the tail
-  int page_shift, num_pages;
-  const float* k_scales;  // of the KV head
-  const float* v_scales;
-  int heads_kv;
-  int* status;
-};
+constexpr float kSumFactor = std::is_same<T, S8>::value ? -kS8Bias : 1.f;
+template <class T>
+constexpr uint32_t kSumOperand = std::is_same<T, S8>::value ? 0xe480e480u : 0x3c003c00u;  // two of it in fp16
 
-// Keys pos0 ... pos_end - 1 for the query rows of a CTA, one 16-key slice of every kPagedWarps to a warp.
-template <int D, class T, int NT, int STAGES>
-__device__ __forceinline__ void paged_stream(const PagedSource<T>& src, uint32_t ring, uint32_t ring_scales, int pos0,
-                                             int pos_end, int real_chunks, float c2, const int (&limit)[NT][2], int min_limit,
-                                             PagedState<D, NT>& st) {
-  using Tile = PagedTile<D, T>;
-  constexpr bool kScaled = Elem<T>::kScaled;
-  constexpr int kLoads = kPagedSlice * Tile::kChunks / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int slices = (pos_end - pos0 + kPagedSlice - 1) / kPagedSlice;
-  const int mine = (slices - warp + kPagedWarps - 1) / kPagedWarps;
-  const int page_mask = (1 << src.page_shift) - 1;
-
-  auto page_of = [&](int i) {
-    const int slice = i * kPagedWarps + warp;
-    return src.table != nullptr && slice < slices ? __ldg(src.table + ((pos0 + slice * kPagedSlice) >> src.page_shift)) : 0;
-  };
-  int next_page = page_of(0);
-  auto issue = [&](int i) {
-    const int slice = i * kPagedWarps + warp;
-    const int page = next_page;
-    next_page = page_of(i + 1);
-    if (slice < slices) {
-      const int key0 = pos0 + slice * kPagedSlice;
-      const uint32_t sb = ring + (i % STAGES) * 2 * Tile::kSliceBytes;
-      const bool there = page >= 0 && page < src.num_pages;  // (else its rows are zeros)
-      if (!there && lane == 0 && src.status) atomicCAS(src.status, 0, kDevNoPage);
-      const int64_t id = there ? page : 0;
-      const int row0 = src.table != nullptr ? key0 & page_mask : key0;
-      const uint8_t* kp = src.k + id * src.k_page + row0 * src.k_row;
-      const uint8_t* vp = src.v + id * src.v_page + row0 * src.v_row;
-#pragma unroll
-      for (int it = 0; it < kLoads; ++it) {
-        const int idx = it * 32 + lane;
-        const int row = idx / Tile::kChunks, ch = idx % Tile::kChunks;
-        const bool ok = there && key0 + row < pos_end && ch < real_chunks;
-        const int64_t r = ok ? row : 0;
-        const int sc = ok ? ch : 0;
-        cp_async_16_zfill(sb + row * Tile::kRowBytes + Tile::k_chunk(row, ch) * 16, kp + r * src.k_row + sc * 16, ok);
-        cp_async_16_zfill(sb + Tile::kSliceBytes + row * Tile::kRowBytes + Tile::v_chunk(row, ch) * 16,
-                          vp + r * src.v_row + sc * 16, ok);
-      }
-      if (kScaled && lane < 2)
-        cp_async_4_zfill(ring_scales + (i % STAGES) * 8 + lane * 4, (lane == 0 ? src.k_scales : src.v_scales) + id * src.heads_kv,
-                         there);
-    }
-    cp_async_commit();  // (always, so that the groups count the same)
-  };
-
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(i);
-  for (int i = 0; i < mine; ++i) {
-    issue(i + STAGES - 1);
-    cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const uint32_t sb = ring + (i % STAGES) * 2 * Tile::kSliceBytes;
-    const int key0 = pos0 + (i * kPagedWarps + warp) * kPagedSlice;
-    float k_scale = 1.f, v_scale = 1.f;
-    if constexpr (kScaled)
-      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(ring_scales + (i % STAGES) * 8));
-
-    // ---- S^T = K Q^T: 16 keys x 8 NT query rows ----
-    float s[NT][4];
+// What follows the first product: scores s of this lane's keys key and key + 8 for query rows 2 t and 2 t + 1 of every eight
+// become weights.  W: the type of the pages (kSumFactor).
+template <int D, class W, int NT>
+__device__ __forceinline__ void paged_weights(PagedState<D, NT>& st, float (&s)[NT][4], int key0, int key, float k_scale) {
+  const float f = st.c2 * k_scale;
+  if (key0 + kPagedSlice > st.min_limit) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[nt][e] = key + (e >> 1) * 8 >= st.limit[nt][e & 1] ? -INFINITY : s[nt][e] * f;
+  } else {
 #pragma unroll
-    for (int seg = 0; seg < Tile::kRowBytes / 64; ++seg) {
-      uint32_t r0[4], r1[4];
-      lds16(sb + g * Tile::kRowBytes + Tile::k_chunk(g, seg * 4 + t) * 16, r0);
-      lds16(sb + (g + 8) * Tile::kRowBytes + Tile::k_chunk(g + 8, seg * 4 + t) * 16, r1);
-      if constexpr (kScaled) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t a[4];
-          widen(static_cast<const T*>(nullptr), r0[k], a[0], a[2]);
-          widen(static_cast<const T*>(nullptr), r1[k], a[1], a[3]);
+      for (int e = 0; e < 4; ++e) s[nt][e] *= f;
+  }
+  bool grows = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], a, st.q[seg * 4 + k][0][nt], st.q[seg * 4 + k][1][nt]);
-        }
-      } else {
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t a[4] = {r0[2 * k], r1[2 * k], r0[2 * k + 1], r1[2 * k + 1]};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], a, st.q[seg * 2 + k][0][nt], st.q[seg * 2 + k][1][nt]);
-        }
-      }
-    }
-
-    // ---- softmax over the keys: this lane has keys g and g + 8 of query rows 2 t and 2 t + 1 of every eight ----
-    const float f = c2 * k_scale;
-    const bool masked = key0 + kPagedSlice > min_limit;
-    uint32_t pb[NT][2];
-    float mx[NT][2];
-    bool grows = false;
+    for (int e = 0; e < 2; ++e) grows = grows || fmaxf(s[nt][e], s[nt][2 + e]) - st.m[nt][e] > st.most[nt][e];
+  // The reference follows the largest score only when a weight would exceed 2^8: the output is rescaled a few times per
+  // piece, and the largest is looked for across the lanes only then.
+  if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[nt][e] *= f;
-        if (masked && key0 + g + (e >> 1) * 8 >= limit[nt][e & 1]) s[nt][e] = -INFINITY;
-      }
+      float alpha[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float x = fmaxf(s[nt][e], s[nt][2 + e]);
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        mx[nt][e] = x;
-        grows = grows || x > st.m[nt][e];
-      }
-    }
-    if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float alpha[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float m_new = fmaxf(st.m[nt][e], mx[nt][e]);
-          alpha[e] = fast_exp2(st.m[nt][e] - (m_new == -INFINITY ? 0.f : m_new));
-          st.l[nt][e] *= alpha[e];
+        const bool none = st.most[nt][e] == -INFINITY;  // (then m is 0 and stands for no reference)
+        const float m_new = none ? x : fmaxf(st.m[nt][e], x);
+        alpha[e] = 0.f;
+        if (m_new != -INFINITY) {  // (else no key yet)
+          if (!none) alpha[e] = fast_exp2(st.m[nt][e] - m_new);
           st.m[nt][e] = m_new;
+          st.most[nt][e] = 8.f;
         }
+        st.l[nt][e] *= alpha[e];
+      }
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          st.o[nt][j][0] *= alpha[0];
-          st.o[nt][j][1] *= alpha[1];
-          st.o[nt][j][2] *= alpha[0];
-          st.o[nt][j][3] *= alpha[1];
-        }
+      for (int j = 0; j < D / 16; ++j) {
+        st.o[nt][j][0] *= alpha[0];
+        st.o[nt][j][1] *= alpha[1];
+        st.o[nt][j][2] *= alpha[0];
+        st.o[nt][j][3] *= alpha[1];
       }
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float m_use = st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
-        s[nt][e] = fast_exp2(s[nt][e] - m_use);
-        s[nt][2 + e] = fast_exp2(s[nt][2 + e] - m_use);
-        st.l[nt][e] += s[nt][e] + s[nt][2 + e];
-      }
-      pb[nt][0] = movmatrix(pack_half2(s[nt][0], s[nt][1]));
-      pb[nt][1] = movmatrix(pack_half2(s[nt][2], s[nt][3]));
-    }
-
-    // ---- O^T += V^T P^T ----
-    const uint32_t vb = sb + Tile::kSliceBytes;
-    auto product = [&](int j, const uint32_t (&a)[4]) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (kScaled) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_16816(x, a, pb[nt][0], pb[nt][1]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) st.o[nt][j][e] += v_scale * x[e];
-        } else {
-          mma_16816(st.o[nt][j], a, pb[nt][0], pb[nt][1]);
-        }
-      }
-    };
-    constexpr int kPiece = Tile::kLaneBytes < 16 ? Tile::kLaneBytes : 16;
-#pragma unroll
-    for (int piece = 0; piece < Tile::kLaneBytes / kPiece; ++piece) {
-      uint32_t w[4][4];  // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 2 * t + (r & 1) + (r >> 1) * 8;
-        const int byte = g * Tile::kLaneBytes + piece * 16;
-        const uint32_t addr = vb + row * Tile::kRowBytes + Tile::v_chunk(row, byte >> 4) * 16 + (byte & 15);
-        if constexpr (kPiece == 16) {
-          lds16(addr, w[r]);
-        } else {
-          uint32_t half_row[2];
-          lds8(addr, half_row);
-          w[r][0] = half_row[0];
-          w[r][1] = half_row[1];
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kPiece / 4; ++k) {
-        if constexpr (kScaled) {
-          const int j = piece * 8 + 2 * k;  // two output tiles of two columns a lane
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t a[4];
-            widen(static_cast<const T*>(nullptr), __byte_perm(w[0][k], w[1][k], u == 0 ? 0x5140 : 0x7362), a[0], a[1]);
-            widen(static_cast<const T*>(nullptr), __byte_perm(w[2][k], w[3][k], u == 0 ? 0x5140 : 0x7362), a[2], a[3]);
-            product(j + u, a);
-          }
-        } else {
-          const uint32_t a[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
-                                 __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
-          product(piece * 4 + k, a);
-        }
-      }
-    }
-    __syncwarp();  // all lanes are done with this stage before it is refilled
   }
-  cp_async_wait<0>();
-}
-
-// Grid: (KV head x chunk of 8 NT query rows, split -- the last one of 8-bit caches is the tail --, entry).
-template <int D, class T, int NT>
-__global__ void __launch_bounds__(kPagedThreads) fal_paged_splitk_kernel(const PagedAttnParams p) {
-  using L = PagedSmem<D, T>;
-  constexpr int kRows = 8 * NT;
-  extern __shared__ __align__(128) uint8_t paged_smem[];
-  grid_dependency_wait();    // the append of this step's rows may still run up to here
-  grid_dependency_launch();
-  const PagedCache& c = p.c;
-  const int group = p.heads_q / c.heads_kv;
-  const int chunks = (p.rows * group + kRows - 1) / kRows;
-  const int kv_head = blockIdx.x / chunks;
-  const int row0 = blockIdx.x % chunks * kRows;  // of the KV head's rows * group query rows
-  const int rows_valid = min(kRows, p.rows * group - row0);
-  const int b = blockIdx.z;
-  const int n = paged_len(c, b);
-  const int in_pages = paged_len_in_pages(c, n);
-  const int shift = paged_split_shift(p, in_pages);
-  const bool is_tail = Elem<T>::kScaled && blockIdx.y == static_cast<unsigned>(p.grid_splits);
-  const int split = is_tail ? ((in_pages - 1) >> shift) + 1 : blockIdx.y;  // of the partial results
-  const int pos0 = is_tail ? in_pages : split << shift;
-  const int pos_end = is_tail ? n : min(pos0 + (1 << shift), in_pages);
-  if (pos0 >= pos_end) return;
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  PagedState<D, NT> st;
-  int limit[NT][2];  // first key that a query row does not see
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
+    for (int e = 0; e < 4; ++e) s[nt][e] = fast_exp2(s[nt][e] - st.m[nt][e & 1]);
+    st.p[nt][0] = movmatrix(pack_half2(s[nt][0], s[nt][1]));
+    st.p[nt][1] = movmatrix(pack_half2(s[nt][2], s[nt][3]));
+    // sums of the weights as they are rounded, which is what the output is divided by
+    const uint32_t factor[4] = {kSumOperand<W>, kSumOperand<W>, kSumOperand<W>, kSumOperand<W>};
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_16816_from(st.sum[nt], factor, st.p[nt][0], st.p[nt][1], zero);
+    st.l[nt][0] += st.sum[nt][0];
+    st.l[nt][1] += st.sum[nt][1];
+  }
+}
+
+// s (+)= the product of 16 keys' columns of one step and Q's.
+template <int D, int NT>
+__device__ __forceinline__ void paged_score_step(PagedState<D, NT>& st, float (&s)[NT][4], const uint32_t (&a)[4], int ks) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if (ks == 0) {
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816_from(s[nt], a, st.q[ks][0][nt], st.q[ks][1][nt], zero);
+    } else {
+      mma_16816(s[nt], a, st.q[ks][0][nt], st.q[ks][1][nt]);
+    }
+  }
+}
+
+// Weights of a slice of a page, keys key0 ...; kb: its shared address + k_read.
+template <int D, class T, int NT>
+__device__ __forceinline__ void paged_scores(PagedState<D, NT>& st, uint32_t kb, int key0, float k_scale) {
+  using Tile = PagedTile<D, T>;
+  constexpr int kSteps = Elem<T>::kScaled ? 4 : 2;  // of 16 columns in four lanes' 16 bytes
+  float s[NT][4];
+#pragma unroll
+  for (int seg = 0; seg < Tile::kRowBytes / 64; ++seg) {
+    uint32_t r0[4], r1[4];
+    const uint32_t at = (kb ^ (seg & 1) * 64) + (seg >> 1) * Tile::kBlockBytes;
+    lds16(at, r0);
+    lds16(at + 8 * Tile::kBlockRow, r1);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      uint32_t a[4];
+      if constexpr (Elem<T>::kScaled) {
+        widen(static_cast<const T*>(nullptr), r0[k], a[0], a[2]);
+        widen(static_cast<const T*>(nullptr), r1[k], a[1], a[3]);
+      } else {
+        a[0] = r0[2 * k];
+        a[1] = r1[2 * k];
+        a[2] = r0[2 * k + 1];
+        a[3] = r1[2 * k + 1];
+      }
+      paged_score_step(st, s, a, seg * kSteps + k);
+    }
+  }
+  paged_weights<D, T, NT>(st, s, key0, key0 + Tile::key_of((threadIdx.x & 31) >> 2), k_scale);
+}
+
+// O^T += V^T P^T of a slice of a page; vb: its shared address + v_read.
+template <int D, class T, int NT>
+__device__ __forceinline__ void paged_output(PagedState<D, NT>& st, uint32_t vb, float v_scale) {
+  using Tile = PagedTile<D, T>;
+  auto product = [&](int j, const uint32_t (&a)[4]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if constexpr (Elem<T>::kScaled) {
+        float x[4];
+        if constexpr (std::is_same<T, S8>::value) {
+          // (sums of codes + 1 152 and the sums that take it off cancel within a slice: 2^-23 of 1 152, 2^-13 of a code's step)
+          mma_16816_from(x, a, st.p[nt][0], st.p[nt][1], st.sum[nt]);
+        } else {
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_16816_from(x, a, st.p[nt][0], st.p[nt][1], zero);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const uint64_t y = ffma2(pack_f32x2(x[e], x[e + 1]), pack_f32x2(v_scale, v_scale), pack_f32x2(st.o[nt][j][e], st.o[nt][j][e + 1]));
+          unpack_f32x2(y, st.o[nt][j][e], st.o[nt][j][e + 1]);
+        }
+      } else {
+        mma_16816(st.o[nt][j], a, st.p[nt][0], st.p[nt][1]);
+      }
+    }
+  };
+#pragma unroll
+  for (int block = 0; block < Tile::kBlocks; ++block) {
+    uint32_t w[4][4];  // rows key_of(2 t), key_of(2 t + 1), and 8 further
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t at = ((r & 1) != 0 ? Tile::v_next(vb) : vb) + (r >> 1) * 8 * Tile::kBlockRow + block * Tile::kBlockBytes;
+      if constexpr (Tile::kNarrow) lds8(at, w[r]);
+      else lds16(at, w[r]);
+    }
+#pragma unroll
+    for (int k = 0; k < Tile::kBlockRow / 32; ++k) {
+      if constexpr (Elem<T>::kScaled) {
+        const int j = block * 8 + 2 * k;  // two output tiles of two columns a lane
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a[4];
+          widen_biased(static_cast<const T*>(nullptr), __byte_perm(w[0][k], w[1][k], u == 0 ? 0x5140 : 0x7362), a[0], a[1]);
+          widen_biased(static_cast<const T*>(nullptr), __byte_perm(w[2][k], w[3][k], u == 0 ? 0x5140 : 0x7362), a[2], a[3]);
+          product(j + u, a);
+        }
+      } else {
+        const uint32_t a[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
+                               __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
+        product(block * 4 + k, a);
+      }
+    }
+  }
+}
+
+// The same of a slice of the tail at shared address base; K and V are there one after the other.
+template <int D, class T, int NT>
+__device__ __forceinline__ void paged_tail_scores(PagedState<D, NT>& st, uint32_t base, int key0) {
+  using Tail = PagedTailTile<D, T>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float s[NT][4];
+#pragma unroll
+  for (int seg = 0; seg < D / 64; ++seg) {
+    uint32_t r0[8], r1[8];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      lds16(base + Tail::place(g, (seg * 4 + t) * 2 + x), r0 + 4 * x);
+      lds16(base + Tail::place(g + 8, (seg * 4 + t) * 2 + x), r1 + 4 * x);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a[4] = {r0[2 * k], r1[2 * k], r0[2 * k + 1], r1[2 * k + 1]};
+      paged_score_step(st, s, a, seg * 4 + k);
+    }
+  }
+  paged_weights<D, T, NT>(st, s, key0, key0 + g, 1.f);
+}
+template <int D, class T, int NT>
+__device__ __forceinline__ void paged_tail_output(PagedState<D, NT>& st, uint32_t base) {
+  using Tile = PagedTile<D, T>;
+  using Tail = PagedTailTile<D, T>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int j = 0; j < D / 16; j += 4) {  // eight columns
+    uint32_t w[4][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lds16(base + Tail::place(2 * t + (r & 1) + (r >> 1) * 8, Tile::column(g, j) / 8), w[r]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
+                             __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_16816(st.o[nt][j + k], a, st.p[nt][0], st.p[nt][1]);
+    }
+  }
+}
+
+// A warp's ring: its shared address, a barrier per stage, and their phases (a bit each).
+struct PagedRing {
+  uint32_t base;
+  uint32_t barriers;
+  uint32_t phases;
+  WaitCtx wait;
+};
+constexpr int kPagedBarrierId = 60;
+
+// Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
+template <int D, class T, int NT>
+__device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, PagedRing& ring,
+                                            int b, int n, int kv_head, int row0, int rows_valid, int step0, int step1,
+                                            PagedState<D, NT>& st) {
+  using L = PagedSmem<D, T>;
+  using Tile = PagedTile<D, T>;
+  constexpr bool kScaled = Elem<T>::kScaled;
+  constexpr int kQ = 16 / Elem<T>::kBytes;  // neighbouring columns of a lane in Q's layout
+  constexpr int kAhead = L::kStages - 1;
+  const PagedCache& c = p.c;
+  const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = p.heads_q / c.heads_kv;
+  const int in_pages = paged_len_in_pages(c, n);
+  const int page_steps = (in_pages + kPagedStep - 1) / kPagedStep;
+
+  // this warp's slices: key0 = first + i * 64
+  const int first = step0 * kPagedStep + warp * kPagedSlice;
+  const int page_end = min(step1 * kPagedStep, in_pages);
+  const int slices = page_end > first ? (page_end - first + kPagedStep - 1) / kPagedStep : 0;
+  const int tail_first = (max(step0, page_steps) - page_steps) * kPagedStep + warp * kPagedSlice;  // row of the tail
+  const int tail_end = kScaled ? min((step1 - page_steps) * kPagedStep, n - in_pages) : 0;
+  const int tail_slices = tail_end > tail_first ? (tail_end - tail_first + kPagedStep - 1) / kPagedStep : 0;
+
+  // Pages and scales of 32 slices at a time, one to a lane: of the slices whose loads are being issued, of the 32 before them
+  // (some of which are still to be worked on), and of the 32 behind them.
+  const int32_t* table = c.table + b * c.table_stride;
+  auto pages_of = [&](int i) { return i + lane < slices ? __ldg(table + ((first + (i + lane) * kPagedStep) >> c.page_shift)) : 0; };
+  auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages); };
+  auto scale_of = [&](const float* scales, int page) {
+    return kScaled && there(page) ? __ldg(scales + static_cast<int64_t>(page) * c.heads_kv + kv_head) : 0.f;
+  };
+  int pages = pages_of(0), next_pages = 0;
+  float k_scales = 0.f, v_scales = 0.f, next_k = 0.f, next_v = 0.f, last_k = 0.f, last_v = 0.f;
+  uint32_t fill = 0;  // stage that the next loads go to
+  auto issue = [&](int i) {
+    if (i < slices) {
+      if ((i & 31) == 0 && i > 0) {
+        pages = next_pages;
+        last_k = k_scales;
+        last_v = v_scales;
+        k_scales = next_k;
+        v_scales = next_v;
+      }
+      if ((i & 31) == 4) next_pages = pages_of((i & ~31) + 32);
+      if (kScaled && (i & 31) == 20) {
+        next_k = scale_of(c.k_scales, next_pages);
+        next_v = scale_of(c.v_scales, next_pages);
+      }
+      int page = __shfl_sync(0xffffffffu, pages, i & 31);
+      const int row = (first + i * kPagedStep) & ((1 << c.page_shift) - 1);
+      if (elect_one()) {
+        const uint32_t bar = ring.barriers + fill * 8;
+        const uint32_t stage = ring.base + fill * L::kStageBytes;
+        if (!there(page)) {  // (TMA fills a box outside of the tensor with zeros)
+          page = c.num_pages;
+          if (p.status) atomicCAS(p.status, 0, kDevNoPage);
+        }
+        mbar_arrive_expect_tx(bar, L::kStageBytes);
+#pragma unroll
+        for (int x = 0; x < Tile::kBlocks; ++x) {
+          const int column = x * Tile::kBlockRow / Elem<T>::kBytes;
+          tma_load_4d(stage + x * Tile::kBlockBytes, k_map, bar, column, row, kv_head, page);
+          tma_load_4d(stage + Tile::kSliceBytes + x * Tile::kBlockBytes, v_map, bar, column, row, kv_head, page);
+        }
+      }
+    } else if (kScaled && i < slices + 2 * tail_slices) {  // K, then V of a slice of the tail
+      using Tail = PagedTailTile<D, T>;
+      const int j = i - slices;
+      const bool is_v = (j & 1) != 0;
+      const RowStrides& s = is_v ? c.v_tail_strides : c.k_tail_strides;
+      const int row = tail_first + (j >> 1) * kPagedStep;
+      const __half* src = static_cast<const __half*>(is_v ? c.v_tail : c.k_tail) + b * s.batch + kv_head * s.head + row * s.row;
+      const int ch = lane % Tail::kChunks;
+#pragma unroll
+      for (int it = 0; it < Tail::kLoads; ++it) {
+        const int r = it * Tail::kCopyRows + lane / Tail::kChunks;
+        const bool ok = row + r < tail_end && ch * 8 < c.head_dim;
+        cp_async_16_bytes(ring.base + fill * L::kStageBytes + Tail::place(r, ch), ok ? src + r * s.row + ch * 8 : src, ok ? 16u : 0u);
+      }
+      cp_async_commit();
+    }
+    fill = fill + 1 < L::kStages ? fill + 1 : 0;
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) issue(i);
+  k_scales = scale_of(c.k_scales, pages);
+  v_scales = scale_of(c.v_scales, pages);
+
+  // ---- queries and their limits, under the first loads ----
+  const int seen_end = kScaled ? n : page_end;  // (pages of 8-bit caches are full)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = nt * 8 + g;
+    const int r = row0 + row;
+    const __half* q = static_cast<const __half*>(p.q) + b * p.q_strides.batch + r / group * p.q_strides.row +
+                      (kv_head * group + r % group) * p.q_strides.head;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int col = (ks / (kQ / 4)) * 4 * kQ + t * kQ + (ks % (kQ / 4)) * 4;
+      uint2 x = make_uint2(0u, 0u);
+      if (row < rows_valid && col < c.head_dim) x = *reinterpret_cast<const uint2*>(q + col);
+      st.q[ks][0][nt] = x.x;
+      st.q[ks][1][nt] = x.y;
+    }
+#pragma unroll
     for (int e = 0; e < 2; ++e) {
-      limit[nt][e] = min(pos_end, n - p.rows + (row0 + nt * 8 + 2 * t + e) / group + 1);
-      st.m[nt][e] = -INFINITY;
+      st.limit[nt][e] = min(seen_end, n - p.rows + (row0 + nt * 8 + 2 * t + e) / group + 1);
+      st.m[nt][e] = 0.f;
+      st.most[nt][e] = -INFINITY;
       st.l[nt][e] = 0.f;
     }
 #pragma unroll
@@ -673,151 +895,245 @@ __global__ void __launch_bounds__(kPagedThreads) fal_paged_splitk_kernel(const P
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[nt][j][e] = 0.f;
   }
-  const int min_limit = min(pos_end, n - p.rows + row0 / group + 1);
-  const float c2 = p.scale * kLog2e;
-  const uint32_t ring = smem_u32(paged_smem) + warp * L::kRingBytes;
-  const uint32_t ring_scales = smem_u32(paged_smem) + L::kScaleOffset + warp * L::kScaleBytes;
+  st.min_limit = min(seen_end, n - p.rows + row0 / group + 1);
+  st.c2 = p.scale * kLog2e;
 
-  // Q as the first product's second operand: of every group of four columns that a lane's key fragment holds, two each.
-  auto load_q = [&](auto elem) {
-    constexpr int kE = 16 / Elem<decltype(elem)>::kBytes;  // columns of a lane's 16 bytes
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = nt * 8 + g;
-      const __half* q = nullptr;
-      if (row < rows_valid)
-        q = static_cast<const __half*>(p.q) + b * p.q_strides.batch + (row0 + row) / group * p.q_strides.row +
-            (kv_head * group + (row0 + row) % group) * p.q_strides.head;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const int col = (ks / (kE / 4)) * 4 * kE + t * kE + (ks % (kE / 4)) * 4;
-        uint2 x = make_uint2(0u, 0u);
-        if (row < rows_valid && col < c.head_dim) x = *reinterpret_cast<const uint2*>(q + col);
-        st.q[ks][0][nt] = x.x;
-        st.q[ks][1][nt] = x.y;
-      }
+  const uint32_t k_read = Tile::k_read(g, t), v_read = Tile::kSliceBytes + Tile::v_read(g, t);
+  uint32_t drain = 0;
+  for (int i = 0; i < slices; ++i) {
+    issue(i + kAhead);
+    const uint32_t stage = ring.base + drain * L::kStageBytes;
+    const int key0 = first + i * kPagedStep;
+    float k_scale = 1.f, v_scale = 1.f;
+    if constexpr (kScaled) {
+      const bool before = (min(i + kAhead, slices - 1) ^ i) >= 32;
+      k_scale = __shfl_sync(0xffffffffu, before ? last_k : k_scales, i & 31);
+      v_scale = __shfl_sync(0xffffffffu, before ? last_v : v_scales, i & 31);
     }
-  };
-  const int real_bytes = c.head_dim;  // x the element's bytes
-  if (is_tail) {
-    if constexpr (Elem<T>::kScaled) {
-      load_q(__half{});
-      PagedSource<__half> src{};
-      src.k_row = c.k_tail_strides.row * 2;
-      src.v_row = c.v_tail_strides.row * 2;
-      src.k = static_cast<const uint8_t*>(c.k_tail) + (b * c.k_tail_strides.batch + kv_head * c.k_tail_strides.head) * 2 -
-              in_pages * src.k_row;
-      src.v = static_cast<const uint8_t*>(c.v_tail) + (b * c.v_tail_strides.batch + kv_head * c.v_tail_strides.head) * 2 -
-              in_pages * src.v_row;
-      src.num_pages = 1;
-      paged_stream<D, __half, NT, L::kTailStages>(src, ring, ring_scales, pos0, pos_end, real_bytes / 8, c2, limit, min_limit, st);
+    mbar_wait(ring.barriers + drain * 8, (ring.phases >> drain) & 1u, ring.wait, kPagedBarrierId);
+    ring.phases ^= 1u << drain;
+    if (!kScaled && key0 + kPagedSlice > page_end) {
+      // whatever the page holds behind the entry's length: as V rows with weights of 0 its NaN would still reach the output
+      const int rows = page_end - key0;
+      for (int x = rows * (Tile::kBlockRow / 16) + lane; x < kPagedSlice * (Tile::kBlockRow / 16); x += 32)
+#pragma unroll
+        for (int block = 0; block < Tile::kBlocks; ++block)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(stage + Tile::kSliceBytes + block * Tile::kBlockBytes + x * 16), "r"(0) : "memory");
+      __syncwarp();
     }
-  } else {
-    load_q(T{});
-    constexpr int kB = Elem<T>::kBytes;
-    PagedSource<T> src{};
-    src.k = static_cast<const uint8_t*>(c.k_pages) + kv_head * c.k_strides.head * kB;
-    src.v = static_cast<const uint8_t*>(c.v_pages) + kv_head * c.v_strides.head * kB;
-    src.k_page = c.k_strides.batch * kB;
-    src.v_page = c.v_strides.batch * kB;
-    src.k_row = c.k_strides.row * kB;
-    src.v_row = c.v_strides.row * kB;
-    src.table = c.table + b * c.table_stride;
-    src.page_shift = c.page_shift;
-    src.num_pages = c.num_pages;
-    src.k_scales = c.k_scales + (Elem<T>::kScaled ? kv_head : 0);
-    src.v_scales = c.v_scales + (Elem<T>::kScaled ? kv_head : 0);
-    src.heads_kv = c.heads_kv;
-    src.status = p.status;
-    paged_stream<D, T, NT, L::kStages>(src, ring, ring_scales, pos0, pos_end, real_bytes * kB / 16, c2, limit, min_limit, st);
+    paged_scores<D, T, NT>(st, stage + k_read, key0, k_scale);
+    paged_output<D, T, NT>(st, stage + v_read, v_scale);
+    drain = drain + 1 < L::kStages ? drain + 1 : 0;
+    __syncwarp();  // all lanes are done with this stage before it is refilled
   }
+  if constexpr (kScaled) {
+    for (int j = 0; j < 2 * tail_slices; ++j) {
+      issue(slices + j + kAhead);
+      cp_async_wait<0>();
+      __syncwarp();
+      const uint32_t stage = ring.base + drain * L::kStageBytes;
+      if ((j & 1) == 0) paged_tail_scores<D, T, NT>(st, stage, in_pages + tail_first + (j >> 1) * kPagedStep);
+      else paged_tail_output<D, T, NT>(st, stage);
+      drain = drain + 1 < L::kStages ? drain + 1 : 0;
+      __syncwarp();
+    }
+  }
+}
+
+// What a pair of columns is exclusive-or'ed with where the warps' results lie: a number of its lane, below the pairs of a lane.
+template <int D, class T>
+__device__ __forceinline__ int paged_merge_mix(int pair) {
+  constexpr int kPairs = PagedTile<D, T>::kLaneCols / 2;
+  return (pair / kPairs >> 1) & (kPairs - 1) & 3;
+}
+
+// CTAs per SM: what shared memory holds, as far as the registers of a result of 8 NT rows allow.
+template <int D, class T, int NT>
+constexpr int paged_ctas_per_sm() {
+  const int by_memory = (227 << 10) / (PagedSmem<D, T>::bytes(8 * NT) + (2 << 10));
+  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 ? 4 : 3;
+  return by_memory < by_registers ? by_memory : by_registers;
+}
+
+template <int D, class T, int NT>
+__global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using L = PagedSmem<D, T>;
+  using Tile = PagedTile<D, T>;
+  constexpr int kRows = 8 * NT;
+  extern __shared__ __align__(128) uint8_t paged_smem_raw[];
+  __shared__ PagedSums sums;
+  __shared__ PagedCut shared_cut;
+  __shared__ int shared_b;
+  __shared__ __align__(8) uint64_t barriers[kPagedWarps][L::kStages];
+  __shared__ int abort_flag;
+  uint8_t* paged_smem = paged_smem_raw + (L::kAlign - smem_u32(paged_smem_raw) % L::kAlign) % L::kAlign;
+  if (threadIdx.x < kPagedWarps * L::kStages) mbar_init(smem_u32(&barriers[0][0] + threadIdx.x), 1);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
+  fence_mbar_init();
+  grid_dependency_wait();    // the append of this step's rows may still run up to here
+  grid_dependency_launch();
+  const PagedCache& c = p.c;
+  const int group = p.heads_q / c.heads_kv;
+  const int chunks = (p.rows * group + kRows - 1) / kRows;
+  const unsigned heads = c.heads_kv * chunks;  // units of an entry
+  const int unit = blockIdx.x % heads;
+  int b = -1;
+  PagedCut cut;
+  if (!paged_find(sums, cut, p, heads, blockIdx.x / heads, b, shared_cut, shared_b)) return;
+  const int part = static_cast<int>(blockIdx.x / heads - cut.group);
+  const int step0 = static_cast<int>(static_cast<int64_t>(cut.steps) * part / cut.parts);
+  const int step1 = static_cast<int>(static_cast<int64_t>(cut.steps) * (part + 1) / cut.parts);
+  const int kv_head = unit / chunks;
+  const int row0 = unit % chunks * kRows;  // of the KV head's rows * group query rows
+  const int rows_valid = min(kRows, p.rows * group - row0);
+  const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  PagedRing ring{smem_u32(paged_smem) + warp * L::kRingBytes, smem_u32(&barriers[warp][0]), 0u, WaitCtx{&abort_flag, p.status}};
+  PagedState<D, NT> st;
+  paged_piece<D, T, NT>(p, &k_map, &v_map, ring, b, cut.n, kv_head, row0, rows_valid, step0, step1, st);
   __syncthreads();  // the ring becomes the place of the warps' results
 
-  float* mo = reinterpret_cast<float*>(paged_smem);  // [warp][row][D]
-  float* mml = mo + kPagedWarps * kRows * D;         // [warp][row][2]
+  // (column pair c of a row is at c ^ (its lane / 2): eight lanes and four rows of a store hit different banks)
+  float* mo = reinterpret_cast<float*>(paged_smem);          // [warp][row][kPitch]
+  float* mml = mo + kPagedWarps * kRows * L::kPitch;         // [warp][row][2]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = warp * kRows + nt * 8 + 2 * t + e;
+    for (int x = 0; x < 2; ++x) {
+      const int row = warp * kRows + nt * 8 + 2 * t + x;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        *reinterpret_cast<float2*>(mo + row * D + g * (D / 8) + 2 * j) = make_float2(st.o[nt][j][e], st.o[nt][j][2 + e]);
-      float l = st.l[nt][e];
-      l += __shfl_xor_sync(0xffffffffu, l, 4);
-      l += __shfl_xor_sync(0xffffffffu, l, 8);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      if (g == 0) *reinterpret_cast<float2*>(mml + row * 2) = make_float2(st.m[nt][e], l);
+      for (int j = 0; j < D / 16; ++j) {
+        const int pair = Tile::column(g, j) / 2;
+        *reinterpret_cast<float2*>(mo + row * L::kPitch + (pair ^ paged_merge_mix<D, T>(pair)) * 2) =
+            make_float2(st.o[nt][j][x], st.o[nt][j][2 + x]);
+      }
+      if (g == 0)
+        *reinterpret_cast<float2*>(mml + row * 2) =
+            make_float2(st.most[nt][x] == -INFINITY ? -INFINITY : st.m[nt][x], st.l[nt][x] * (1.f / kSumFactor<T>));
     }
   }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < rows_valid * D; idx += kPagedThreads) {
-    const int r = idx / D, col = idx % D;
+  const int64_t slot = ((cut.slot + part) * heads + unit) * kRows;
+  for (int idx = threadIdx.x; idx < rows_valid * (D / 2); idx += kPagedThreads) {
+    const int r = idx / (D / 2), pair = idx % (D / 2);
     float most = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) most = fmaxf(most, mml[(w * kRows + r) * 2]);
     const float use = most == -INFINITY ? 0.f : most;
-    float o = 0.f, l = 0.f;
+    float o0 = 0.f, o1 = 0.f, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) {
       const float x = fast_exp2(mml[(w * kRows + r) * 2] - use);
-      o += x * mo[(w * kRows + r) * D + col];
+      const float2 y = *reinterpret_cast<const float2*>(mo + (w * kRows + r) * L::kPitch + (pair ^ paged_merge_mix<D, T>(pair)) * 2);
+      o0 += x * y.x;
+      o1 += x * y.y;
       l += x * mml[(w * kRows + r) * 2 + 1];
     }
-    const int64_t head = kv_head * group + (row0 + r) % group;
-    const int64_t at = ((static_cast<int64_t>(b) * p.rows + (row0 + r) / group) * p.heads_q + head) * p.splits + split;
-    p.part_o[at * D + col] = o;
-    if (col == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(most, l);
+    if (cut.parts == 1) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;  // (0: the row sees no key)
+      const int head = kv_head * group + (row0 + r) % group;
+      __half* out = static_cast<__half*>(p.o) + ((static_cast<int64_t>(b) * p.rows + (row0 + r) / group) * p.heads_q + head) * c.head_dim;
+      if (2 * pair < c.head_dim) *reinterpret_cast<uint32_t*>(out + 2 * pair) = pack_half2(o0 * inv, o1 * inv);
+    } else {
+      *reinterpret_cast<float2*>(p.part_o + (slot + r) * D + 2 * pair) = make_float2(o0, o1);
+      if (pair == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + r) * 2) = make_float2(most, l);
+    }
   }
 }
 
-template <int D, int WARPS>
+// Merges the parts of the entries that were cut, and writes the zeros of entries without positions.
+template <int D, int NT>
 __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(const PagedAttnParams p) {
-  constexpr int kRows = kCombineThreads / (32 * WARPS);
-  const int tid = threadIdx.x % (32 * WARPS);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (32 * WARPS);
-  const bool row_ok = row < static_cast<int64_t>(p.c.batch) * p.rows * p.heads_q;
-  int n = 0;
-  if (row_ok) {
-    const int len = paged_len(p.c, static_cast<int>(row / (static_cast<int64_t>(p.rows) * p.heads_q)));
-    const int in_pages = paged_len_in_pages(p.c, len);
-    n = ((in_pages - 1) >> paged_split_shift(p, in_pages)) + 1 + (len > in_pages ? 1 : 0);
-  }
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * p.splits;
-  const float4* po = reinterpret_cast<const float4*>(p.part_o) + row * p.splits * (D / 4);
-  combine_row<D, WARPS>(tid, row_ok, n, ml, po, static_cast<__half*>(p.o) + row * p.c.head_dim, p.c.head_dim, nullptr);
+  static_assert(kCombineThreads == kPagedThreads, "a block finds an entry's cut");
+  constexpr int kRows = 8 * NT;
+  __shared__ PagedSums sums;
+  __shared__ PagedCut shared_cut;
+  __shared__ int shared_b;
+  const PagedCache& c = p.c;
+  const int group = p.heads_q / c.heads_kv;
+  const int chunks = (p.rows * group + kRows - 1) / kRows;
+  const int heads = c.heads_kv * chunks;
+  const int row = blockIdx.x;
+  const int head = row % p.heads_q, token = row / p.heads_q % p.rows;
+  int b = row / p.heads_q / p.rows;
+  PagedCut cut;
+  // (the lengths were not written by the grid before, and whatever wrote them ended before that grid let this one start)
+  paged_find(sums, cut, p, heads, 0, b, shared_cut, shared_b);
+  if (cut.parts == 1) return;
+  const int in_head = token * group + head % group;  // query row of the KV head
+  const int64_t first = (cut.slot * heads + head / group * chunks + in_head / kRows) * kRows + in_head % kRows;
+  auto at = [&](int i) { return first + static_cast<int64_t>(i) * heads * kRows; };
+  combine_row<D, kCombineThreads / 32>(threadIdx.x, true, cut.parts, reinterpret_cast<const float2*>(p.part_ml),
+                                       reinterpret_cast<const float4*>(p.part_o), at,
+                                       static_cast<__half*>(p.o) + static_cast<int64_t>(row) * c.head_dim, c.head_dim, nullptr);
 }
 
+// CTAs of the split-K kernel that the GPU holds at once.
 template <int D, class T, int NT>
-cudaError_t launch_splitk_t(const PagedAttnParams& p, cudaStream_t stream) {
+cudaError_t resident_ctas(int* ctas) {
   auto kern = fal_paged_splitk_kernel<D, T, NT>;
   constexpr int kBytes = PagedSmem<D, T>::bytes(8 * NT);
   static DeviceOnce configured;
-  cudaError_t e = configured.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes); });
+  static int per_device[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  const int group = p.heads_q / p.c.heads_kv;
-  const dim3 grid(p.c.heads_kv * ((p.rows * group + 8 * NT - 1) / (8 * NT)), p.splits, p.c.batch);
-  e = launch_dependent(kern, grid, dim3(kPagedThreads), kBytes, stream, p);
+  e = configured.run([&] {
+    cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    int per_sm = 0, sms = 0;
+    if (err == cudaSuccess) err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kPagedThreads, kBytes);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    per_device[dev] = per_sm * sms;
+    return err == cudaSuccess && per_device[dev] <= 0 ? cudaErrorLaunchOutOfResources : err;
+  });
+  if (e == cudaSuccess) *ctas = per_device[dev];
+  return e;
+}
+
+template <int D, class T, int NT>
+cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) {
+  int resident = 0;
+  cudaError_t e = resident_ctas<D, T, NT>(&resident);
   if (e != cudaSuccess) return e;
-  const int64_t rows = static_cast<int64_t>(p.c.batch) * p.rows * p.heads_q;
-  if (p.splits * p.kernel_dim * 4 <= (rows >= 256 ? 4096 : 2048))
-    return launch_dependent(fal_paged_combine_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kCombineThreads), 0, stream, p);
-  return launch_dependent(fal_paged_combine_kernel<D, 4>, dim3(static_cast<unsigned>(rows)), dim3(kCombineThreads), 0, stream, p);
+  const int64_t chunks = (static_cast<int64_t>(p.rows) * (p.heads_q / p.c.heads_kv) + 8 * NT - 1) / (8 * NT);
+  const int64_t heads = p.c.heads_kv * chunks;
+  p.parts = kPagedWaves * resident;
+  // Parts of all entries: one each, and p.parts / heads more; and no more than kPagedMinSteps make of full entries.
+  const int64_t steps = ((static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) + kPagedStep - 1) / kPagedStep + 1;
+  const int64_t groups = std::min<int64_t>(p.c.batch + p.parts / heads, p.c.batch * ((steps + kPagedMinSteps - 1) / kPagedMinSteps));
+  // (a cut entry is longer than one part: its parts are at most twice its steps in parts)
+  p.slots = std::min<int64_t>(groups, 2 * (p.parts / heads) + 2) * heads;
+  if (groups * heads > 0x7fffffff) return cudaErrorInvalidValue;
+  if (maps == nullptr) return e;
+  p.part_ml = p.part_o + p.slots * 8 * NT * D;
+  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads), PagedSmem<D, T>::bytes(8 * NT), stream, p, maps[0], maps[1]);
+  if (e != cudaSuccess) return e;
+  const unsigned rows = static_cast<unsigned>(p.c.batch) * p.rows * p.heads_q;
+  return launch_dependent(fal_paged_combine_kernel<D, NT>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
 }
 
 template <int D, class T>
-cudaError_t launch_splitk_d(const PagedAttnParams& p, cudaStream_t stream) {
+cudaError_t splitk_d(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) {
   if constexpr (D < 256) {
-    if (paged_rows_per_cta(p.rows * (p.heads_q / p.c.heads_kv), D) == 16) return launch_splitk_t<D, T, 2>(p, stream);
+    if (paged_rows_per_cta(p.rows * (p.heads_q / p.c.heads_kv), D) == 16) return splitk_t<D, T, 2>(p, maps, stream);
   }
-  return launch_splitk_t<D, T, 1>(p, stream);
+  return splitk_t<D, T, 1>(p, maps, stream);
 }
 
 template <class T>
-cudaError_t launch_splitk(const PagedAttnParams& p, cudaStream_t stream) {
-  if (p.kernel_dim == 64) return launch_splitk_d<64, T>(p, stream);
-  if (p.kernel_dim == 128) return launch_splitk_d<128, T>(p, stream);
-  return launch_splitk_d<256, T>(p, stream);
+cudaError_t splitk(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) {
+  if (p.kernel_dim == 64) return splitk_d<64, T>(p, maps, stream);
+  if (p.kernel_dim == 128) return splitk_d<128, T>(p, maps, stream);
+  return splitk_d<256, T>(p, maps, stream);
+}
+
+cudaError_t splitk(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) {
+  if (p.c.type == kPagedF16) return splitk<__half>(p, maps, stream);
+  if (p.c.type == kPagedS8) return splitk<S8>(p, maps, stream);
+  return splitk<E4M3>(p, maps, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -895,11 +1211,9 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream)
   return p.c.type == kPagedS8 ? launch_seal<S8>(p, stream) : launch_seal<E4M3>(p, stream);
 }
 
-cudaError_t launch_paged_attn(const PagedAttnParams& p, cudaStream_t stream) {
-  if (p.c.type == kPagedF16) return launch_splitk<__half>(p, stream);
-  if (p.c.type == kPagedS8) return launch_splitk<S8>(p, stream);
-  return launch_splitk<E4M3>(p, stream);
-}
+cudaError_t paged_attn_plan(PagedAttnParams& p) { return splitk(p, nullptr, nullptr); }
+
+cudaError_t launch_paged_attn(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) { return splitk(p, maps, stream); }
 
 cudaError_t launch_paged_gather(const PagedGatherParams& p, cudaStream_t stream) {
   const int64_t tasks = (static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) * (p.c.head_dim / 16);
