@@ -322,10 +322,12 @@ cudaError_t launch_seal(const PagedAppendParams& p, cudaStream_t stream) {
 // make a few CTAs for every place on the GPU, whatever the lengths are; the units of one part are CTAs next to each other,
 // because their rows are next to each other in memory where a page holds all heads of a position.  Parts of a cut entry go
 // to the workspace and a second kernel merges them; a CTA that has all keys of its unit writes the result itself.
+#ifndef FAL_PAGED_STAGES
+#define FAL_PAGED_STAGES 2
+#endif
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kPagedSlice = 16;
-constexpr int kPagedStep = kPagedWarps * kPagedSlice;  // keys
 
 template <class T>
 struct Elem {
@@ -337,6 +339,12 @@ struct Elem<__half> {
   static constexpr bool kScaled = false;
   static constexpr int kBytes = 2;
 };
+// Slices that a warp takes at a time, of one page or of two.
+template <int D, class T, int NT>
+constexpr int kPagedSlices = Elem<T>::kScaled && NT == 1 && D <= 128 ? 2 : 1;
+template <int D, class T, int NT>
+constexpr int kPagedStep = kPagedWarps * kPagedSlice * kPagedSlices<D, T, NT>;  // keys of a step of a CTA
+
 constexpr float kS8Bias = 1152.f;  // what widen_biased adds to a code
 
 // Four 8-bit codes as two pairs of fp16.
@@ -435,17 +443,17 @@ struct PagedTailTile {
   static __device__ __forceinline__ uint32_t place(int row, int ch) { return row * kRowBytes + (ch ^ (row & 7)) * 16; }
 };
 
-template <int D, class T>
+template <int D, class T, int NT>
 struct PagedSmem {
-  static constexpr bool kScaled = Elem<T>::kScaled;
-  static constexpr int kStages = D == 64 ? 4 : 3;
-  static constexpr int kStageBytes = 2 * PagedTile<D, T>::kSliceBytes;  // K and V; or one of a slice of the tail
+  static constexpr int kStages = D == 64 && kPagedSlices<D, T, NT> == 1 ? 4 : kPagedSlices<D, T, NT> == 1 ? 3 : FAL_PAGED_STAGES;
+  static constexpr int kTensorBytes = kPagedSlices<D, T, NT> * PagedTile<D, T>::kSliceBytes;
+  static constexpr int kStageBytes = 2 * kTensorBytes;      // K, then V; or K or V of a slice of the tail
   static constexpr int kRingBytes = kStages * kStageBytes;  // per warp
   static constexpr int kPipeBytes = kPagedWarps * kRingBytes;
   static constexpr int kPitch = D + 4;  // floats of a row of a warp's result
-  static constexpr int merge_bytes(int rows) { return kPagedWarps * rows * (kPitch + 2) * 4; }
+  static constexpr int kMergeBytes = kPagedWarps * 8 * NT * (kPitch + 2) * 4;
   static constexpr int kAlign = 1024;   // of TMA's permuted blocks
-  static constexpr int bytes(int rows) { return (kPipeBytes > merge_bytes(rows) ? kPipeBytes : merge_bytes(rows)) + kAlign; }
+  static constexpr int kBytes = (kPipeBytes > kMergeBytes ? kPipeBytes : kMergeBytes) + kAlign;
 };
 
 // ---- the deal ----
@@ -453,9 +461,10 @@ __device__ __forceinline__ int paged_len_in_pages(const PagedCache& c, int n) {
   return c.type == kPagedF16 ? n : n >> c.page_shift << c.page_shift;
 }
 // Steps of one unit of an entry with n positions: those of its pages, then those of its tail.
+template <int STEP>
 __device__ __forceinline__ int paged_steps(const PagedCache& c, int n) {
   const int in_pages = paged_len_in_pages(c, n);
-  return (in_pages + kPagedStep - 1) / kPagedStep + (n - in_pages + kPagedStep - 1) / kPagedStep;
+  return (in_pages + STEP - 1) / STEP + (n - in_pages + STEP - 1) / STEP;
 }
 
 // Sums over the block's threads up to this one, and over all of them.
@@ -481,8 +490,8 @@ __device__ __forceinline__ uint64_t paged_block_sum(PagedSums& sums, uint64_t mi
   return mine;
 }
 
-// A part is at least kPagedMinSteps long, and otherwise as long as makes `p.parts` CTAs of all units: kPagedWaves for every place.
-constexpr int kPagedMinSteps = 4;
+// A part is at least kPagedMinKeys long, and otherwise as long as makes `p.parts` CTAs of all units: kPagedWaves for every place.
+constexpr int kPagedMinKeys = 256;
 #ifndef FAL_PAGED_WAVES
 #define FAL_PAGED_WAVES 2
 #endif
@@ -497,7 +506,8 @@ struct PagedCut {
   int64_t slot;   // the same, of those that are cut (their results go to the workspace)
 };
 // Finds the entry `b` (if b >= 0), or else the one that has part `group` of all entries' parts (b is set).  False: there is none.
-// Called by all threads of a block.
+// Called by all threads of a block.  STEP: keys of a step.
+template <int STEP>
 __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, const PagedAttnParams& p, int64_t heads, int64_t group, int& b,
                                            PagedCut& shared_cut, int& shared_b) {
   const PagedCache& c = p.c;
@@ -508,15 +518,15 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, c
     const int e = base + threadIdx.x;
     n = e < c.batch ? paged_len(c, e) : 0;
     uint64_t all;
-    paged_block_sum(sums, paged_steps(c, n), all);
+    paged_block_sum(sums, paged_steps<STEP>(c, n), all);
     total += all;
   }
-  const int64_t length = max((total * heads + p.parts - 1) / p.parts, static_cast<int64_t>(kPagedMinSteps));
+  const int64_t length = max((total * heads + p.parts - 1) / p.parts, static_cast<int64_t>(kPagedMinKeys / STEP));
   uint64_t before = 0;  // parts in the low half, parts of cut entries in the high half
   for (int base = 0; base <= last; base += kPagedThreads) {
     const int e = base + threadIdx.x;
     if (base > 0) n = e < c.batch ? paged_len(c, e) : 0;
-    const int steps = paged_steps(c, n);
+    const int steps = paged_steps<STEP>(c, n);
     const uint64_t parts = (steps + length - 1) / length;
     uint64_t all;
     const uint64_t upto = before + paged_block_sum(sums, parts | (parts > 1 ? parts << 32 : 0), all);
@@ -540,11 +550,11 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, c
 }
 
 // ---- one piece of a unit ----
-template <int D, int NT>
+template <int D, int NT, int H>
 struct PagedState {
   uint32_t q[D / 16][2][NT];
-  uint32_t p[NT][2];  // the weights of the slice in hand, as the second product's operand
-  float sum[NT][4];   // of those weights, times kSumFactor
+  uint32_t p[H][NT][2];  // the weights of the slices in hand, as the second product's operand
+  float sum[H][NT][4];   // of those weights, times kSumFactor
   float o[NT][D / 16][4];
   float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far
   float most[NT][2];  // what an exponent may be before the reference moves: 8, or -infinity before the first key
@@ -561,36 +571,47 @@ constexpr float kSumFactor = std::is_same<T, S8>::value ? -kS8Bias : 1.f;
 template <class T>
 constexpr uint32_t kSumOperand = std::is_same<T, S8>::value ? 0xe480e480u : 0x3c003c00u;  // two of it in fp16
 
-// What follows the first product: scores s of this lane's keys key and key + 8 for query rows 2 t and 2 t + 1 of every eight
-// become weights.  W: the type of the pages (kSumFactor).
-template <int D, class W, int NT>
-__device__ __forceinline__ void paged_weights(PagedState<D, NT>& st, float (&s)[NT][4], int key0, int key, float k_scale) {
-  const float f = st.c2 * k_scale;
-  if (key0 + kPagedSlice > st.min_limit) {
+// What follows the first product: scores s of this lane's keys key and key + 8 of H slices, from key0 on, for query rows 2 t and
+// 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have.  W: the type of the pages (kSumFactor).
+template <int H, class W, int D, int NT, int HS>
+__device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
+                                              const float (&k_scale)[H]) {
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const float f = st.c2 * k_scale[h];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = key + (e >> 1) * 8 >= st.limit[nt][e & 1] ? -INFINITY : s[nt][e] * f;
-  } else {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] *= f;
+      for (int e = 0; e < 4; ++e) s[h][nt][e] *= f;
   }
+  if (key0 + H * kPagedSlice > min(st.min_limit, end)) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key + h * kPagedSlice + (e >> 1) * 8 >= min(st.limit[nt][e & 1], end)) s[h][nt][e] = -INFINITY;
+  }
+  float most[NT][2];
   bool grows = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) grows = grows || fmaxf(s[nt][e], s[nt][2 + e]) - st.m[nt][e] > st.most[nt][e];
+    for (int e = 0; e < 2; ++e) {
+      most[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+      if (H == 2) most[nt][e] = fmaxf(most[nt][e], fmaxf(s[H - 1][nt][e], s[H - 1][nt][2 + e]));
+      grows = grows || most[nt][e] - st.m[nt][e] > st.most[nt][e];
+    }
   // The reference follows the largest score only when a weight would exceed 2^8: the output is rescaled a few times per
-  // piece, and the largest is looked for across the lanes only then.
+  // part, and the largest is looked for across the lanes only then.
   if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float alpha[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = fmaxf(s[nt][e], s[nt][2 + e]);
+        float x = most[nt][e];
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -614,23 +635,25 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT>& st, float (&s)[
     }
   }
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int h = 0; h < H; ++h)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[nt][e] = fast_exp2(s[nt][e] - st.m[nt][e & 1]);
-    st.p[nt][0] = movmatrix(pack_half2(s[nt][0], s[nt][1]));
-    st.p[nt][1] = movmatrix(pack_half2(s[nt][2], s[nt][3]));
-    // sums of the weights as they are rounded, which is what the output is divided by
-    const uint32_t factor[4] = {kSumOperand<W>, kSumOperand<W>, kSumOperand<W>, kSumOperand<W>};
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_16816_from(st.sum[nt], factor, st.p[nt][0], st.p[nt][1], zero);
-    st.l[nt][0] += st.sum[nt][0];
-    st.l[nt][1] += st.sum[nt][1];
-  }
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[h][nt][e] = fast_exp2(s[h][nt][e] - st.m[nt][e & 1]);
+      st.p[h][nt][0] = movmatrix(pack_half2(s[h][nt][0], s[h][nt][1]));
+      st.p[h][nt][1] = movmatrix(pack_half2(s[h][nt][2], s[h][nt][3]));
+      // sums of the weights as they are rounded, which is what the output is divided by
+      const uint32_t factor[4] = {kSumOperand<W>, kSumOperand<W>, kSumOperand<W>, kSumOperand<W>};
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816_from(st.sum[h][nt], factor, st.p[h][nt][0], st.p[h][nt][1], zero);
+      st.l[nt][0] += st.sum[h][nt][0];
+      st.l[nt][1] += st.sum[h][nt][1];
+    }
 }
 
 // s (+)= the product of 16 keys' columns of one step and Q's.
-template <int D, int NT>
-__device__ __forceinline__ void paged_score_step(PagedState<D, NT>& st, float (&s)[NT][4], const uint32_t (&a)[4], int ks) {
+template <int D, int NT, int H>
+__device__ __forceinline__ void paged_score_step(PagedState<D, NT, H>& st, float (&s)[NT][4], const uint32_t (&a)[4], int ks) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     if (ks == 0) {
@@ -642,12 +665,11 @@ __device__ __forceinline__ void paged_score_step(PagedState<D, NT>& st, float (&
   }
 }
 
-// Weights of a slice of a page, keys key0 ...; kb: its shared address + k_read.
-template <int D, class T, int NT>
-__device__ __forceinline__ void paged_scores(PagedState<D, NT>& st, uint32_t kb, int key0, float k_scale) {
+// Scores of a slice of a page; kb: its shared address + k_read.
+template <class T, int D, int NT, int H>
+__device__ __forceinline__ void paged_scores(PagedState<D, NT, H>& st, float (&s)[NT][4], uint32_t kb) {
   using Tile = PagedTile<D, T>;
   constexpr int kSteps = Elem<T>::kScaled ? 4 : 2;  // of 16 columns in four lanes' 16 bytes
-  float s[NT][4];
 #pragma unroll
   for (int seg = 0; seg < Tile::kRowBytes / 64; ++seg) {
     uint32_t r0[4], r1[4];
@@ -669,12 +691,11 @@ __device__ __forceinline__ void paged_scores(PagedState<D, NT>& st, uint32_t kb,
       paged_score_step(st, s, a, seg * kSteps + k);
     }
   }
-  paged_weights<D, T, NT>(st, s, key0, key0 + Tile::key_of((threadIdx.x & 31) >> 2), k_scale);
 }
 
-// O^T += V^T P^T of a slice of a page; vb: its shared address + v_read.
-template <int D, class T, int NT>
-__device__ __forceinline__ void paged_output(PagedState<D, NT>& st, uint32_t vb, float v_scale) {
+// O^T += V^T P^T of the h-th slice, of a page; vb: its shared address + v_read.
+template <class T, int D, int NT, int H>
+__device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, uint32_t vb, float v_scale) {
   using Tile = PagedTile<D, T>;
   auto product = [&](int j, const uint32_t (&a)[4]) {
 #pragma unroll
@@ -683,10 +704,10 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT>& st, uint32_t vb,
         float x[4];
         if constexpr (std::is_same<T, S8>::value) {
           // (sums of codes + 1 152 and the sums that take it off cancel within a slice: 2^-23 of 1 152, 2^-13 of a code's step)
-          mma_16816_from(x, a, st.p[nt][0], st.p[nt][1], st.sum[nt]);
+          mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], st.sum[h][nt]);
         } else {
           const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_16816_from(x, a, st.p[nt][0], st.p[nt][1], zero);
+          mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], zero);
         }
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
@@ -694,7 +715,7 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT>& st, uint32_t vb,
           unpack_f32x2(y, st.o[nt][j][e], st.o[nt][j][e + 1]);
         }
       } else {
-        mma_16816(st.o[nt][j], a, st.p[nt][0], st.p[nt][1]);
+        mma_16816(st.o[nt][j], a, st.p[h][nt][0], st.p[h][nt][1]);
       }
     }
   };
@@ -728,11 +749,11 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT>& st, uint32_t vb,
 }
 
 // The same of a slice of the tail at shared address base; K and V are there one after the other.
-template <int D, class T, int NT>
-__device__ __forceinline__ void paged_tail_scores(PagedState<D, NT>& st, uint32_t base, int key0) {
+template <class T, int D, int NT, int H>
+__device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint32_t base, int key0, int end) {
   using Tail = PagedTailTile<D, T>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float s[NT][4];
+  float s[1][NT][4];
 #pragma unroll
   for (int seg = 0; seg < D / 64; ++seg) {
     uint32_t r0[8], r1[8];
@@ -744,13 +765,14 @@ __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT>& st, uint32_
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t a[4] = {r0[2 * k], r1[2 * k], r0[2 * k + 1], r1[2 * k + 1]};
-      paged_score_step(st, s, a, seg * 4 + k);
+      paged_score_step(st, s[0], a, seg * 4 + k);
     }
   }
-  paged_weights<D, T, NT>(st, s, key0, key0 + g, 1.f);
+  const float scale[1] = {1.f};
+  paged_weights<1, T>(st, s, key0, key0 + g, end, scale);
 }
-template <int D, class T, int NT>
-__device__ __forceinline__ void paged_tail_output(PagedState<D, NT>& st, uint32_t base) {
+template <class T, int D, int NT, int H>
+__device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint32_t base) {
   using Tile = PagedTile<D, T>;
   using Tail = PagedTailTile<D, T>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -764,7 +786,7 @@ __device__ __forceinline__ void paged_tail_output(PagedState<D, NT>& st, uint32_
       const uint32_t a[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
                              __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_16816(st.o[nt][j + k], a, st.p[nt][0], st.p[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) mma_16816(st.o[nt][j + k], a, st.p[0][nt][0], st.p[0][nt][1]);
     }
   }
 }
@@ -777,35 +799,45 @@ struct PagedRing {
   WaitCtx wait;
 };
 constexpr int kPagedBarrierId = 60;
+constexpr int kNoSlice = -2147483647;  // in place of a page: beyond the part
 
 // Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
 template <int D, class T, int NT>
 __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, PagedRing& ring,
                                             int b, int n, int kv_head, int row0, int rows_valid, int step0, int step1,
-                                            PagedState<D, NT>& st) {
-  using L = PagedSmem<D, T>;
+                                            PagedState<D, NT, kPagedSlices<D, T, NT>>& st) {
+  using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
   constexpr bool kScaled = Elem<T>::kScaled;
+  constexpr int kH = kPagedSlices<D, T, NT>;
+  constexpr int kKeys = kH * kPagedSlice;  // of a warp's turn
+  constexpr int kStep = kPagedStep<D, T, NT>;
   constexpr int kQ = 16 / Elem<T>::kBytes;  // neighbouring columns of a lane in Q's layout
   constexpr int kAhead = L::kStages - 1;
   const PagedCache& c = p.c;
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = p.heads_q / c.heads_kv;
   const int in_pages = paged_len_in_pages(c, n);
-  const int page_steps = (in_pages + kPagedStep - 1) / kPagedStep;
+  const int page_steps = (in_pages + kStep - 1) / kStep;
 
-  // this warp's slices: key0 = first + i * 64
-  const int first = step0 * kPagedStep + warp * kPagedSlice;
-  const int page_end = min(step1 * kPagedStep, in_pages);
-  const int slices = page_end > first ? (page_end - first + kPagedStep - 1) / kPagedStep : 0;
-  const int tail_first = (max(step0, page_steps) - page_steps) * kPagedStep + warp * kPagedSlice;  // row of the tail
-  const int tail_end = kScaled ? min((step1 - page_steps) * kPagedStep, n - in_pages) : 0;
-  const int tail_slices = tail_end > tail_first ? (tail_end - tail_first + kPagedStep - 1) / kPagedStep : 0;
+  // this warp's turns: keys first + i * kStep ... + kKeys - 1
+  const int first = step0 * kStep + warp * kKeys;
+  const int page_end = min(step1 * kStep, in_pages);
+  const int turns = page_end > first ? (page_end - first + kStep - 1) / kStep : 0;
+  // and its slices of the tail: rows tail_first + i * 64 ... + 15
+  const int tail_first = (max(step0, page_steps) - page_steps) * kStep + warp * kPagedSlice;
+  const int tail_end = kScaled ? min((step1 - page_steps) * kStep, n - in_pages) : 0;
+  constexpr int kTailStep = kPagedWarps * kPagedSlice;
+  const int tail_slices = tail_end > tail_first ? (tail_end - tail_first + kTailStep - 1) / kTailStep : 0;
 
   // Pages and scales of 32 slices at a time, one to a lane: of the slices whose loads are being issued, of the 32 before them
   // (some of which are still to be worked on), and of the 32 behind them.
+  constexpr int kBatch = 32 / kH;  // turns
   const int32_t* table = c.table + b * c.table_stride;
-  auto pages_of = [&](int i) { return i + lane < slices ? __ldg(table + ((first + (i + lane) * kPagedStep) >> c.page_shift)) : 0; };
+  auto pages_of = [&](int i) {
+    const int key = first + (i + lane / kH) * kStep + lane % kH * kPagedSlice;
+    return key < page_end ? __ldg(table + (key >> c.page_shift)) : kNoSlice;
+  };
   auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages); };
   auto scale_of = [&](const float* scales, int page) {
     return kScaled && there(page) ? __ldg(scales + static_cast<int64_t>(page) * c.heads_kv + kv_head) : 0.f;
@@ -814,42 +846,50 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
   float k_scales = 0.f, v_scales = 0.f, next_k = 0.f, next_v = 0.f, last_k = 0.f, last_v = 0.f;
   uint32_t fill = 0;  // stage that the next loads go to
   auto issue = [&](int i) {
-    if (i < slices) {
-      if ((i & 31) == 0 && i > 0) {
+    if (i < turns) {
+      const int in_batch = i & (kBatch - 1);
+      if (in_batch == 0 && i > 0) {
         pages = next_pages;
         last_k = k_scales;
         last_v = v_scales;
         k_scales = next_k;
         v_scales = next_v;
       }
-      if ((i & 31) == 4) next_pages = pages_of((i & ~31) + 32);
-      if (kScaled && (i & 31) == 20) {
+      if (in_batch == kBatch / 8) next_pages = pages_of((i & ~(kBatch - 1)) + kBatch);
+      if (kScaled && in_batch == kBatch * 5 / 8) {
         next_k = scale_of(c.k_scales, next_pages);
         next_v = scale_of(c.v_scales, next_pages);
       }
-      int page = __shfl_sync(0xffffffffu, pages, i & 31);
-      const int row = (first + i * kPagedStep) & ((1 << c.page_shift) - 1);
+      int page[kH];
+#pragma unroll
+      for (int h = 0; h < kH; ++h) page[h] = __shfl_sync(0xffffffffu, pages, in_batch * kH + h);
+      const int key0 = first + i * kStep;
       if (elect_one()) {
         const uint32_t bar = ring.barriers + fill * 8;
         const uint32_t stage = ring.base + fill * L::kStageBytes;
-        if (!there(page)) {  // (TMA fills a box outside of the tensor with zeros)
-          page = c.num_pages;
-          if (p.status) atomicCAS(p.status, 0, kDevNoPage);
-        }
         mbar_arrive_expect_tx(bar, L::kStageBytes);
 #pragma unroll
-        for (int x = 0; x < Tile::kBlocks; ++x) {
-          const int column = x * Tile::kBlockRow / Elem<T>::kBytes;
-          tma_load_4d(stage + x * Tile::kBlockBytes, k_map, bar, column, row, kv_head, page);
-          tma_load_4d(stage + Tile::kSliceBytes + x * Tile::kBlockBytes, v_map, bar, column, row, kv_head, page);
+        for (int h = 0; h < kH; ++h) {
+          const int row = (key0 + h * kPagedSlice) & ((1 << c.page_shift) - 1);
+          if (!there(page[h])) {  // (TMA fills a box outside of the tensor with zeros)
+            if (page[h] != kNoSlice && p.status) atomicCAS(p.status, 0, kDevNoPage);
+            page[h] = c.num_pages;
+          }
+#pragma unroll
+          for (int x = 0; x < Tile::kBlocks; ++x) {
+            const int column = x * Tile::kBlockRow / Elem<T>::kBytes;
+            const uint32_t at = stage + h * Tile::kSliceBytes + x * Tile::kBlockBytes;
+            tma_load_4d(at, k_map, bar, column, row, kv_head, page[h]);
+            tma_load_4d(at + L::kTensorBytes, v_map, bar, column, row, kv_head, page[h]);
+          }
         }
       }
-    } else if (kScaled && i < slices + 2 * tail_slices) {  // K, then V of a slice of the tail
+    } else if (kScaled && i < turns + 2 * tail_slices) {  // K, then V of a slice of the tail
       using Tail = PagedTailTile<D, T>;
-      const int j = i - slices;
+      const int j = i - turns;
       const bool is_v = (j & 1) != 0;
       const RowStrides& s = is_v ? c.v_tail_strides : c.k_tail_strides;
-      const int row = tail_first + (j >> 1) * kPagedStep;
+      const int row = tail_first + (j >> 1) * kTailStep;
       const __half* src = static_cast<const __half*>(is_v ? c.v_tail : c.k_tail) + b * s.batch + kv_head * s.head + row * s.row;
       const int ch = lane % Tail::kChunks;
 #pragma unroll
@@ -898,17 +938,21 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
   st.min_limit = min(seen_end, n - p.rows + row0 / group + 1);
   st.c2 = p.scale * kLog2e;
 
-  const uint32_t k_read = Tile::k_read(g, t), v_read = Tile::kSliceBytes + Tile::v_read(g, t);
+  const uint32_t k_read = Tile::k_read(g, t), v_read = L::kTensorBytes + Tile::v_read(g, t);
   uint32_t drain = 0;
-  for (int i = 0; i < slices; ++i) {
+  for (int i = 0; i < turns; ++i) {
     issue(i + kAhead);
     const uint32_t stage = ring.base + drain * L::kStageBytes;
-    const int key0 = first + i * kPagedStep;
-    float k_scale = 1.f, v_scale = 1.f;
-    if constexpr (kScaled) {
-      const bool before = (min(i + kAhead, slices - 1) ^ i) >= 32;
-      k_scale = __shfl_sync(0xffffffffu, before ? last_k : k_scales, i & 31);
-      v_scale = __shfl_sync(0xffffffffu, before ? last_v : v_scales, i & 31);
+    const int key0 = first + i * kStep;
+    float k_scale[kH], v_scale[kH];
+    const bool before = (min(i + kAhead, turns - 1) ^ i) >= kBatch;
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      k_scale[h] = v_scale[h] = 1.f;
+      if constexpr (kScaled) {
+        k_scale[h] = __shfl_sync(0xffffffffu, before ? last_k : k_scales, i * kH + h);
+        v_scale[h] = __shfl_sync(0xffffffffu, before ? last_v : v_scales, i * kH + h);
+      }
     }
     mbar_wait(ring.barriers + drain * 8, (ring.phases >> drain) & 1u, ring.wait, kPagedBarrierId);
     ring.phases ^= 1u << drain;
@@ -918,22 +962,26 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       for (int x = rows * (Tile::kBlockRow / 16) + lane; x < kPagedSlice * (Tile::kBlockRow / 16); x += 32)
 #pragma unroll
         for (int block = 0; block < Tile::kBlocks; ++block)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(stage + Tile::kSliceBytes + block * Tile::kBlockBytes + x * 16), "r"(0) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(stage + L::kTensorBytes + block * Tile::kBlockBytes + x * 16), "r"(0) : "memory");
       __syncwarp();
     }
-    paged_scores<D, T, NT>(st, stage + k_read, key0, k_scale);
-    paged_output<D, T, NT>(st, stage + v_read, v_scale);
+    float s[kH][NT][4];
+#pragma unroll
+    for (int h = 0; h < kH; ++h) paged_scores<T>(st, s[h], stage + k_read + h * Tile::kSliceBytes);
+    paged_weights<kH, T>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale);
+#pragma unroll
+    for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes, v_scale[h]);
     drain = drain + 1 < L::kStages ? drain + 1 : 0;
     __syncwarp();  // all lanes are done with this stage before it is refilled
   }
   if constexpr (kScaled) {
     for (int j = 0; j < 2 * tail_slices; ++j) {
-      issue(slices + j + kAhead);
+      issue(turns + j + kAhead);
       cp_async_wait<0>();
       __syncwarp();
       const uint32_t stage = ring.base + drain * L::kStageBytes;
-      if ((j & 1) == 0) paged_tail_scores<D, T, NT>(st, stage, in_pages + tail_first + (j >> 1) * kPagedStep);
-      else paged_tail_output<D, T, NT>(st, stage);
+      if ((j & 1) == 0) paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n);
+      else paged_tail_output<T>(st, stage);
       drain = drain + 1 < L::kStages ? drain + 1 : 0;
       __syncwarp();
     }
@@ -950,14 +998,14 @@ __device__ __forceinline__ int paged_merge_mix(int pair) {
 // CTAs per SM: what shared memory holds, as far as the registers of a result of 8 NT rows allow.
 template <int D, class T, int NT>
 constexpr int paged_ctas_per_sm() {
-  const int by_memory = (227 << 10) / (PagedSmem<D, T>::bytes(8 * NT) + (2 << 10));
-  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 ? 4 : 3;
+  const int by_memory = (227 << 10) / (PagedSmem<D, T, NT>::kBytes + (2 << 10));
+  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : 3;
   return by_memory < by_registers ? by_memory : by_registers;
 }
 
 template <int D, class T, int NT>
 __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-  using L = PagedSmem<D, T>;
+  using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t paged_smem_raw[];
@@ -983,7 +1031,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
   const int unit = blockIdx.x % heads;
   int b = -1;
   PagedCut cut;
-  if (!paged_find(sums, cut, p, heads, blockIdx.x / heads, b, shared_cut, shared_b)) return;
+  if (!paged_find<kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads, b, shared_cut, shared_b)) return;
   const int part = static_cast<int>(blockIdx.x / heads - cut.group);
   const int step0 = static_cast<int>(static_cast<int64_t>(cut.steps) * part / cut.parts);
   const int step1 = static_cast<int>(static_cast<int64_t>(cut.steps) * (part + 1) / cut.parts);
@@ -992,7 +1040,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
   const int rows_valid = min(kRows, p.rows * group - row0);
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   PagedRing ring{smem_u32(paged_smem) + warp * L::kRingBytes, smem_u32(&barriers[warp][0]), 0u, WaitCtx{&abort_flag, p.status}};
-  PagedState<D, NT> st;
+  PagedState<D, NT, kPagedSlices<D, T, NT>> st;
   paged_piece<D, T, NT>(p, &k_map, &v_map, ring, b, cut.n, kv_head, row0, rows_valid, step0, step1, st);
   __syncthreads();  // the ring becomes the place of the warps' results
 
@@ -1045,7 +1093,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
 }
 
 // Merges the parts of the entries that were cut, and writes the zeros of entries without positions.
-template <int D, int NT>
+template <int D, int NT, int STEP>
 __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(const PagedAttnParams p) {
   static_assert(kCombineThreads == kPagedThreads, "a block finds an entry's cut");
   constexpr int kRows = 8 * NT;
@@ -1061,7 +1109,7 @@ __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(cons
   int b = row / p.heads_q / p.rows;
   PagedCut cut;
   // (the lengths were not written by the grid before, and whatever wrote them ended before that grid let this one start)
-  paged_find(sums, cut, p, heads, 0, b, shared_cut, shared_b);
+  paged_find<STEP>(sums, cut, p, heads, 0, b, shared_cut, shared_b);
   if (cut.parts == 1) return;
   const int in_head = token * group + head % group;  // query row of the KV head
   const int64_t first = (cut.slot * heads + head / group * chunks + in_head / kRows) * kRows + in_head % kRows;
@@ -1075,7 +1123,7 @@ __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(cons
 template <int D, class T, int NT>
 cudaError_t resident_ctas(int* ctas) {
   auto kern = fal_paged_splitk_kernel<D, T, NT>;
-  constexpr int kBytes = PagedSmem<D, T>::bytes(8 * NT);
+  constexpr int kBytes = PagedSmem<D, T, NT>::kBytes;
   static DeviceOnce configured;
   static int per_device[64] = {};
   int dev = 0;
@@ -1101,18 +1149,19 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
   const int64_t chunks = (static_cast<int64_t>(p.rows) * (p.heads_q / p.c.heads_kv) + 8 * NT - 1) / (8 * NT);
   const int64_t heads = p.c.heads_kv * chunks;
   p.parts = kPagedWaves * resident;
-  // Parts of all entries: one each, and p.parts / heads more; and no more than kPagedMinSteps make of full entries.
-  const int64_t steps = ((static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) + kPagedStep - 1) / kPagedStep + 1;
-  const int64_t groups = std::min<int64_t>(p.c.batch + p.parts / heads, p.c.batch * ((steps + kPagedMinSteps - 1) / kPagedMinSteps));
+  // Parts of all entries: one each, and p.parts / heads more; and no more than kPagedMinKeys make of full entries.
+  constexpr int kStep = kPagedStep<D, T, NT>, kMinSteps = kPagedMinKeys / kStep;
+  const int64_t steps = ((static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) + kStep - 1) / kStep + 1;
+  const int64_t groups = std::min<int64_t>(p.c.batch + p.parts / heads, p.c.batch * ((steps + kMinSteps - 1) / kMinSteps));
   // (a cut entry is longer than one part: its parts are at most twice its steps in parts)
   p.slots = std::min<int64_t>(groups, 2 * (p.parts / heads) + 2) * heads;
   if (groups * heads > 0x7fffffff) return cudaErrorInvalidValue;
   if (maps == nullptr) return e;
   p.part_ml = p.part_o + p.slots * 8 * NT * D;
-  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads), PagedSmem<D, T>::bytes(8 * NT), stream, p, maps[0], maps[1]);
+  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads), PagedSmem<D, T, NT>::kBytes, stream, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const unsigned rows = static_cast<unsigned>(p.c.batch) * p.rows * p.heads_q;
-  return launch_dependent(fal_paged_combine_kernel<D, NT>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
+  return launch_dependent(fal_paged_combine_kernel<D, NT, kPagedStep<D, T, NT>>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
 }
 
 template <int D, class T>
