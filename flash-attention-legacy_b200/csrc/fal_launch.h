@@ -246,14 +246,14 @@ struct PagedAttnParams {
   int heads_q;
   int rows;              // query i sees the keys up to position len - rows + i
   int kernel_dim;        // 64, 128 or 256
-  int parts;             // CTAs that all entries' keys are cut for
+  int resident;          // CTAs of the split-K kernel that run at once
   int64_t slots;         // CTAs whose results can go to the workspace
   float scale;
   int* status;
 };
 // Query rows that one CTA takes.
 int paged_rows_per_cta(int rows, int kernel_dim);
-cudaError_t paged_attn_plan(PagedAttnParams& p);  // sets p.parts and p.slots, from the shapes and types in p
+cudaError_t paged_attn_plan(PagedAttnParams& p);  // sets p.resident and p.slots, from the shapes and types in p
 // maps: of the K and of the V pages, (head_dim, row, head, page) with boxes of kPagedBoxRows rows x 128 bytes (64 where the
 // kernel's rows are that short), permuted as wide.
 constexpr int kPagedBoxRows = 16;

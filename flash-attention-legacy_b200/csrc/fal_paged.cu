@@ -345,6 +345,10 @@ constexpr int kPagedSlices = Elem<T>::kScaled && NT == 1 && D <= 128 ? 2 : 1;
 template <int D, class T, int NT>
 constexpr int kPagedStep = kPagedWarps * kPagedSlice * kPagedSlices<D, T, NT>;  // keys of a step of a CTA
 
+// Where the queries are: in registers, or in shared memory where registers hold many rows of the output.
+template <int D, int NT>
+constexpr bool kPagedQueriesShared = NT * D > 256;
+
 constexpr float kS8Bias = 1152.f;  // what widen_biased adds to a code
 
 // Four 8-bit codes as two pairs of fp16.
@@ -453,7 +457,8 @@ struct PagedSmem {
   static constexpr int kPitch = D + 4;  // floats of a row of a warp's result
   static constexpr int kMergeBytes = kPagedWarps * 8 * NT * (kPitch + 2) * 4;
   static constexpr int kAlign = 1024;   // of TMA's permuted blocks
-  static constexpr int kBytes = (kPipeBytes > kMergeBytes ? kPipeBytes : kMergeBytes) + kAlign;
+  static constexpr int kQueryOffset = kPipeBytes > kMergeBytes ? kPipeBytes : kMergeBytes;
+  static constexpr int kBytes = kQueryOffset + (kPagedQueriesShared<D, NT> ? D / 16 * NT * 256 : 0) + kAlign;
 };
 
 // ---- the deal ----
@@ -490,12 +495,15 @@ __device__ __forceinline__ uint64_t paged_block_sum(PagedSums& sums, uint64_t mi
   return mine;
 }
 
-// A part is at least kPagedMinKeys long, and otherwise as long as makes `p.parts` CTAs of all units: kPagedWaves for every place.
+// A part is as long as makes kPagedWaves CTAs of all units for every place on the GPU, but no shorter than kPagedGoodSteps,
+// which a CTA's set-up is small beside, as long as there is a CTA for every place, nor than kPagedMinKeys.
+constexpr float kNoKey = -1e30f;  // further below any score than an exponential notices
 constexpr int kPagedMinKeys = 256;
 #ifndef FAL_PAGED_WAVES
-#define FAL_PAGED_WAVES 2
+#define FAL_PAGED_WAVES 4
 #endif
 constexpr int kPagedWaves = FAL_PAGED_WAVES;
+constexpr int kPagedGoodSteps = 8;
 
 // How an entry is cut.
 struct PagedCut {
@@ -521,7 +529,9 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, c
     paged_block_sum(sums, paged_steps<STEP>(c, n), all);
     total += all;
   }
-  const int64_t length = max((total * heads + p.parts - 1) / p.parts, static_cast<int64_t>(kPagedMinKeys / STEP));
+  const int64_t once = (total * heads + p.resident - 1) / p.resident;
+  const int64_t length = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<int64_t>(kPagedGoodSteps))),
+                             static_cast<int64_t>(kPagedMinKeys / STEP));
   uint64_t before = 0;  // parts in the low half, parts of cut entries in the high half
   for (int base = 0; base <= last; base += kPagedThreads) {
     const int e = base + threadIdx.x;
@@ -552,12 +562,13 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, c
 // ---- one piece of a unit ----
 template <int D, int NT, int H>
 struct PagedState {
-  uint32_t q[D / 16][2][NT];
+  // the first product's second operand, or where it is: [step][n tile][lane], two words each
+  uint32_t q[kPagedQueriesShared<D, NT> ? 1 : D / 16][2][kPagedQueriesShared<D, NT> ? 1 : NT];
+  uint32_t q_shared;
   uint32_t p[H][NT][2];  // the weights of the slices in hand, as the second product's operand
   float sum[H][NT][4];   // of those weights, times kSumFactor
   float o[NT][D / 16][4];
-  float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far
-  float most[NT][2];  // what an exponent may be before the reference moves: 8, or -infinity before the first key
+  float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far; kNoKey before the first
   float l[NT][2];     // times kSumFactor
   float c2;
   int limit[NT][2];  // first key that a query row does not see
@@ -601,7 +612,7 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
     for (int e = 0; e < 2; ++e) {
       most[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
       if (H == 2) most[nt][e] = fmaxf(most[nt][e], fmaxf(s[H - 1][nt][e], s[H - 1][nt][2 + e]));
-      grows = grows || most[nt][e] - st.m[nt][e] > st.most[nt][e];
+      grows = grows || most[nt][e] - st.m[nt][e] > 8.f;
     }
   // The reference follows the largest score only when a weight would exceed 2^8: the output is rescaled a few times per
   // part, and the largest is looked for across the lanes only then.
@@ -615,14 +626,9 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        const bool none = st.most[nt][e] == -INFINITY;  // (then m is 0 and stands for no reference)
-        const float m_new = none ? x : fmaxf(st.m[nt][e], x);
-        alpha[e] = 0.f;
-        if (m_new != -INFINITY) {  // (else no key yet)
-          if (!none) alpha[e] = fast_exp2(st.m[nt][e] - m_new);
-          st.m[nt][e] = m_new;
-          st.most[nt][e] = 8.f;
-        }
+        const float m_new = fmaxf(st.m[nt][e], x);
+        alpha[e] = fast_exp2(st.m[nt][e] - m_new);
+        st.m[nt][e] = m_new;
         st.l[nt][e] *= alpha[e];
       }
 #pragma unroll
@@ -656,11 +662,18 @@ template <int D, int NT, int H>
 __device__ __forceinline__ void paged_score_step(PagedState<D, NT, H>& st, float (&s)[NT][4], const uint32_t (&a)[4], int ks) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    uint32_t q[2];
+    if constexpr (kPagedQueriesShared<D, NT>) {
+      lds8(st.q_shared + (ks * NT + nt) * 256, q);
+    } else {
+      q[0] = st.q[ks][0][nt];
+      q[1] = st.q[ks][1][nt];
+    }
     if (ks == 0) {
       const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_16816_from(s[nt], a, st.q[ks][0][nt], st.q[ks][1][nt], zero);
+      mma_16816_from(s[nt], a, q[0], q[1], zero);
     } else {
-      mma_16816(s[nt], a, st.q[ks][0][nt], st.q[ks][1][nt]);
+      mma_16816(s[nt], a, q[0], q[1]);
     }
   }
 }
@@ -803,7 +816,7 @@ constexpr int kNoSlice = -2147483647;  // in place of a page: beyond the part
 
 // Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
 template <int D, class T, int NT>
-__device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, PagedRing& ring,
+__device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, PagedRing& ring, uint32_t queries,
                                             int b, int n, int kv_head, int row0, int rows_valid, int step0, int step1,
                                             PagedState<D, NT, kPagedSlices<D, T, NT>>& st) {
   using L = PagedSmem<D, T, NT>;
@@ -909,25 +922,36 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
 
   // ---- queries and their limits, under the first loads ----
   const int seen_end = kScaled ? n : page_end;  // (pages of 8-bit caches are full)
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  auto query = [&](int nt, int ks) {
     const int row = nt * 8 + g;
     const int r = row0 + row;
-    const __half* q = static_cast<const __half*>(p.q) + b * p.q_strides.batch + r / group * p.q_strides.row +
-                      (kv_head * group + r % group) * p.q_strides.head;
+    const int col = (ks / (kQ / 4)) * 4 * kQ + t * kQ + (ks % (kQ / 4)) * 4;
+    if (row >= rows_valid || col >= c.head_dim) return make_uint2(0u, 0u);
+    return *reinterpret_cast<const uint2*>(static_cast<const __half*>(p.q) + b * p.q_strides.batch + r / group * p.q_strides.row +
+                                           (kv_head * group + r % group) * p.q_strides.head + col);
+  };
+  if constexpr (kPagedQueriesShared<D, NT>) {
+    st.q_shared = queries + lane * 8;
+    for (int x = warp; x < D / 16 * NT; x += kPagedWarps) {
+      const uint2 q = query(x % NT, x / NT);
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(st.q_shared + x * 256), "r"(q.x), "r"(q.y) : "memory");
+    }
+    __syncthreads();
+  }
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      const int col = (ks / (kQ / 4)) * 4 * kQ + t * kQ + (ks % (kQ / 4)) * 4;
-      uint2 x = make_uint2(0u, 0u);
-      if (row < rows_valid && col < c.head_dim) x = *reinterpret_cast<const uint2*>(q + col);
-      st.q[ks][0][nt] = x.x;
-      st.q[ks][1][nt] = x.y;
+  for (int nt = 0; nt < NT; ++nt) {
+    if constexpr (!kPagedQueriesShared<D, NT>) {
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint2 q = query(nt, ks);
+        st.q[ks][0][nt] = q.x;
+        st.q[ks][1][nt] = q.y;
+      }
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       st.limit[nt][e] = min(seen_end, n - p.rows + (row0 + nt * 8 + 2 * t + e) / group + 1);
-      st.m[nt][e] = 0.f;
-      st.most[nt][e] = -INFINITY;
+      st.m[nt][e] = kNoKey;
       st.l[nt][e] = 0.f;
     }
 #pragma unroll
@@ -999,7 +1023,7 @@ __device__ __forceinline__ int paged_merge_mix(int pair) {
 template <int D, class T, int NT>
 constexpr int paged_ctas_per_sm() {
   const int by_memory = (227 << 10) / (PagedSmem<D, T, NT>::kBytes + (2 << 10));
-  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : 3;
+  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : NT * D < 256 || (NT * D == 256 && NT <= 2) ? 3 : 2;
   return by_memory < by_registers ? by_memory : by_registers;
 }
 
@@ -1041,7 +1065,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   PagedRing ring{smem_u32(paged_smem) + warp * L::kRingBytes, smem_u32(&barriers[warp][0]), 0u, WaitCtx{&abort_flag, p.status}};
   PagedState<D, NT, kPagedSlices<D, T, NT>> st;
-  paged_piece<D, T, NT>(p, &k_map, &v_map, ring, b, cut.n, kv_head, row0, rows_valid, step0, step1, st);
+  paged_piece<D, T, NT>(p, &k_map, &v_map, ring, smem_u32(paged_smem) + L::kQueryOffset, b, cut.n, kv_head, row0, rows_valid, step0, step1, st);
   __syncthreads();  // the ring becomes the place of the warps' results
 
   // (column pair c of a row is at c ^ (its lane / 2): eight lanes and four rows of a store hit different banks)
@@ -1060,21 +1084,20 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
       }
       if (g == 0)
         *reinterpret_cast<float2*>(mml + row * 2) =
-            make_float2(st.most[nt][x] == -INFINITY ? -INFINITY : st.m[nt][x], st.l[nt][x] * (1.f / kSumFactor<T>));
+            make_float2(st.m[nt][x], st.l[nt][x] * (1.f / kSumFactor<T>));
     }
   }
   __syncthreads();
   const int64_t slot = ((cut.slot + part) * heads + unit) * kRows;
   for (int idx = threadIdx.x; idx < rows_valid * (D / 2); idx += kPagedThreads) {
     const int r = idx / (D / 2), pair = idx % (D / 2);
-    float most = -INFINITY;
+    float most = kNoKey;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) most = fmaxf(most, mml[(w * kRows + r) * 2]);
-    const float use = most == -INFINITY ? 0.f : most;
     float o0 = 0.f, o1 = 0.f, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) {
-      const float x = fast_exp2(mml[(w * kRows + r) * 2] - use);
+      const float x = fast_exp2(mml[(w * kRows + r) * 2] - most);
       const float2 y = *reinterpret_cast<const float2*>(mo + (w * kRows + r) * L::kPitch + (pair ^ paged_merge_mix<D, T>(pair)) * 2);
       o0 += x * y.x;
       o1 += x * y.y;
@@ -1143,18 +1166,17 @@ cudaError_t resident_ctas(int* ctas) {
 
 template <int D, class T, int NT>
 cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) {
-  int resident = 0;
-  cudaError_t e = resident_ctas<D, T, NT>(&resident);
+  cudaError_t e = resident_ctas<D, T, NT>(&p.resident);
   if (e != cudaSuccess) return e;
   const int64_t chunks = (static_cast<int64_t>(p.rows) * (p.heads_q / p.c.heads_kv) + 8 * NT - 1) / (8 * NT);
   const int64_t heads = p.c.heads_kv * chunks;
-  p.parts = kPagedWaves * resident;
-  // Parts of all entries: one each, and p.parts / heads more; and no more than kPagedMinKeys make of full entries.
+  // Parts of all entries: one each, and as many more as there are CTAs to make; and no more than kPagedMinKeys make of full entries.
   constexpr int kStep = kPagedStep<D, T, NT>, kMinSteps = kPagedMinKeys / kStep;
   const int64_t steps = ((static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) + kStep - 1) / kStep + 1;
-  const int64_t groups = std::min<int64_t>(p.c.batch + p.parts / heads, p.c.batch * ((steps + kMinSteps - 1) / kMinSteps));
+  const int64_t parts = static_cast<int64_t>(kPagedWaves) * p.resident;
+  const int64_t groups = std::min<int64_t>(p.c.batch + parts / heads, p.c.batch * ((steps + kMinSteps - 1) / kMinSteps));
   // (a cut entry is longer than one part: its parts are at most twice its steps in parts)
-  p.slots = std::min<int64_t>(groups, 2 * (p.parts / heads) + 2) * heads;
+  p.slots = std::min<int64_t>(groups, 2 * (parts / heads) + 2) * heads;
   if (groups * heads > 0x7fffffff) return cudaErrorInvalidValue;
   if (maps == nullptr) return e;
   p.part_ml = p.part_o + p.slots * 8 * NT * D;
@@ -1166,9 +1188,12 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
 
 template <int D, class T>
 cudaError_t splitk_d(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream) {
+  const int tiles = paged_rows_per_cta(p.rows * (p.heads_q / p.c.heads_kv), D) / 8;
   if constexpr (D < 256) {
-    if (paged_rows_per_cta(p.rows * (p.heads_q / p.c.heads_kv), D) == 16) return splitk_t<D, T, 2>(p, maps, stream);
+    if (tiles == 4) return splitk_t<D, T, 4>(p, maps, stream);
+    if (tiles == 3) return splitk_t<D, T, 3>(p, maps, stream);
   }
+  if (tiles == 2) return splitk_t<D, T, 2>(p, maps, stream);
   return splitk_t<D, T, 1>(p, maps, stream);
 }
 
@@ -1248,7 +1273,11 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
 
 }  // namespace
 
-int paged_rows_per_cta(int rows, int kernel_dim) { return rows > 8 && kernel_dim < 256 ? 16 : 8; }
+int paged_rows_per_cta(int rows, int kernel_dim) {
+  const int tiles = (rows + 7) / 8, most = kernel_dim < 256 ? 4 : 2;
+  const int passes = (tiles + most - 1) / most;
+  return 8 * ((tiles + passes - 1) / passes);
+}
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
   const int tasks = (p.heads_q + 2 * p.c.heads_kv) * (p.c.head_dim / 16);
