@@ -377,19 +377,21 @@ __device__ __forceinline__ void widen_biased(const E4M3* type, uint32_t w, uint3
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ void cp_async_16_bytes(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// D = A * B + C of mma_16816, C and D apart
+// D = A * B + C (fp16 16 x 16 and 16 x 8, fp32)
 __device__ __forceinline__ void mma_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ void mma_16816_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  mma_16816_from(d, a, b0, b1, d);
 }
 __device__ __forceinline__ void lds16(uint32_t addr, uint32_t* w) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
@@ -571,8 +573,7 @@ struct PagedState {
   float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far; kNoKey before the first
   float l[NT][2];     // times kSumFactor
   float c2;
-  int limit[NT][2];  // first key that a query row does not see
-  int min_limit;
+  int min_limit;     // first key that some query row does not see
 };
 
 // The column sums of the weights come from a product with this number in every place: int8 wants them times what
@@ -583,10 +584,11 @@ template <class T>
 constexpr uint32_t kSumOperand = std::is_same<T, S8>::value ? 0xe480e480u : 0x3c003c00u;  // two of it in fp16
 
 // What follows the first product: scores s of this lane's keys key and key + 8 of H slices, from key0 on, for query rows 2 t and
-// 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have.  W: the type of the pages (kSumFactor).
+// 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have; first_limit: first key that the
+// entry's first token does not see; W: the type of the pages (kSumFactor).
 template <int H, class W, int D, int NT, int HS>
 __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
-                                              const float (&k_scale)[H]) {
+                                              const float (&k_scale)[H], int first_limit, int row0, int group) {
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     const float f = st.c2 * k_scale[h];
@@ -597,12 +599,16 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
   }
   if (key0 + H * kPagedSlice > min(st.min_limit, end)) {
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int x = 0; x < 2; ++x) {
+        const int limit = min(end, first_limit + (row0 + nt * 8 + 2 * static_cast<int>(threadIdx.x & 3) + x) / group);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key + h * kPagedSlice + (e >> 1) * 8 >= min(st.limit[nt][e & 1], end)) s[h][nt][e] = -INFINITY;
+        for (int h = 0; h < H; ++h) {
+          if (key + h * kPagedSlice >= limit) s[h][nt][x] = -INFINITY;
+          if (key + h * kPagedSlice + 8 >= limit) s[h][nt][2 + x] = -INFINITY;
+        }
+      }
   }
   float most[NT][2];
   bool grows = false;
@@ -673,7 +679,7 @@ __device__ __forceinline__ void paged_score_step(PagedState<D, NT, H>& st, float
       const float zero[4] = {0.f, 0.f, 0.f, 0.f};
       mma_16816_from(s[nt], a, q[0], q[1], zero);
     } else {
-      mma_16816(s[nt], a, q[0], q[1]);
+      mma_16816_add(s[nt], a, q[0], q[1]);
     }
   }
 }
@@ -728,7 +734,7 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
           unpack_f32x2(y, st.o[nt][j][e], st.o[nt][j][e + 1]);
         }
       } else {
-        mma_16816(st.o[nt][j], a, st.p[h][nt][0], st.p[h][nt][1]);
+        mma_16816_add(st.o[nt][j], a, st.p[h][nt][0], st.p[h][nt][1]);
       }
     }
   };
@@ -763,7 +769,8 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
 
 // The same of a slice of the tail at shared address base; K and V are there one after the other.
 template <class T, int D, int NT, int H>
-__device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint32_t base, int key0, int end) {
+__device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint32_t base, int key0, int end, int first_limit,
+                                                  int row0, int group) {
   using Tail = PagedTailTile<D, T>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float s[1][NT][4];
@@ -782,7 +789,7 @@ __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint
     }
   }
   const float scale[1] = {1.f};
-  paged_weights<1, T>(st, s, key0, key0 + g, end, scale);
+  paged_weights<1, T>(st, s, key0, key0 + g, end, scale, first_limit, row0, group);
 }
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint32_t base) {
@@ -799,7 +806,7 @@ __device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint
       const uint32_t a[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
                              __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_16816(st.o[nt][j + k], a, st.p[0][nt][0], st.p[0][nt][1]);
+      for (int nt = 0; nt < NT; ++nt) mma_16816_add(st.o[nt][j + k], a, st.p[0][nt][0], st.p[0][nt][1]);
     }
   }
 }
@@ -921,7 +928,6 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
   v_scales = scale_of(c.v_scales, pages);
 
   // ---- queries and their limits, under the first loads ----
-  const int seen_end = kScaled ? n : page_end;  // (pages of 8-bit caches are full)
   auto query = [&](int nt, int ks) {
     const int row = nt * 8 + g;
     const int r = row0 + row;
@@ -950,7 +956,6 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      st.limit[nt][e] = min(seen_end, n - p.rows + (row0 + nt * 8 + 2 * t + e) / group + 1);
       st.m[nt][e] = kNoKey;
       st.l[nt][e] = 0.f;
     }
@@ -959,7 +964,8 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[nt][j][e] = 0.f;
   }
-  st.min_limit = min(seen_end, n - p.rows + row0 / group + 1);
+  const int first_limit = n - p.rows + 1;
+  st.min_limit = first_limit + row0 / group;
   st.c2 = p.scale * kLog2e;
 
   const uint32_t k_read = Tile::k_read(g, t), v_read = L::kTensorBytes + Tile::v_read(g, t);
@@ -992,7 +998,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     float s[kH][NT][4];
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_scores<T>(st, s[h], stage + k_read + h * Tile::kSliceBytes);
-    paged_weights<kH, T>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale);
+    paged_weights<kH, T>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, first_limit, row0, group);
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes, v_scale[h]);
     drain = drain + 1 < L::kStages ? drain + 1 : 0;
@@ -1004,7 +1010,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       cp_async_wait<0>();
       __syncwarp();
       const uint32_t stage = ring.base + drain * L::kStageBytes;
-      if ((j & 1) == 0) paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n);
+      if ((j & 1) == 0) paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n, first_limit, row0, group);
       else paged_tail_output<T>(st, stage);
       drain = drain + 1 < L::kStages ? drain + 1 : 0;
       __syncwarp();
