@@ -39,6 +39,10 @@ __device__ __forceinline__ int paged_len(const PagedCache& c, int b) { return mi
 // Bound by HBM on prompts, by latency for single tokens.  A thread takes 16 columns of a head: the two 8-column pieces
 // whose columns are rotated with each other, or two neighbouring ones.
 constexpr int kAppendThreads = 256;
+// Blocks per SM: 48 registers a thread, 64 with 8-bit pages.  us on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, 4 / 5 / 6
+// blocks: fp16 64.6 / 60.5 / 65.5; int8, 3 / 4 / 5: 96.9 / 83.1 / 85.2.
+template <class T>
+constexpr int kAppendBlocks = std::is_same<T, __half>::value ? 5 : 4;
 
 struct Piece {
   int first, second;  // columns of the two pieces
@@ -79,229 +83,301 @@ __device__ __forceinline__ void turn(float& x1, float& x2, float c, float s) {
   x2 = y2;
 }
 
-// The two pieces of a row of q or k (v: not rotated) at position pos, rotated.
+// cos and sin of the eight column pairs of piece c at position pos.
+struct Angles {
+  float cs[8], sn[8];
+};
+__device__ __forceinline__ Angles append_angles(const PagedAppendParams& p, int c, int pos) {
+  Angles x;
+  const int64_t at = static_cast<int64_t>(pos) * (p.rotary_dim / 2) + c * 8;
+  load_angles(p.cos, p.half_tables, at, x.cs);
+  load_angles(p.sin, p.half_tables, at, x.sn);
+  return x;
+}
+__device__ __forceinline__ void append_turn(const PagedAppendParams& p, const Angles& x, uint4& a, uint4& b) {
+  __half2* ha = reinterpret_cast<__half2*>(&a);
+  __half2* hb = reinterpret_cast<__half2*>(&b);
+  if (p.interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 u = __half22float2(ha[i]), v = __half22float2(hb[i]);
+      turn(u.x, u.y, x.cs[i], x.sn[i]);
+      turn(v.x, v.y, x.cs[4 + i], x.sn[4 + i]);
+      ha[i] = __floats2half2_rn(u.x, u.y);
+      hb[i] = __floats2half2_rn(v.x, v.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 u = __half22float2(ha[i]), v = __half22float2(hb[i]);
+      turn(u.x, v.x, x.cs[2 * i], x.sn[2 * i]);
+      turn(u.y, v.y, x.cs[2 * i + 1], x.sn[2 * i + 1]);
+      ha[i] = __floats2half2_rn(u.x, u.y);
+      hb[i] = __floats2half2_rn(v.x, v.y);
+    }
+  }
+}
+
+// The two pieces of a row of k (v: not rotated) at position pos, rotated.
 __device__ __forceinline__ void append_load(const PagedAppendParams& p, const __half* row, int c, bool turned, int pos,
                                             uint4& a, uint4& b, Piece& at) {
   at = append_piece(p, c);
   if (!turned) at = Piece{c * 16, c * 16 + 8, false};
   a = *reinterpret_cast<const uint4*>(row + at.first);
   b = *reinterpret_cast<const uint4*>(row + at.second);
-  if (!at.rotated) return;
-  __half2* ha = reinterpret_cast<__half2*>(&a);
-  __half2* hb = reinterpret_cast<__half2*>(&b);
-  float cs[8], sn[8];
-  const int64_t angle = static_cast<int64_t>(pos) * (p.rotary_dim / 2) + c * 8;
-  load_angles(p.cos, p.half_tables, angle, cs);
-  load_angles(p.sin, p.half_tables, angle, sn);
-  if (p.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 x = __half22float2(ha[i]), y = __half22float2(hb[i]);
-      turn(x.x, x.y, cs[i], sn[i]);
-      turn(y.x, y.y, cs[4 + i], sn[4 + i]);
-      ha[i] = __floats2half2_rn(x.x, x.y);
-      hb[i] = __floats2half2_rn(y.x, y.y);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 x = __half22float2(ha[i]), y = __half22float2(hb[i]);
-      turn(x.x, y.x, cs[2 * i], sn[2 * i]);
-      turn(x.y, y.y, cs[2 * i + 1], sn[2 * i + 1]);
-      ha[i] = __floats2half2_rn(x.x, x.y);
-      hb[i] = __floats2half2_rn(y.x, y.y);
-    }
-  }
+  if (at.rotated) append_turn(p, append_angles(p, c, pos), a, b);
 }
 
 __device__ __forceinline__ const __half* new_row(const void* base, const RowStrides& s, int b, int h, int r) {
   return static_cast<const __half*>(base) + b * s.batch + h * s.head + r * s.row;
 }
 
-// Page of position pos of entry b, or -1 (and the status word says so).
-__device__ __forceinline__ int append_page(const PagedAppendParams& p, int b, int pos) {
-  int page = -1;
-  if (pos < paged_capacity(p.c)) page = p.c.table[b * p.c.table_stride + (pos >> p.c.page_shift)];
-  if (page < 0 || page >= p.c.num_pages) {
-    if (p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
-    page = -1;
-  }
-  return page;
-}
-
-// Grid: (token, piece of its q, k and v heads).  Rows of 8-bit caches that finish a page are the next kernel's business,
-// and so are those behind such a page: their places in the tail are read there first.
-__global__ void __launch_bounds__(kAppendThreads) fal_paged_append_kernel(const PagedAppendParams p) {
-  grid_dependency_wait();
-  grid_dependency_launch();
-  const int b = blockIdx.x / p.rows;
-  const int i = blockIdx.x % p.rows;
+// Half a token block: one token.  A thread takes one piece of every few heads, so that it fetches its angles once (a thread for
+// every piece of a token's heads, angles and all: 4 x 1 024 tokens of 48 heads of 128, int8, 36 us, against 26.5).
+// Rows of 8-bit caches that finish a page are the page blocks' business, and so are those behind such a page: their places in
+// the tail are read there first.
+constexpr int kTokenThreads = kAppendThreads / 2;
+__device__ __forceinline__ void append_token(const PagedAppendParams& p, int token, int thread) {
+  const int b = token / p.rows;
+  const int i = token % p.rows;
   const int start = p.c.lens[b];
   const int capacity = paged_capacity(p.c);
-  if (i == 0 && blockIdx.y == 0 && threadIdx.x == 0)
-    p.new_lens[b] = start < 0 ? start : static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
   const int pieces = p.c.head_dim / 16;
-  const int task = blockIdx.y * kAppendThreads + threadIdx.x;
-  int h = task / pieces;
-  const int c = task % pieces;
-  if (h >= p.heads_q + 2 * p.c.heads_kv) return;
+  const int lanes = kTokenThreads / pieces, lane = thread / pieces, c = thread % pieces;
   const int64_t pos64 = static_cast<int64_t>(start) + i;
   const bool placed = start >= 0 && pos64 < capacity;  // (start < 0: an unused entry of a padded batch)
   const int pos = placed ? static_cast<int>(pos64) : 0;
-  uint4 a, z;
-  Piece at;
-  if (h < p.heads_q) {
-    append_load(p, new_row(p.q, p.q_strides, b, h, i), c, true, pos, a, z, at);
-    if (!placed) a = z = make_uint4(0, 0, 0, 0);
-    __half* out = static_cast<__half*>(p.q_out) + (static_cast<int64_t>(blockIdx.x) * p.heads_q + h) * p.c.head_dim;
-    *reinterpret_cast<uint4*>(out + at.first) = a;
-    *reinterpret_cast<uint4*>(out + at.second) = z;
-    return;
+  if (thread == 0) {
+    if (i == 0) p.new_lens[b] = start < 0 ? start : static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
+    if (start >= 0 && !placed && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
   }
-  h -= p.heads_q;
-  const bool is_v = h >= p.c.heads_kv;
-  if (is_v) h -= p.c.heads_kv;
-  if (!placed) {
-    if (start >= 0 && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
-    return;
-  }
-  __half* dst;
+  if (lane >= lanes) return;  // (head_dim 96)
   const int shift = p.c.page_shift;
   const int in_page = pos & ((1 << shift) - 1);
+  // where head 0 of the token's K and V rows goes, or nowhere
+  __half *k_to = nullptr, *v_to = nullptr;
+  int64_t k_head = 0, v_head = 0;
   if (p.c.type == kPagedF16) {
-    const int page = append_page(p, b, pos);
-    if (page < 0) return;
-    const RowStrides& s = is_v ? p.c.v_strides : p.c.k_strides;
-    dst = static_cast<__half*>(is_v ? p.c.v_pages : p.c.k_pages) + page * s.batch + h * s.head + in_page * s.row;
+    int page = -1;
+    if (placed) {
+      page = p.c.table[b * p.c.table_stride + (pos >> shift)];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.num_pages)) {
+        page = -1;
+        if (thread == 0 && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
+      }
+    }
+    if (page >= 0) {
+      k_to = static_cast<__half*>(p.c.k_pages) + page * p.c.k_strides.batch + in_page * p.c.k_strides.row;
+      v_to = static_cast<__half*>(p.c.v_pages) + page * p.c.v_strides.batch + in_page * p.c.v_strides.row;
+    }
+    k_head = p.c.k_strides.head;
+    v_head = p.c.v_strides.head;
   } else {
     const int64_t end = min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity));
-    if ((end >> shift) != (start >> shift)) return;
-    const RowStrides& s = is_v ? p.c.v_tail_strides : p.c.k_tail_strides;
-    dst = static_cast<__half*>(is_v ? p.c.v_tail : p.c.k_tail) + b * s.batch + h * s.head + in_page * s.row;
+    if (placed && (end >> shift) == (start >> shift)) {
+      k_to = static_cast<__half*>(p.c.k_tail) + b * p.c.k_tail_strides.batch + in_page * p.c.k_tail_strides.row;
+      v_to = static_cast<__half*>(p.c.v_tail) + b * p.c.v_tail_strides.batch + in_page * p.c.v_tail_strides.row;
+    }
+    k_head = p.c.k_tail_strides.head;
+    v_head = p.c.v_tail_strides.head;
   }
-  const __half* src = is_v ? new_row(p.v, p.v_new_strides, b, h, i) : new_row(p.k, p.k_new_strides, b, h, i);
-  append_load(p, src, c, !is_v, pos, a, z, at);
-  *reinterpret_cast<uint4*>(dst + at.first) = a;
-  *reinterpret_cast<uint4*>(dst + at.second) = z;
+  const Piece turned = append_piece(p, c), plain{c * 16, c * 16 + 8, false};
+  Angles angles;
+  if (turned.rotated) angles = append_angles(p, c, pos);
+  const int heads = p.heads_q + (k_to != nullptr ? 2 * p.c.heads_kv : 0);
+  for (int h = lane; h < heads; h += lanes) {
+    const int hk = h - p.heads_q, hv = hk - p.c.heads_kv;
+    const __half* src = hk < 0 ? new_row(p.q, p.q_strides, b, h, i) : hv < 0 ? new_row(p.k, p.k_new_strides, b, hk, i)
+                                                                            : new_row(p.v, p.v_new_strides, b, hv, i);
+    const Piece& at = hv < 0 ? turned : plain;
+    uint4 a = *reinterpret_cast<const uint4*>(src + at.first), z = *reinterpret_cast<const uint4*>(src + at.second);
+    if (at.rotated) append_turn(p, angles, a, z);
+    __half* dst = hk < 0 ? static_cast<__half*>(p.q_out) + (static_cast<int64_t>(token) * p.heads_q + h) * p.c.head_dim
+                         : hv < 0 ? k_to + hk * k_head : v_to + hv * v_head;
+    if (!placed) a = z = make_uint4(0, 0, 0, 0);  // (a query without a position)
+    *reinterpret_cast<uint4*>(dst + at.first) = a;
+    *reinterpret_cast<uint4*>(dst + at.second) = z;
+  }
 }
 
-// The codes of two fp16 values as two bytes; most: the page's largest magnitude, not 0.
-__device__ __forceinline__ uint32_t codes_of(const S8*, float2 x, float most) {
-  const int lo = __float2int_rn(__fdiv_rn(x.x * 127.f, most)), hi = __float2int_rn(__fdiv_rn(x.y * 127.f, most));
+// x / a from r, about 1 / a: one step of Newton's method, whose residual is exact in a fused multiply-add.  Within a unit of the
+// last place, and exact where the quotient is a number of 24 bits -- a rounding border of the codes --, which is all that
+// their rounding needs.
+__device__ __forceinline__ float quotient(float x, float a, float r) {
+  const float y = x * r;
+  return y == 0.f ? y : __fmaf_rn(__fmaf_rn(-y, a, x), r, y);  // (a zero keeps its sign)
+}
+// The codes of two fp16 values as two bytes; most: the page's largest magnitude, not 0; r: 1 / most.
+__device__ __forceinline__ uint32_t codes_of(const S8*, float2 x, float most, float r) {
+  const int lo = __float2int_rn(quotient(x.x * 127.f, most, r)), hi = __float2int_rn(quotient(x.y * 127.f, most, r));
   return (lo & 0xff) | ((hi & 0xff) << 8);
 }
-__device__ __forceinline__ uint32_t codes_of(const E4M3*, float2 x, float most) {
+__device__ __forceinline__ uint32_t codes_of(const E4M3*, float2 x, float most, float r) {
   uint16_t out;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
       : "=h"(out)
-      : "f"(__fdiv_rn(x.y * 448.f, most)), "f"(__fdiv_rn(x.x * 448.f, most)));
+      : "f"(quotient(x.y * 448.f, most, r)), "f"(quotient(x.x * 448.f, most, r)));
   return out;
 }
 __device__ __forceinline__ float code_max(const S8*) { return 127.f; }
 __device__ __forceinline__ float code_max(const E4M3*) { return 448.f; }
 
-// Full pages of 8-bit caches.  Grid: (page counted from the one of the first new row, KV head of K then of V, entry).
-// The rows of a page are put together in shared memory -- the first page's earlier rows from the tail, the others from
-// the call, rotated --, their largest magnitude is found, and the codes leave in 16-byte stores.  The first page's block
-// also writes the rows behind the last full page to the tail, once it has read it.
+// A page block: the index-th page from the one of entry b's first new row, for a few KV heads of K or of V, `threads` to a head.
+// A thread keeps the first kSealKept pieces that it reads (the rows before the new ones from the tail, the others from the
+// call, rotated) and reads further ones, of pages of more than 8 192 values a head, again: once for the largest magnitude, once
+// for the codes.  The first page's block also writes the rows behind the last full page to the tail, once it has read it.
+// (256 threads to a head: 4 x 2 987 tokens, pages of 16 x 128, 104 us against HERE_US.)
+constexpr int kSealKept = 2;
 template <class T>
-__global__ void __launch_bounds__(kAppendThreads) fal_paged_seal_kernel(const PagedAppendParams p) {
-  extern __shared__ __align__(16) __half seal_rows[];
+__device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, int b, int first_head, int index_from, int threads) {
   __shared__ uint32_t warp_most[kAppendThreads / 32];
-  grid_dependency_wait();
-  grid_dependency_launch();
-  const int b = blockIdx.z;
   const int start = p.c.lens[b];
   const int capacity = paged_capacity(p.c);
   const int shift = p.c.page_shift;
   if (start < 0 || start >= capacity) return;
   const int end = static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
-  const int index = (start >> shift) + blockIdx.x;  // page of the entry
+  const int index = (start >> shift) + index_from;  // page of the entry
   if (index >= (end >> shift)) return;              // not full
-  const bool is_v = blockIdx.y >= static_cast<unsigned>(p.c.heads_kv);
-  const int h = is_v ? blockIdx.y - p.c.heads_kv : blockIdx.y;
-  const int d = p.c.head_dim, pieces = d / 16, page_rows = 1 << shift;
+  const int head = min(first_head + static_cast<int>(threadIdx.x) / threads, 2 * p.c.heads_kv - 1);
+  const bool active = first_head + static_cast<int>(threadIdx.x) / threads == head;
+  const int thread = threadIdx.x % threads;
+  const int page = p.c.table[b * p.c.table_stride + index];
+  const bool is_v = head >= p.c.heads_kv;
+  const int h = is_v ? head - p.c.heads_kv : head;
+  const int pieces = p.c.head_dim / 16, page_rows = 1 << shift, tasks = active ? page_rows * pieces : 0;
   const RowStrides& ts = is_v ? p.c.v_tail_strides : p.c.k_tail_strides;
   __half* tail = static_cast<__half*>(is_v ? p.c.v_tail : p.c.k_tail) + b * ts.batch + h * ts.head;
   const void* src = is_v ? p.v : p.k;
   const RowStrides& ss = is_v ? p.v_new_strides : p.k_new_strides;
-
-  uint32_t most = 0;  // of the magnitudes' bits: infinities and NaN are larger than any number
-  for (int task = threadIdx.x; task < page_rows * pieces; task += kAppendThreads) {
+  auto load = [&](int task, uint4& a, uint4& z, Piece& at) {
     const int r = task / pieces, c = task % pieces;
     const int pos = (index << shift) + r;
-    uint4 a, z;
-    Piece at;
     if (pos < start) {
-      at = Piece{c * 16, c * 16 + 8, false};
+      // (in the pieces that the rotation of a new row takes together, so that one place holds one piece)
+      at = append_piece(p, c);
+      if (is_v) at = Piece{c * 16, c * 16 + 8, false};
       a = *reinterpret_cast<const uint4*>(tail + r * ts.row + at.first);
       z = *reinterpret_cast<const uint4*>(tail + r * ts.row + at.second);
     } else {
       append_load(p, new_row(src, ss, b, h, pos - start), c, !is_v, pos, a, z, at);
     }
-    *reinterpret_cast<uint4*>(seal_rows + r * d + at.first) = a;
-    *reinterpret_cast<uint4*>(seal_rows + r * d + at.second) = z;
-    for (const uint32_t w : {a.x, a.y, a.z, a.w, z.x, z.y, z.z, z.w}) most = __vmaxu2(most, w & 0x7fff7fffu);
+  };
+  uint32_t most = 0;  // of the magnitudes' bits: infinities and NaN are larger than any number
+  auto look = [&](const uint4& x) {
+    for (const uint32_t w : {x.x, x.y, x.z, x.w}) most = __vmaxu2(most, w & 0x7fff7fffu);
+  };
+  uint4 kept[kSealKept][2];
+  Piece at;
+#pragma unroll
+  for (int k = 0; k < kSealKept; ++k) {
+    kept[k][0] = kept[k][1] = make_uint4(0, 0, 0, 0);
+    const int task = thread + k * threads;
+    if (task < tasks) load(task, kept[k][0], kept[k][1], at);
+    look(kept[k][0]);
+    look(kept[k][1]);
+  }
+  for (int task = thread + kSealKept * threads; task < tasks; task += threads) {
+    uint4 a, z;
+    load(task, a, z, at);
+    look(a);
+    look(z);
   }
   most = max(most & 0xffffu, most >> 16);
   most = __reduce_max_sync(0xffffffffu, most);
   if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = most;
   __syncthreads();
-  most = warp_most[0];
-#pragma unroll
-  for (int w = 1; w < kAppendThreads / 32; ++w) most = max(most, warp_most[w]);
-  const float a = __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
+  const int first_warp = (threadIdx.x - thread) / 32;
+  for (int w = 0; w < threads / 32; ++w) most = max(most, warp_most[first_warp + w]);
+  const float largest = __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
   const bool finite = most < 0x7c00u;
   const bool some = finite && most != 0;
+  const float inverse = some ? __fdiv_rn(1.f, largest) : 0.f;
 
-  const int page = threadIdx.x == 0 ? append_page(p, b, index << shift) : p.c.table[b * p.c.table_stride + index];
-  if (page >= 0 && page < p.c.num_pages) {
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.num_pages)) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
+  } else {
     const RowStrides& s = is_v ? p.c.v_strides : p.c.k_strides;
     uint8_t* out = static_cast<uint8_t*>(is_v ? p.c.v_pages : p.c.k_pages) + page * s.batch + h * s.head;
-    for (int task = threadIdx.x; task < page_rows * pieces; task += kAppendThreads) {
-      const int r = task / pieces, c = task % pieces;
-      const __half2* x = reinterpret_cast<const __half2*>(seal_rows + r * d + c * 16);
-      uint32_t w[4] = {0, 0, 0, 0};
+    auto codes = [&](const uint4& x) {
+      uint2 w = make_uint2(0u, 0u);
       if (some) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = codes_of(static_cast<const T*>(nullptr), __half22float2(x[2 * k]), a) |
-                 (codes_of(static_cast<const T*>(nullptr), __half22float2(x[2 * k + 1]), a) << 16);
+        const __half2* y = reinterpret_cast<const __half2*>(&x);
+        const T* type = nullptr;
+        w.x = codes_of(type, __half22float2(y[0]), largest, inverse) | codes_of(type, __half22float2(y[1]), largest, inverse) << 16;
+        w.y = codes_of(type, __half22float2(y[2]), largest, inverse) | codes_of(type, __half22float2(y[3]), largest, inverse) << 16;
       }
-      *reinterpret_cast<uint4*>(out + r * s.row + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      return w;
+    };
+    auto store = [&](int task, const uint4& a, const uint4& z) {
+      const int r = task / pieces, c = task % pieces;
+      Piece to = append_piece(p, c);
+      if (is_v) to = Piece{c * 16, c * 16 + 8, false};
+      *reinterpret_cast<uint2*>(out + r * s.row + to.first) = codes(a);
+      *reinterpret_cast<uint2*>(out + r * s.row + to.second) = codes(z);
+    };
+#pragma unroll
+    for (int k = 0; k < kSealKept; ++k) {
+      const int task = thread + k * threads;
+      if (task < tasks) store(task, kept[k][0], kept[k][1]);
     }
-    if (threadIdx.x == 0) {
+    for (int task = thread + kSealKept * threads; task < tasks; task += threads) {
+      uint4 a, z;
+      load(task, a, z, at);
+      store(task, a, z);
+    }
+    if (active && thread == 0) {
       float* scales = is_v ? p.c.v_scales : p.c.k_scales;
       // a page with an infinity or a NaN has none that stands for it: what sees the page becomes NaN
       scales[static_cast<int64_t>(page) * p.c.heads_kv + h] =
-          finite ? __fdiv_rn(a, code_max(static_cast<const T*>(nullptr))) : __int_as_float(0x7fffffff);
+          finite ? __fdiv_rn(largest, code_max(static_cast<const T*>(nullptr))) : __int_as_float(0x7fffffff);
     }
   }
-  if (blockIdx.x != 0) return;
-  const int left = end & (page_rows - 1);  // rows behind the last full page (the tail was read before the barrier above)
-  const int first = end - left;
-  for (int task = threadIdx.x; task < left * pieces; task += kAppendThreads) {
+  if (index_from != 0) return;
+  __syncthreads();  // the tail's rows of this page have been read
+  const int left = active ? end & (page_rows - 1) : 0;  // rows behind the last full page
+  const int first = end & ~(page_rows - 1);
+  for (int task = thread; task < left * pieces; task += threads) {
     const int r = task / pieces, c = task % pieces;
     uint4 x, z;
-    Piece at;
     append_load(p, new_row(src, ss, b, h, first + r - start), c, !is_v, first + r, x, z, at);
     *reinterpret_cast<uint4*>(tail + r * ts.row + at.first) = x;
     *reinterpret_cast<uint4*>(tail + r * ts.row + at.second) = z;
   }
 }
 
+// One launch: first the page blocks (8-bit caches: heads of K and of V, then page, then entry), then the token blocks.
 template <class T>
-cudaError_t launch_seal(const PagedAppendParams& p, cudaStream_t stream) {
-  auto kern = fal_paged_seal_kernel<T>;
-  static DeviceOnce configured;
-  cudaError_t e = configured.run([&] {
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedMostRows * 256 * 2);
-  });
-  if (e != cudaSuccess) return e;
-  const int64_t page_rows = 1 << p.c.page_shift;
-  const unsigned pages = static_cast<unsigned>((p.rows + page_rows - 1) >> p.c.page_shift);  // that one entry can finish
-  return launch_dependent(kern, dim3(pages, 2 * p.c.heads_kv, p.c.batch), dim3(kAppendThreads),
-                          static_cast<size_t>(p.c.head_dim) * page_rows * 2, stream, p);
+__global__ void __launch_bounds__(kAppendThreads, kAppendBlocks<T>) fal_paged_append_kernel(const PagedAppendParams p, unsigned page_blocks, unsigned pages,
+                                                                                         unsigned head_threads, unsigned tokens) {
+  grid_dependency_wait();
+  grid_dependency_launch();
+  if constexpr (!std::is_same<T, __half>::value) {
+    if (blockIdx.x < page_blocks) {
+      const unsigned at_once = kAppendThreads / head_threads, groups = (2 * p.c.heads_kv + at_once - 1) / at_once;
+      const unsigned which = blockIdx.x / groups;
+      append_page_codes<T>(p, which / pages, blockIdx.x % groups * at_once, which % pages, head_threads);
+      return;
+    }
+  }
+  const unsigned token = (blockIdx.x - page_blocks) * 2 + threadIdx.x / kTokenThreads;
+  if (token < tokens) append_token(p, token, threadIdx.x % kTokenThreads);
+}
+
+template <class T>
+cudaError_t append_t(const PagedAppendParams& p, cudaStream_t stream) {
+  const int64_t tokens = static_cast<int64_t>(p.c.batch) * p.rows;
+  // pages that one entry can finish
+  const int64_t pages = std::is_same<T, __half>::value ? 0 : (p.rows + (int64_t{1} << p.c.page_shift) - 1) >> p.c.page_shift;
+  // threads to a head: kSealKept pieces each where that fills warps
+  int64_t head_threads = 32;
+  while (head_threads < kAppendThreads && head_threads * kSealKept < (int64_t{p.c.head_dim / 16} << p.c.page_shift)) head_threads *= 2;
+  const int64_t at_once = kAppendThreads / head_threads;
+  const int64_t page_blocks = pages * ((2 * p.c.heads_kv + at_once - 1) / at_once) * p.c.batch;
+  const int64_t blocks = page_blocks + (tokens + 1) / 2;
+  if (tokens > 0x7fffffff || blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  return launch_dependent(fal_paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream, p,
+                          static_cast<unsigned>(page_blocks), static_cast<unsigned>(pages), static_cast<unsigned>(head_threads),
+                          static_cast<unsigned>(tokens));
 }
 
 // ---------------------------------------------------------------------------
@@ -505,7 +581,8 @@ constexpr int kPagedMinKeys = 256;
 #define FAL_PAGED_WAVES 4
 #endif
 constexpr int kPagedWaves = FAL_PAGED_WAVES;
-constexpr int kPagedGoodSteps = 8;
+template <int D>
+constexpr int kPagedGoodSteps = D == 64 ? 16 : D == 128 ? 8 : 32;
 
 // How an entry is cut.
 struct PagedCut {
@@ -517,7 +594,7 @@ struct PagedCut {
 };
 // Finds the entry `b` (if b >= 0), or else the one that has part `group` of all entries' parts (b is set).  False: there is none.
 // Called by all threads of a block.  STEP: keys of a step.
-template <int STEP>
+template <int D, int STEP>
 __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, const PagedAttnParams& p, int64_t heads, int64_t group, int& b,
                                            PagedCut& shared_cut, int& shared_b) {
   const PagedCache& c = p.c;
@@ -532,7 +609,7 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, c
     total += all;
   }
   const int64_t once = (total * heads + p.resident - 1) / p.resident;
-  const int64_t length = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<int64_t>(kPagedGoodSteps))),
+  const int64_t length = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<int64_t>(kPagedGoodSteps<D>))),
                              static_cast<int64_t>(kPagedMinKeys / STEP));
   uint64_t before = 0;  // parts in the low half, parts of cut entries in the high half
   for (int base = 0; base <= last; base += kPagedThreads) {
@@ -1061,7 +1138,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
   const int unit = blockIdx.x % heads;
   int b = -1;
   PagedCut cut;
-  if (!paged_find<kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads, b, shared_cut, shared_b)) return;
+  if (!paged_find<D, kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads, b, shared_cut, shared_b)) return;
   const int part = static_cast<int>(blockIdx.x / heads - cut.group);
   const int step0 = static_cast<int>(static_cast<int64_t>(cut.steps) * part / cut.parts);
   const int step1 = static_cast<int>(static_cast<int64_t>(cut.steps) * (part + 1) / cut.parts);
@@ -1138,7 +1215,7 @@ __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(cons
   int b = row / p.heads_q / p.rows;
   PagedCut cut;
   // (the lengths were not written by the grid before, and whatever wrote them ended before that grid let this one start)
-  paged_find<STEP>(sums, cut, p, heads, 0, b, shared_cut, shared_b);
+  paged_find<D, STEP>(sums, cut, p, heads, 0, b, shared_cut, shared_b);
   if (cut.parts == 1) return;
   const int in_head = token * group + head % group;  // query row of the KV head
   const int64_t first = (cut.slot * heads + head / group * chunks + in_head / kRows) * kRows + in_head % kRows;
@@ -1286,13 +1363,8 @@ int paged_rows_per_cta(int rows, int kernel_dim) {
 }
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
-  const int tasks = (p.heads_q + 2 * p.c.heads_kv) * (p.c.head_dim / 16);
-  const int64_t tokens = static_cast<int64_t>(p.c.batch) * p.rows;
-  const int groups = (tasks + kAppendThreads - 1) / kAppendThreads;
-  if (tokens > 0x7fffffff || groups > 65535) return cudaErrorInvalidValue;
-  cudaError_t e = launch_dependent(fal_paged_append_kernel, dim3(static_cast<unsigned>(tokens), groups), dim3(kAppendThreads), 0, stream, p);
-  if (e != cudaSuccess || p.c.type == kPagedF16) return e;
-  return p.c.type == kPagedS8 ? launch_seal<S8>(p, stream) : launch_seal<E4M3>(p, stream);
+  if (p.c.type == kPagedF16) return append_t<__half>(p, stream);
+  return p.c.type == kPagedS8 ? append_t<S8>(p, stream) : append_t<E4M3>(p, stream);
 }
 
 cudaError_t paged_attn_plan(PagedAttnParams& p) { return splitk(p, nullptr, nullptr); }
