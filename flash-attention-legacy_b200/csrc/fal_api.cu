@@ -1172,8 +1172,12 @@ int make_paged_map(CUtensorMap* map, const void* base, const fal_paged_cache& c,
   return FAL_OK;
 }
 
-// Query rows of a KV head up to which the split-K pass takes them, 8 or 16 to a CTA that streams the keys for itself.
-constexpr int64_t kPagedFewRows = 64;
+// Query tokens up to which the split-K pass takes a call, 8 to 32 (token, head) rows to a CTA that streams the keys for itself.
+// The forward kernel takes as long for one token as for 128, per query head, behind a pass that puts the pages in order.  us,
+// this / that: 8 entries of 6 000 int8 positions, 32 / 8 heads of 128, 17 tokens 115 / 201, 24 129 / 201, 32 171 / 202, 48 244 /
+// 202; one such entry, 17 21.7 / 28.0, 32 35.2 / 28.7; 16 x 1 000, 16 / 16 of 64, 16 34 / 41, 24 44 / 41, 32 53 / 43; 32 x 500 fp16,
+// 8 / 8 of 256, 16 48 / 85, 24 76 / 86; 8 x 6 000 int8, 16 / 16 of 128, 24 91 / 188.
+constexpr int kPagedFewTokens = 24;
 constexpr int64_t kPagedGatherBytes = int64_t{1} << 30;
 
 constexpr int64_t kPagedUnknownSlots = 148 * 24;  // without a GPU to ask
@@ -1203,7 +1207,7 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
   const int64_t rows = static_cast<int64_t>(a.rows) * group;
   const int dim = kernel_head_dim(c.head_dim);
   PagedPlan p{};
-  p.few_rows = rows <= kPagedFewRows;
+  p.few_rows = a.rows <= kPagedFewTokens;
   if (p.few_rows) {
     fal::PagedAttnParams k = paged_attn_params(a);
     const cudaError_t e = fal::paged_attn_plan(k);

@@ -391,16 +391,13 @@ cudaError_t append_t(const PagedAppendParams& p, cudaStream_t stream) {
 // and Q is laid out to match; lane g of eight takes 16 neighbouring bytes of a V row.
 // 8-bit codes become fp16 in registers (exact), the scales enter in 32 bits: K's with the softmax scale, V's where the
 // product of a 16-key slice is added to the output.  P^T of the scores' layout becomes the second product's operand by
-// movmatrix; its column sums, as one more product with ones, are the softmax sum and remove what int8's widening adds.
+// movmatrix; its column sums, one more product with ones, are the softmax sum.
 //
 // An (entry, KV head, chunk of 8 NT query rows) is a unit; its keys count in steps of 64, a 16-key slice for each of four
 // warps.  Entries are cut into parts of one length that the GPU works out from all lengths, so that all units together
 // make a few CTAs for every place on the GPU, whatever the lengths are; the units of one part are CTAs next to each other,
 // because their rows are next to each other in memory where a page holds all heads of a position.  Parts of a cut entry go
 // to the workspace and a second kernel merges them; a CTA that has all keys of its unit writes the result itself.
-#ifndef FAL_PAGED_STAGES
-#define FAL_PAGED_STAGES 2
-#endif
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kPagedSlice = 16;
@@ -425,17 +422,12 @@ constexpr int kPagedStep = kPagedWarps * kPagedSlice * kPagedSlices<D, T, NT>;  
 template <int D, int NT>
 constexpr bool kPagedQueriesShared = NT * D > 256;
 
-constexpr float kS8Bias = 1152.f;  // what widen_biased adds to a code
-
 // Four 8-bit codes as two pairs of fp16.
-__device__ __forceinline__ void widen_biased(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ void widen(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
   // 1024 + u, u = code + 128, as fp16 is 0x6400 + u
   const uint32_t u = w ^ 0x80808080u;
   lo = __byte_perm(u, 0x64646464u, 0x4140);
   hi = __byte_perm(u, 0x64646464u, 0x4342);
-}
-__device__ __forceinline__ void widen(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
-  widen_biased(static_cast<const S8*>(nullptr), w, lo, hi);
   asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x64806480u));
   asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x64806480u));
 }
@@ -449,7 +441,6 @@ __device__ __forceinline__ void widen(const E4M3*, uint32_t w, uint32_t& lo, uin
       : "=r"(lo), "=r"(hi)
       : "r"(w));
 }
-__device__ __forceinline__ void widen_biased(const E4M3* type, uint32_t w, uint32_t& lo, uint32_t& hi) { widen(type, w, lo, hi); }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
@@ -527,7 +518,7 @@ struct PagedTailTile {
 
 template <int D, class T, int NT>
 struct PagedSmem {
-  static constexpr int kStages = D == 64 && kPagedSlices<D, T, NT> == 1 ? 4 : kPagedSlices<D, T, NT> == 1 ? 3 : FAL_PAGED_STAGES;
+  static constexpr int kStages = D == 64 && kPagedSlices<D, T, NT> == 1 ? 4 : kPagedSlices<D, T, NT> == 1 || D == 64 ? 3 : 2;
   static constexpr int kTensorBytes = kPagedSlices<D, T, NT> * PagedTile<D, T>::kSliceBytes;
   static constexpr int kStageBytes = 2 * kTensorBytes;      // K, then V; or K or V of a slice of the tail
   static constexpr int kRingBytes = kStages * kStageBytes;  // per warp
@@ -573,14 +564,12 @@ __device__ __forceinline__ uint64_t paged_block_sum(PagedSums& sums, uint64_t mi
   return mine;
 }
 
-// A part is as long as makes kPagedWaves CTAs of all units for every place on the GPU, but no shorter than kPagedGoodSteps,
-// which a CTA's set-up is small beside, as long as there is a CTA for every place, nor than kPagedMinKeys.
+// A part is as long as makes kPagedWaves CTAs of all units for every place on the GPU (SMs get unequal shares of the memory's
+// bandwidth), but no shorter than kPagedGoodSteps, which a CTA's set-up is small beside, as long as there is a CTA for every
+// place, nor than kPagedMinKeys.  (A length that makes the CTAs fill the places a whole number of times is no better.)
 constexpr float kNoKey = -1e30f;  // further below any score than an exponential notices
 constexpr int kPagedMinKeys = 256;
-#ifndef FAL_PAGED_WAVES
-#define FAL_PAGED_WAVES 4
-#endif
-constexpr int kPagedWaves = FAL_PAGED_WAVES;
+constexpr int kPagedWaves = 4;
 template <int D>
 constexpr int kPagedGoodSteps = D == 64 ? 16 : D == 128 ? 8 : 32;
 
@@ -645,25 +634,17 @@ struct PagedState {
   uint32_t q[kPagedQueriesShared<D, NT> ? 1 : D / 16][2][kPagedQueriesShared<D, NT> ? 1 : NT];
   uint32_t q_shared;
   uint32_t p[H][NT][2];  // the weights of the slices in hand, as the second product's operand
-  float sum[H][NT][4];   // of those weights, times kSumFactor
   float o[NT][D / 16][4];
   float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far; kNoKey before the first
-  float l[NT][2];     // times kSumFactor
+  float l[NT][2];     // sums of the weights
   float c2;
   int min_limit;     // first key that some query row does not see
 };
 
-// The column sums of the weights come from a product with this number in every place: int8 wants them times what
-// widen_biased adds, to take it off again.
-template <class T>
-constexpr float kSumFactor = std::is_same<T, S8>::value ? -kS8Bias : 1.f;
-template <class T>
-constexpr uint32_t kSumOperand = std::is_same<T, S8>::value ? 0xe480e480u : 0x3c003c00u;  // two of it in fp16
-
 // What follows the first product: scores s of this lane's keys key and key + 8 of H slices, from key0 on, for query rows 2 t and
 // 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have; first_limit: first key that the
-// entry's first token does not see; W: the type of the pages (kSumFactor).
-template <int H, class W, int D, int NT, int HS>
+// entry's first token does not see; 
+template <int H, int D, int NT, int HS>
 __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
                                               const float (&k_scale)[H], int first_limit, int row0, int group) {
 #pragma unroll
@@ -732,11 +713,12 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
       st.p[h][nt][0] = movmatrix(pack_half2(s[h][nt][0], s[h][nt][1]));
       st.p[h][nt][1] = movmatrix(pack_half2(s[h][nt][2], s[h][nt][3]));
       // sums of the weights as they are rounded, which is what the output is divided by
-      const uint32_t factor[4] = {kSumOperand<W>, kSumOperand<W>, kSumOperand<W>, kSumOperand<W>};
+      const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
       const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_16816_from(st.sum[h][nt], factor, st.p[h][nt][0], st.p[h][nt][1], zero);
-      st.l[nt][0] += st.sum[h][nt][0];
-      st.l[nt][1] += st.sum[h][nt][1];
+      float sum[4];
+      mma_16816_from(sum, ones, st.p[h][nt][0], st.p[h][nt][1], zero);
+      st.l[nt][0] += sum[0];
+      st.l[nt][1] += sum[1];
     }
 }
 
@@ -798,13 +780,8 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
     for (int nt = 0; nt < NT; ++nt) {
       if constexpr (Elem<T>::kScaled) {
         float x[4];
-        if constexpr (std::is_same<T, S8>::value) {
-          // (sums of codes + 1 152 and the sums that take it off cancel within a slice: 2^-23 of 1 152, 2^-13 of a code's step)
-          mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], st.sum[h][nt]);
-        } else {
-          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], zero);
-        }
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], zero);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           const uint64_t y = ffma2(pack_f32x2(x[e], x[e + 1]), pack_f32x2(v_scale, v_scale), pack_f32x2(st.o[nt][j][e], st.o[nt][j][e + 1]));
@@ -831,8 +808,8 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           uint32_t a[4];
-          widen_biased(static_cast<const T*>(nullptr), __byte_perm(w[0][k], w[1][k], u == 0 ? 0x5140 : 0x7362), a[0], a[1]);
-          widen_biased(static_cast<const T*>(nullptr), __byte_perm(w[2][k], w[3][k], u == 0 ? 0x5140 : 0x7362), a[2], a[3]);
+          widen(static_cast<const T*>(nullptr), __byte_perm(w[0][k], w[1][k], u == 0 ? 0x5140 : 0x7362), a[0], a[1]);
+          widen(static_cast<const T*>(nullptr), __byte_perm(w[2][k], w[3][k], u == 0 ? 0x5140 : 0x7362), a[2], a[3]);
           product(j + u, a);
         }
       } else {
@@ -866,7 +843,7 @@ __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint
     }
   }
   const float scale[1] = {1.f};
-  paged_weights<1, T>(st, s, key0, key0 + g, end, scale, first_limit, row0, group);
+  paged_weights<1>(st, s, key0, key0 + g, end, scale, first_limit, row0, group);
 }
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint32_t base) {
@@ -1075,7 +1052,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     float s[kH][NT][4];
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_scores<T>(st, s[h], stage + k_read + h * Tile::kSliceBytes);
-    paged_weights<kH, T>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, first_limit, row0, group);
+    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, first_limit, row0, group);
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes, v_scale[h]);
     drain = drain + 1 < L::kStages ? drain + 1 : 0;
@@ -1106,7 +1083,7 @@ __device__ __forceinline__ int paged_merge_mix(int pair) {
 template <int D, class T, int NT>
 constexpr int paged_ctas_per_sm() {
   const int by_memory = (227 << 10) / (PagedSmem<D, T, NT>::kBytes + (2 << 10));
-  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : NT * D < 256 || (NT * D == 256 && NT <= 2) ? 3 : 2;
+  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : NT * D < 256 || (NT * D == 256 && NT <= 2) || (NT * D == 384) ? 3 : 2;
   return by_memory < by_registers ? by_memory : by_registers;
 }
 
@@ -1167,7 +1144,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
       }
       if (g == 0)
         *reinterpret_cast<float2*>(mml + row * 2) =
-            make_float2(st.m[nt][x], st.l[nt][x] * (1.f / kSumFactor<T>));
+            make_float2(st.m[nt][x], st.l[nt][x]);
     }
   }
   __syncthreads();
@@ -1263,10 +1240,11 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
   if (groups * heads > 0x7fffffff) return cudaErrorInvalidValue;
   if (maps == nullptr) return e;
   p.part_ml = p.part_o + p.slots * 8 * NT * D;
-  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads), PagedSmem<D, T, NT>::kBytes, stream, p, maps[0], maps[1]);
+  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads), PagedSmem<D, T, NT>::kBytes, stream, p,
+                       maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const unsigned rows = static_cast<unsigned>(p.c.batch) * p.rows * p.heads_q;
-  return launch_dependent(fal_paged_combine_kernel<D, NT, kPagedStep<D, T, NT>>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
+  return launch_dependent(fal_paged_combine_kernel<D, NT, kStep>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
 }
 
 template <int D, class T>

@@ -110,8 +110,8 @@ def flash_attn_with_paged_kvcache(
     as a row of zeros and the device status word becomes 3000.  (Between new tokens the mask is a weight of 0: a NaN or an
     infinity in the value row of one of them reaches the earlier ones of the same call.)  Inference only.
 
-    Few query rows per KV head (L x Hq / Hkv up to 64) run on a split-K pass that reads every page once for 8 or 16 of them;
-    more run on the forward kernel, over the pages put in order in a workspace as large as the block table allows for (up to
+    Up to 24 tokens run on a split-K pass that reads every page once for up to 32 (token, head) rows of a KV head; more run on
+    the forward kernel, over the pages put in order in a workspace as large as the block table allows for (up to
     1 GiB at a time): pass a view of the table's first columns where entries are much shorter than it.
     """
     out = flash_attn_legacy_cuda.paged_attend_plain(q, k, v, k_pages, v_pages, block_table, cache_seqlens, rotary_cos, rotary_sin,

@@ -138,7 +138,7 @@ def test_attention_over_pages(ext, fal, dtype, hq, hkv, d, page, layout, rows, l
     o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens),
                                           cache_layout=layout, **cache.on_gpu(layout)).cpu()
     for e, n in enumerate(lens):
-        k, v = cache.dense(e, max(n, 0), as_half=rows * hq // hkv > 64)
+        k, v = cache.dense(e, max(n, 0), as_half=rows > 24)
         want, mag = attention(q[e], k, v, scale)
         assert_close(o[e], want, mag, n, v.abs().max().item() if n > 0 else 0.0)
         first = max(rows - max(n, 0), 0)
@@ -163,7 +163,7 @@ def test_a_run_of_steps_as_a_server_makes_them(ext, fal):
                                                   rotary_cos=cos.cuda(), rotary_sin=sin.cuda(), **got).cpu()
             for e in range(2):
                 cache.append(e, rotate(k[e, at:at + n], at, cos, sin, False), v[e, at:at + n])
-                kd, vd = cache.dense(e, at + n, as_half=n * hq // hkv > 64)
+                kd, vd = cache.dense(e, at + n, as_half=n > 24)
                 want, mag = attention(rotate(q[e, at:at + n], at, cos, sin, False), kd, vd, 1 / math.sqrt(d))
                 assert_close(o[e], want, mag, at + n, vd.abs().max().item())
             at += n
@@ -278,7 +278,7 @@ def test_a_position_without_a_page_counts_as_zeros(ext, fal, dtype, rows):
     o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=table.cuda(), **args).cpu()
     assert ext.device_status() == 3000
     for e, (n, gone) in enumerate(zip(lens, (2, 0))):
-        k, v = cache.dense(e, n, as_half=rows * hq // hkv > 64)
+        k, v = cache.dense(e, n, as_half=rows > 24)
         k[gone * page:(gone + 1) * page] = 0
         v[gone * page:(gone + 1) * page] = 0
         want, mag = attention(q[e], k, v, 1 / math.sqrt(d))
