@@ -29,7 +29,8 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(LIB_DIR, "libfal_b200.so")
 HOST_SOURCE = os.path.join(CSRC, "fal_host.cpp")
 
-SOURCES = ["fal_api.cu", "fal_fwd.cu", "fal_bwd.cu", "fal_decode.cu", "fal_paged.cu", "fal_ring.cu", "fal_selftest.cu"]
+SOURCES = ["fal_api.cu", "fal_fwd.cu", "fal_bwd.cu", "fal_decode.cu", "fal_paged_append.cu", "fal_paged_attn.cu", "fal_ring.cu",
+           "fal_selftest.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",

@@ -1270,7 +1270,7 @@ int fal_paged_append_run(const fal_paged_append_args* a) {
   p.c = paged_cache(c);
   p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out;
   p.q_strides = to_rs(&a->q_strides); p.k_new_strides = to_rs(&a->k_new_strides); p.v_new_strides = to_rs(&a->v_new_strides);
-  p.cos = a->rotary_cos; p.sin = a->rotary_sin; p.half_tables = a->rotary_half; p.positions = a->rotary_positions;
+  p.cos = a->rotary_cos; p.sin = a->rotary_sin; p.half_tables = a->rotary_half;
   p.rotary_dim = a->rotary_cos != nullptr ? a->rotary_dim : 0;
   p.interleaved = a->rotary_interleaved;
   p.heads_q = a->heads_q; p.rows = a->rows; p.new_lens = a->new_seqlens; p.status = a->status;

@@ -189,7 +189,7 @@ cudaError_t decode_static_scratch(float** ptr);
 cudaError_t launch_decode_splitk(const DecodeParams& p, cudaStream_t stream);
 cudaError_t launch_decode_combine(const DecodeParams& p, cudaStream_t stream);
 
-// Paged caches (fal_paged.cu): position p of entry b is row p % page of page table[b, p / page].  8-bit pages hold codes
+// Paged caches (fal_paged_append.cu, fal_paged_attn.cu): position p of entry b is row p % page of page table[b, p / page].  8-bit pages hold codes
 // with one fp32 scale per page and KV head; the rows of an entry's last, unfinished page are fp16 rows of its tail.
 constexpr int kPagedMostRows = 256;  // of a page
 enum PagedType : int { kPagedF16 = 0, kPagedS8 = 1, kPagedE4M3 = 2 };
@@ -225,7 +225,6 @@ struct PagedAppendParams {
   const void* cos;       // [positions, rotary_dim / 2] fp32 or fp16, or null: no rotation
   const void* sin;
   int half_tables;
-  int positions;
   int rotary_dim;
   int interleaved;       // pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2)
   int heads_q;           // 0 without q

@@ -1,384 +1,18 @@
-// Paged key/value caches: append of new rows with the position rotation on the way, attention over the pages (fp16, or
-// 8 bits with a scale for each page and head), and the pages' rows in order for the forward kernel.
+// Attention over the pages of a key/value cache, in fp16 or in 8 bits with a scale for each page and head; and the pages' rows
+// in order for the forward kernel, which takes the calls with many query tokens.
 //
 // The reference has no paged cache; its hook attends eagerly over dense ones (flash_attn_legacy/integrations.py:77-98).
-//
-// 8-bit pages.  A value is rounded to 8 bits once, when its page is full: a = max |x| over the page's rows of a head,
-// scale = a / m and code = round(x m / a), m = 127 (int8, nearest whole number) or 448 (e4m3, nearest such number).  Until
-// then the row waits as fp16 in the entry's tail, so that the cache does not depend on how the rows came in, token by
-// token or as chunks, and no page is rounded again when a larger value arrives.  x m is exact in 32 bits (11 + 7 bits) and
-// its quotient by a, rounded once, is on the same side of every rounding border as the exact one: the border is a multiple
-// of 2^-5 of the code's leading bit at least 2^-16 away relative to it, or the quotient is exactly the border.
 #include <algorithm>
 #include <type_traits>
 
 #include "fal_combine.cuh"
-#include "fal_common.h"
-#include "fal_launch.h"
-#include "sm100_ptx.cuh"
+#include "fal_paged.cuh"
 
 namespace fal {
 
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-
-struct S8 {
-  uint8_t bits;
-};
-struct E4M3 {
-  uint8_t bits;
-};
-
-__device__ __forceinline__ int paged_capacity(const PagedCache& c) { return c.pages_per_entry << c.page_shift; }
-__device__ __forceinline__ int paged_len(const PagedCache& c, int b) { return min(max(c.lens[b], 0), paged_capacity(c)); }
-
-// ---------------------------------------------------------------------------
-// Append
-// ---------------------------------------------------------------------------
-// Bound by HBM on prompts, by latency for single tokens.  A thread takes 16 columns of a head: the two 8-column pieces
-// whose columns are rotated with each other, or two neighbouring ones.
-constexpr int kAppendThreads = 256;
-// Blocks per SM: 48 registers a thread, 64 with 8-bit pages.  us on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, 4 / 5 / 6
-// blocks: fp16 64.6 / 60.5 / 65.5; int8, 3 / 4 / 5: 96.9 / 83.1 / 85.2.
-template <class T>
-constexpr int kAppendBlocks = std::is_same<T, __half>::value ? 5 : 4;
-
-struct Piece {
-  int first, second;  // columns of the two pieces
-  bool rotated;
-};
-__device__ __forceinline__ Piece append_piece(const PagedAppendParams& p, int c) {
-  Piece x;
-  x.rotated = c * 16 < p.rotary_dim;
-  const bool apart = x.rotated && !p.interleaved;
-  x.first = apart ? c * 8 : c * 16;
-  x.second = x.first + (apart ? p.rotary_dim / 2 : 8);
-  return x;
-}
-
-__device__ __forceinline__ void load_angles(const void* table, int half_tables, int64_t at, float (&x)[8]) {
-  if (half_tables) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(table) + at));
-    const __half2* h = reinterpret_cast<const __half2*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  } else {
-    const float4* t = reinterpret_cast<const float4*>(static_cast<const float*>(table) + at);
-    const float4 a = __ldg(t), b = __ldg(t + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  }
-}
-
-// (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin) in 32 bits, rounded once to the cache's fp16.
-__device__ __forceinline__ void turn(float& x1, float& x2, float c, float s) {
-  const float y1 = __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s));
-  const float y2 = __fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s));
-  x1 = y1;
-  x2 = y2;
-}
-
-// cos and sin of the eight column pairs of piece c at position pos.
-struct Angles {
-  float cs[8], sn[8];
-};
-__device__ __forceinline__ Angles append_angles(const PagedAppendParams& p, int c, int pos) {
-  Angles x;
-  const int64_t at = static_cast<int64_t>(pos) * (p.rotary_dim / 2) + c * 8;
-  load_angles(p.cos, p.half_tables, at, x.cs);
-  load_angles(p.sin, p.half_tables, at, x.sn);
-  return x;
-}
-__device__ __forceinline__ void append_turn(const PagedAppendParams& p, const Angles& x, uint4& a, uint4& b) {
-  __half2* ha = reinterpret_cast<__half2*>(&a);
-  __half2* hb = reinterpret_cast<__half2*>(&b);
-  if (p.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 u = __half22float2(ha[i]), v = __half22float2(hb[i]);
-      turn(u.x, u.y, x.cs[i], x.sn[i]);
-      turn(v.x, v.y, x.cs[4 + i], x.sn[4 + i]);
-      ha[i] = __floats2half2_rn(u.x, u.y);
-      hb[i] = __floats2half2_rn(v.x, v.y);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 u = __half22float2(ha[i]), v = __half22float2(hb[i]);
-      turn(u.x, v.x, x.cs[2 * i], x.sn[2 * i]);
-      turn(u.y, v.y, x.cs[2 * i + 1], x.sn[2 * i + 1]);
-      ha[i] = __floats2half2_rn(u.x, u.y);
-      hb[i] = __floats2half2_rn(v.x, v.y);
-    }
-  }
-}
-
-// The two pieces of a row of k (v: not rotated) at position pos, rotated.
-__device__ __forceinline__ void append_load(const PagedAppendParams& p, const __half* row, int c, bool turned, int pos,
-                                            uint4& a, uint4& b, Piece& at) {
-  at = append_piece(p, c);
-  if (!turned) at = Piece{c * 16, c * 16 + 8, false};
-  a = *reinterpret_cast<const uint4*>(row + at.first);
-  b = *reinterpret_cast<const uint4*>(row + at.second);
-  if (at.rotated) append_turn(p, append_angles(p, c, pos), a, b);
-}
-
-__device__ __forceinline__ const __half* new_row(const void* base, const RowStrides& s, int b, int h, int r) {
-  return static_cast<const __half*>(base) + b * s.batch + h * s.head + r * s.row;
-}
-
-// Half a token block: one token.  A thread takes one piece of every few heads, so that it fetches its angles once (a thread for
-// every piece of a token's heads, angles and all: 4 x 1 024 tokens of 48 heads of 128, int8, 36 us, against 26.5).
-// Rows of 8-bit caches that finish a page are the page blocks' business, and so are those behind such a page: their places in
-// the tail are read there first.
-constexpr int kTokenThreads = kAppendThreads / 2;
-__device__ __forceinline__ void append_token(const PagedAppendParams& p, int token, int thread) {
-  const int b = token / p.rows;
-  const int i = token % p.rows;
-  const int start = p.c.lens[b];
-  const int capacity = paged_capacity(p.c);
-  const int pieces = p.c.head_dim / 16;
-  const int lanes = kTokenThreads / pieces, lane = thread / pieces, c = thread % pieces;
-  const int64_t pos64 = static_cast<int64_t>(start) + i;
-  const bool placed = start >= 0 && pos64 < capacity;  // (start < 0: an unused entry of a padded batch)
-  const int pos = placed ? static_cast<int>(pos64) : 0;
-  if (thread == 0) {
-    if (i == 0) p.new_lens[b] = start < 0 ? start : static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
-    if (start >= 0 && !placed && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
-  }
-  if (lane >= lanes) return;  // (head_dim 96)
-  const int shift = p.c.page_shift;
-  const int in_page = pos & ((1 << shift) - 1);
-  // where head 0 of the token's K and V rows goes, or nowhere
-  __half *k_to = nullptr, *v_to = nullptr;
-  int64_t k_head = 0, v_head = 0;
-  if (p.c.type == kPagedF16) {
-    int page = -1;
-    if (placed) {
-      page = p.c.table[b * p.c.table_stride + (pos >> shift)];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.num_pages)) {
-        page = -1;
-        if (thread == 0 && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
-      }
-    }
-    if (page >= 0) {
-      k_to = static_cast<__half*>(p.c.k_pages) + page * p.c.k_strides.batch + in_page * p.c.k_strides.row;
-      v_to = static_cast<__half*>(p.c.v_pages) + page * p.c.v_strides.batch + in_page * p.c.v_strides.row;
-    }
-    k_head = p.c.k_strides.head;
-    v_head = p.c.v_strides.head;
-  } else {
-    const int64_t end = min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity));
-    if (placed && (end >> shift) == (start >> shift)) {
-      k_to = static_cast<__half*>(p.c.k_tail) + b * p.c.k_tail_strides.batch + in_page * p.c.k_tail_strides.row;
-      v_to = static_cast<__half*>(p.c.v_tail) + b * p.c.v_tail_strides.batch + in_page * p.c.v_tail_strides.row;
-    }
-    k_head = p.c.k_tail_strides.head;
-    v_head = p.c.v_tail_strides.head;
-  }
-  const Piece turned = append_piece(p, c), plain{c * 16, c * 16 + 8, false};
-  Angles angles;
-  if (turned.rotated) angles = append_angles(p, c, pos);
-  const int heads = p.heads_q + (k_to != nullptr ? 2 * p.c.heads_kv : 0);
-  for (int h = lane; h < heads; h += lanes) {
-    const int hk = h - p.heads_q, hv = hk - p.c.heads_kv;
-    const __half* src = hk < 0 ? new_row(p.q, p.q_strides, b, h, i) : hv < 0 ? new_row(p.k, p.k_new_strides, b, hk, i)
-                                                                            : new_row(p.v, p.v_new_strides, b, hv, i);
-    const Piece& at = hv < 0 ? turned : plain;
-    uint4 a = *reinterpret_cast<const uint4*>(src + at.first), z = *reinterpret_cast<const uint4*>(src + at.second);
-    if (at.rotated) append_turn(p, angles, a, z);
-    __half* dst = hk < 0 ? static_cast<__half*>(p.q_out) + (static_cast<int64_t>(token) * p.heads_q + h) * p.c.head_dim
-                         : hv < 0 ? k_to + hk * k_head : v_to + hv * v_head;
-    if (!placed) a = z = make_uint4(0, 0, 0, 0);  // (a query without a position)
-    *reinterpret_cast<uint4*>(dst + at.first) = a;
-    *reinterpret_cast<uint4*>(dst + at.second) = z;
-  }
-}
-
-// x / a from r, about 1 / a: one step of Newton's method, whose residual is exact in a fused multiply-add.  Within a unit of the
-// last place, and exact where the quotient is a number of 24 bits -- a rounding border of the codes --, which is all that
-// their rounding needs.
-__device__ __forceinline__ float quotient(float x, float a, float r) {
-  const float y = x * r;
-  return y == 0.f ? y : __fmaf_rn(__fmaf_rn(-y, a, x), r, y);  // (a zero keeps its sign)
-}
-// The codes of two fp16 values as two bytes; most: the page's largest magnitude, not 0; r: 1 / most.
-__device__ __forceinline__ uint32_t codes_of(const S8*, float2 x, float most, float r) {
-  const int lo = __float2int_rn(quotient(x.x * 127.f, most, r)), hi = __float2int_rn(quotient(x.y * 127.f, most, r));
-  return (lo & 0xff) | ((hi & 0xff) << 8);
-}
-__device__ __forceinline__ uint32_t codes_of(const E4M3*, float2 x, float most, float r) {
-  uint16_t out;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-      : "=h"(out)
-      : "f"(quotient(x.y * 448.f, most, r)), "f"(quotient(x.x * 448.f, most, r)));
-  return out;
-}
-__device__ __forceinline__ float code_max(const S8*) { return 127.f; }
-__device__ __forceinline__ float code_max(const E4M3*) { return 448.f; }
-
-// A page block: the index-th page from the one of entry b's first new row, for a few KV heads of K or of V, `threads` to a head.
-// A thread keeps the first kSealKept pieces that it reads (the rows before the new ones from the tail, the others from the
-// call, rotated) and reads further ones, of pages of more than 8 192 values a head, again: once for the largest magnitude, once
-// for the codes.  The first page's block also writes the rows behind the last full page to the tail, once it has read it.
-// (256 threads to a head: 4 x 2 987 tokens, pages of 16 x 128, 104 us against HERE_US.)
-constexpr int kSealKept = 2;
-template <class T>
-__device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, int b, int first_head, int index_from, int threads) {
-  __shared__ uint32_t warp_most[kAppendThreads / 32];
-  const int start = p.c.lens[b];
-  const int capacity = paged_capacity(p.c);
-  const int shift = p.c.page_shift;
-  if (start < 0 || start >= capacity) return;
-  const int end = static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
-  const int index = (start >> shift) + index_from;  // page of the entry
-  if (index >= (end >> shift)) return;              // not full
-  const int head = min(first_head + static_cast<int>(threadIdx.x) / threads, 2 * p.c.heads_kv - 1);
-  const bool active = first_head + static_cast<int>(threadIdx.x) / threads == head;
-  const int thread = threadIdx.x % threads;
-  const int page = p.c.table[b * p.c.table_stride + index];
-  const bool is_v = head >= p.c.heads_kv;
-  const int h = is_v ? head - p.c.heads_kv : head;
-  const int pieces = p.c.head_dim / 16, page_rows = 1 << shift, tasks = active ? page_rows * pieces : 0;
-  const RowStrides& ts = is_v ? p.c.v_tail_strides : p.c.k_tail_strides;
-  __half* tail = static_cast<__half*>(is_v ? p.c.v_tail : p.c.k_tail) + b * ts.batch + h * ts.head;
-  const void* src = is_v ? p.v : p.k;
-  const RowStrides& ss = is_v ? p.v_new_strides : p.k_new_strides;
-  auto load = [&](int task, uint4& a, uint4& z, Piece& at) {
-    const int r = task / pieces, c = task % pieces;
-    const int pos = (index << shift) + r;
-    if (pos < start) {
-      // (in the pieces that the rotation of a new row takes together, so that one place holds one piece)
-      at = append_piece(p, c);
-      if (is_v) at = Piece{c * 16, c * 16 + 8, false};
-      a = *reinterpret_cast<const uint4*>(tail + r * ts.row + at.first);
-      z = *reinterpret_cast<const uint4*>(tail + r * ts.row + at.second);
-    } else {
-      append_load(p, new_row(src, ss, b, h, pos - start), c, !is_v, pos, a, z, at);
-    }
-  };
-  uint32_t most = 0;  // of the magnitudes' bits: infinities and NaN are larger than any number
-  auto look = [&](const uint4& x) {
-    for (const uint32_t w : {x.x, x.y, x.z, x.w}) most = __vmaxu2(most, w & 0x7fff7fffu);
-  };
-  uint4 kept[kSealKept][2];
-  Piece at;
-#pragma unroll
-  for (int k = 0; k < kSealKept; ++k) {
-    kept[k][0] = kept[k][1] = make_uint4(0, 0, 0, 0);
-    const int task = thread + k * threads;
-    if (task < tasks) load(task, kept[k][0], kept[k][1], at);
-    look(kept[k][0]);
-    look(kept[k][1]);
-  }
-  for (int task = thread + kSealKept * threads; task < tasks; task += threads) {
-    uint4 a, z;
-    load(task, a, z, at);
-    look(a);
-    look(z);
-  }
-  most = max(most & 0xffffu, most >> 16);
-  most = __reduce_max_sync(0xffffffffu, most);
-  if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = most;
-  __syncthreads();
-  const int first_warp = (threadIdx.x - thread) / 32;
-  for (int w = 0; w < threads / 32; ++w) most = max(most, warp_most[first_warp + w]);
-  const float largest = __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
-  const bool finite = most < 0x7c00u;
-  const bool some = finite && most != 0;
-  const float inverse = some ? __fdiv_rn(1.f, largest) : 0.f;
-
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.num_pages)) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
-  } else {
-    const RowStrides& s = is_v ? p.c.v_strides : p.c.k_strides;
-    uint8_t* out = static_cast<uint8_t*>(is_v ? p.c.v_pages : p.c.k_pages) + page * s.batch + h * s.head;
-    auto codes = [&](const uint4& x) {
-      uint2 w = make_uint2(0u, 0u);
-      if (some) {
-        const __half2* y = reinterpret_cast<const __half2*>(&x);
-        const T* type = nullptr;
-        w.x = codes_of(type, __half22float2(y[0]), largest, inverse) | codes_of(type, __half22float2(y[1]), largest, inverse) << 16;
-        w.y = codes_of(type, __half22float2(y[2]), largest, inverse) | codes_of(type, __half22float2(y[3]), largest, inverse) << 16;
-      }
-      return w;
-    };
-    auto store = [&](int task, const uint4& a, const uint4& z) {
-      const int r = task / pieces, c = task % pieces;
-      Piece to = append_piece(p, c);
-      if (is_v) to = Piece{c * 16, c * 16 + 8, false};
-      *reinterpret_cast<uint2*>(out + r * s.row + to.first) = codes(a);
-      *reinterpret_cast<uint2*>(out + r * s.row + to.second) = codes(z);
-    };
-#pragma unroll
-    for (int k = 0; k < kSealKept; ++k) {
-      const int task = thread + k * threads;
-      if (task < tasks) store(task, kept[k][0], kept[k][1]);
-    }
-    for (int task = thread + kSealKept * threads; task < tasks; task += threads) {
-      uint4 a, z;
-      load(task, a, z, at);
-      store(task, a, z);
-    }
-    if (active && thread == 0) {
-      float* scales = is_v ? p.c.v_scales : p.c.k_scales;
-      // a page with an infinity or a NaN has none that stands for it: what sees the page becomes NaN
-      scales[static_cast<int64_t>(page) * p.c.heads_kv + h] =
-          finite ? __fdiv_rn(largest, code_max(static_cast<const T*>(nullptr))) : __int_as_float(0x7fffffff);
-    }
-  }
-  if (index_from != 0) return;
-  __syncthreads();  // the tail's rows of this page have been read
-  const int left = active ? end & (page_rows - 1) : 0;  // rows behind the last full page
-  const int first = end & ~(page_rows - 1);
-  for (int task = thread; task < left * pieces; task += threads) {
-    const int r = task / pieces, c = task % pieces;
-    uint4 x, z;
-    append_load(p, new_row(src, ss, b, h, first + r - start), c, !is_v, first + r, x, z, at);
-    *reinterpret_cast<uint4*>(tail + r * ts.row + at.first) = x;
-    *reinterpret_cast<uint4*>(tail + r * ts.row + at.second) = z;
-  }
-}
-
-// One launch: first the page blocks (8-bit caches: heads of K and of V, then page, then entry), then the token blocks.
-template <class T>
-__global__ void __launch_bounds__(kAppendThreads, kAppendBlocks<T>) fal_paged_append_kernel(const PagedAppendParams p, unsigned page_blocks, unsigned pages,
-                                                                                         unsigned head_threads, unsigned tokens) {
-  grid_dependency_wait();
-  grid_dependency_launch();
-  if constexpr (!std::is_same<T, __half>::value) {
-    if (blockIdx.x < page_blocks) {
-      const unsigned at_once = kAppendThreads / head_threads, groups = (2 * p.c.heads_kv + at_once - 1) / at_once;
-      const unsigned which = blockIdx.x / groups;
-      append_page_codes<T>(p, which / pages, blockIdx.x % groups * at_once, which % pages, head_threads);
-      return;
-    }
-  }
-  const unsigned token = (blockIdx.x - page_blocks) * 2 + threadIdx.x / kTokenThreads;
-  if (token < tokens) append_token(p, token, threadIdx.x % kTokenThreads);
-}
-
-template <class T>
-cudaError_t append_t(const PagedAppendParams& p, cudaStream_t stream) {
-  const int64_t tokens = static_cast<int64_t>(p.c.batch) * p.rows;
-  // pages that one entry can finish
-  const int64_t pages = std::is_same<T, __half>::value ? 0 : (p.rows + (int64_t{1} << p.c.page_shift) - 1) >> p.c.page_shift;
-  // threads to a head: kSealKept pieces each where that fills warps
-  int64_t head_threads = 32;
-  while (head_threads < kAppendThreads && head_threads * kSealKept < (int64_t{p.c.head_dim / 16} << p.c.page_shift)) head_threads *= 2;
-  const int64_t at_once = kAppendThreads / head_threads;
-  const int64_t page_blocks = pages * ((2 * p.c.heads_kv + at_once - 1) / at_once) * p.c.batch;
-  const int64_t blocks = page_blocks + (tokens + 1) / 2;
-  if (tokens > 0x7fffffff || blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_dependent(fal_paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream, p,
-                          static_cast<unsigned>(page_blocks), static_cast<unsigned>(pages), static_cast<unsigned>(head_threads),
-                          static_cast<unsigned>(tokens));
-}
 
 // ---------------------------------------------------------------------------
 // Attention over the pages, few query rows per KV head
@@ -402,16 +36,6 @@ constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kPagedSlice = 16;
 
-template <class T>
-struct Elem {
-  static constexpr bool kScaled = true;
-  static constexpr int kBytes = 1;
-};
-template <>
-struct Elem<__half> {
-  static constexpr bool kScaled = false;
-  static constexpr int kBytes = 2;
-};
 // Slices that a warp takes at a time, of one page or of two.
 template <int D, class T, int NT>
 constexpr int kPagedSlices = Elem<T>::kScaled && NT == 1 && D <= 128 ? 2 : 1;
@@ -421,26 +45,6 @@ constexpr int kPagedStep = kPagedWarps * kPagedSlice * kPagedSlices<D, T, NT>;  
 // Where the queries are: in registers, or in shared memory where registers hold many rows of the output.
 template <int D, int NT>
 constexpr bool kPagedQueriesShared = NT * D > 256;
-
-// Four 8-bit codes as two pairs of fp16.
-__device__ __forceinline__ void widen(const S8*, uint32_t w, uint32_t& lo, uint32_t& hi) {
-  // 1024 + u, u = code + 128, as fp16 is 0x6400 + u
-  const uint32_t u = w ^ 0x80808080u;
-  lo = __byte_perm(u, 0x64646464u, 0x4140);
-  hi = __byte_perm(u, 0x64646464u, 0x4342);
-  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x64806480u));
-  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x64806480u));
-}
-__device__ __forceinline__ void widen(const E4M3*, uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t"
-      ".reg .b16 a, b;\n\t"
-      "mov.b32 {a, b}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t"
-      "}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
@@ -531,9 +135,6 @@ struct PagedSmem {
 };
 
 // ---- the deal ----
-__device__ __forceinline__ int paged_len_in_pages(const PagedCache& c, int n) {
-  return c.type == kPagedF16 ? n : n >> c.page_shift << c.page_shift;
-}
 // Steps of one unit of an entry with n positions: those of its pages, then those of its tail.
 template <int STEP>
 __device__ __forceinline__ int paged_steps(const PagedCache& c, int n) {
@@ -564,10 +165,14 @@ __device__ __forceinline__ uint64_t paged_block_sum(PagedSums& sums, uint64_t mi
   return mine;
 }
 
+constexpr float kNoKey = -1e30f;  // further below any score than an exponential notices
+
 // A part is as long as makes kPagedWaves CTAs of all units for every place on the GPU (SMs get unequal shares of the memory's
 // bandwidth), but no shorter than kPagedGoodSteps, which a CTA's set-up is small beside, as long as there is a CTA for every
 // place, nor than kPagedMinKeys.  (A length that makes the CTAs fill the places a whole number of times is no better.)
-constexpr float kNoKey = -1e30f;  // further below any score than an exponential notices
+// us with 1 / 2 / 4 CTAs for every place: 64 entries of 16 000 int8 positions, 8 heads of 128, 421 / 366 / 339, fp16 623 / 604 / 605, 16
+// fp16 - / 167 / 159; parts of 16 against 8 steps: 16 entries of 32 000 int8, 4 heads of 64, 57 / 61; 34 against 17: 16 of 5 000
+// e4m3, 16 heads of 256, 109 / 114.
 constexpr int kPagedMinKeys = 256;
 constexpr int kPagedWaves = 4;
 template <int D>
@@ -575,56 +180,48 @@ constexpr int kPagedGoodSteps = D == 64 ? 16 : D == 128 ? 8 : 32;
 
 // How an entry is cut.
 struct PagedCut {
+  int entry;
   int n;          // positions
   int steps;      // of a unit
   int parts;
   int64_t group;  // parts of the entries before it
   int64_t slot;   // the same, of those that are cut (their results go to the workspace)
 };
-// Finds the entry `b` (if b >= 0), or else the one that has part `group` of all entries' parts (b is set).  False: there is none.
-// Called by all threads of a block.  STEP: keys of a step.
+// Finds entry b, or for b < 0 the one that has part `group` of all entries' parts.  False: there is none.  Called by all threads
+// of a block, each of which looks at batch / kPagedThreads entries in a row.  STEP: keys of a step; heads: units of an entry.
 template <int D, int STEP>
-__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& cut_out, const PagedAttnParams& p, int64_t heads, int64_t group, int& b,
-                                           PagedCut& shared_cut, int& shared_b) {
+__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, int64_t heads, int64_t group, int b) {
   const PagedCache& c = p.c;
-  const int last = (c.batch - 1) / kPagedThreads * kPagedThreads;
-  int64_t total = 0;
-  int n = 0;
-  for (int base = last; base >= 0; base -= kPagedThreads) {
-    const int e = base + threadIdx.x;
-    n = e < c.batch ? paged_len(c, e) : 0;
-    uint64_t all;
-    paged_block_sum(sums, paged_steps<STEP>(c, n), all);
-    total += all;
-  }
-  const int64_t once = (total * heads + p.resident - 1) / p.resident;
+  const int per = (c.batch + kPagedThreads - 1) / kPagedThreads;
+  const int first = threadIdx.x * per, last = min(first + per, c.batch);
+  if (threadIdx.x == 0) found.entry = -1;  // (seen by all behind the sums' barriers)
+  uint64_t total = 0, all;
+  for (int e = first; e < last; ++e) total += paged_steps<STEP>(c, paged_len(c, e));
+  paged_block_sum(sums, total, all);
+  const int64_t once = (static_cast<int64_t>(all) * heads + p.resident - 1) / p.resident;
   const int64_t length = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<int64_t>(kPagedGoodSteps<D>))),
                              static_cast<int64_t>(kPagedMinKeys / STEP));
-  uint64_t before = 0;  // parts in the low half, parts of cut entries in the high half
-  for (int base = 0; base <= last; base += kPagedThreads) {
-    const int e = base + threadIdx.x;
-    if (base > 0) n = e < c.batch ? paged_len(c, e) : 0;
-    const int steps = paged_steps<STEP>(c, n);
-    const uint64_t parts = (steps + length - 1) / length;
-    uint64_t all;
-    const uint64_t upto = before + paged_block_sum(sums, parts | (parts > 1 ? parts << 32 : 0), all);
-    const uint64_t from = upto - (parts | (parts > 1 ? parts << 32 : 0));
-    const bool here = b >= 0 ? b >= base && b < base + kPagedThreads
-                             : group < static_cast<int64_t>((before + all) & 0xffffffffu);
-    if (here) {
-      const int64_t first = static_cast<int64_t>(from & 0xffffffffu);
-      if (b >= 0 ? e == b : group >= first && group < first + static_cast<int64_t>(parts)) {
-        shared_cut = PagedCut{n, steps, static_cast<int>(parts), first, static_cast<int64_t>(from >> 32)};
-        shared_b = e;
-      }
-      __syncthreads();
-      cut_out = shared_cut;
-      b = shared_b;
-      return true;
+  // parts in the low half, parts of cut entries in the high half
+  auto parts_of = [&](int steps) {
+    const uint64_t parts = static_cast<uint32_t>((steps + length - 1) / length);
+    return parts | (parts > 1 ? parts << 32 : 0);
+  };
+  uint64_t mine = 0;
+  for (int e = first; e < last; ++e) mine += parts_of(paged_steps<STEP>(c, paged_len(c, e)));
+  uint64_t from = paged_block_sum(sums, mine, all) - mine;
+  const int64_t low = static_cast<int64_t>(from & 0xffffffffu), high = low + static_cast<int64_t>(mine & 0xffffffffu);
+  if (b >= 0 ? b >= first && b < last : group >= low && group < high) {
+    for (int e = first; e < last; ++e) {
+      const int n = paged_len(c, e), steps = paged_steps<STEP>(c, n);
+      const uint64_t parts = parts_of(steps);
+      const int64_t before = static_cast<int64_t>(from & 0xffffffffu), count = static_cast<int64_t>(parts & 0xffffffffu);
+      if (b >= 0 ? e == b : group >= before && group < before + count)
+        found = PagedCut{e, n, steps, static_cast<int>(count), before, static_cast<int64_t>(from >> 32)};
+      from += parts;
     }
-    before += all;
   }
-  return false;
+  __syncthreads();
+  return found.entry >= 0;
 }
 
 // ---- one piece of a unit ----
@@ -643,7 +240,7 @@ struct PagedState {
 
 // What follows the first product: scores s of this lane's keys key and key + 8 of H slices, from key0 on, for query rows 2 t and
 // 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have; first_limit: first key that the
-// entry's first token does not see; 
+// entry's first token does not see.
 template <int H, int D, int NT, int HS>
 __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
                                               const float (&k_scale)[H], int first_limit, int row0, int group) {
@@ -1083,19 +680,20 @@ __device__ __forceinline__ int paged_merge_mix(int pair) {
 template <int D, class T, int NT>
 constexpr int paged_ctas_per_sm() {
   const int by_memory = (227 << 10) / (PagedSmem<D, T, NT>::kBytes + (2 << 10));
-  const int by_registers = NT * D <= 64 ? 5 : NT * D <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : NT * D < 256 || (NT * D == 256 && NT <= 2) || (NT * D == 384) ? 3 : 2;
+  constexpr int kOutput = NT * D;  // floats of a lane's share of the output, times four
+  const int by_registers = kOutput <= 64 ? 5 : kOutput <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : kOutput == 384 || (kOutput <= 256 && NT < 4) ? 3 : 2;
   return by_memory < by_registers ? by_memory : by_registers;
 }
 
 template <int D, class T, int NT>
-__global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+__global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>())
+fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(128) uint8_t paged_smem_raw[];
   __shared__ PagedSums sums;
-  __shared__ PagedCut shared_cut;
-  __shared__ int shared_b;
+  __shared__ PagedCut cut;
   __shared__ __align__(8) uint64_t barriers[kPagedWarps][L::kStages];
   __shared__ int abort_flag;
   uint8_t* paged_smem = paged_smem_raw + (L::kAlign - smem_u32(paged_smem_raw) % L::kAlign) % L::kAlign;
@@ -1113,9 +711,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>()) 
   const int chunks = (p.rows * group + kRows - 1) / kRows;
   const unsigned heads = c.heads_kv * chunks;  // units of an entry
   const int unit = blockIdx.x % heads;
-  int b = -1;
-  PagedCut cut;
-  if (!paged_find<D, kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads, b, shared_cut, shared_b)) return;
+  if (!paged_find<D, kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads, -1)) return;
+  const int b = cut.entry;
   const int part = static_cast<int>(blockIdx.x / heads - cut.group);
   const int step0 = static_cast<int>(static_cast<int64_t>(cut.steps) * part / cut.parts);
   const int step1 = static_cast<int>(static_cast<int64_t>(cut.steps) * (part + 1) / cut.parts);
@@ -1181,19 +778,19 @@ __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(cons
   static_assert(kCombineThreads == kPagedThreads, "a block finds an entry's cut");
   constexpr int kRows = 8 * NT;
   __shared__ PagedSums sums;
-  __shared__ PagedCut shared_cut;
-  __shared__ int shared_b;
+  __shared__ PagedCut cut;
   const PagedCache& c = p.c;
   const int group = p.heads_q / c.heads_kv;
   const int chunks = (p.rows * group + kRows - 1) / kRows;
   const int heads = c.heads_kv * chunks;
   const int row = blockIdx.x;
   const int head = row % p.heads_q, token = row / p.heads_q % p.rows;
-  int b = row / p.heads_q / p.rows;
-  PagedCut cut;
   // (the lengths were not written by the grid before, and whatever wrote them ended before that grid let this one start)
-  paged_find<D, STEP>(sums, cut, p, heads, 0, b, shared_cut, shared_b);
-  if (cut.parts == 1) return;
+  paged_find<D, STEP>(sums, cut, p, heads, 0, row / p.heads_q / p.rows);
+  if (cut.parts == 1) {
+    grid_dependency_wait();  // (this grid must not end before the one that wrote the result)
+    return;
+  }
   const int in_head = token * group + head % group;  // query row of the KV head
   const int64_t first = (cut.slot * heads + head / group * chunks + in_head / kRows) * kRows + in_head % kRows;
   auto at = [&](int i) { return first + static_cast<int64_t>(i) * heads * kRows; };
@@ -1240,8 +837,8 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
   if (groups * heads > 0x7fffffff) return cudaErrorInvalidValue;
   if (maps == nullptr) return e;
   p.part_ml = p.part_o + p.slots * 8 * NT * D;
-  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads), PagedSmem<D, T, NT>::kBytes, stream, p,
-                       maps[0], maps[1]);
+  e = launch_dependent(fal_paged_splitk_kernel<D, T, NT>, dim3(static_cast<unsigned>(groups * heads)), dim3(kPagedThreads),
+                       PagedSmem<D, T, NT>::kBytes, stream, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const unsigned rows = static_cast<unsigned>(p.c.batch) * p.rows * p.heads_q;
   return launch_dependent(fal_paged_combine_kernel<D, NT, kStep>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
@@ -1338,11 +935,6 @@ int paged_rows_per_cta(int rows, int kernel_dim) {
   const int tiles = (rows + 7) / 8, most = kernel_dim < 256 ? 4 : 2;
   const int passes = (tiles + most - 1) / most;
   return 8 * ((tiles + passes - 1) / passes);
-}
-
-cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
-  if (p.c.type == kPagedF16) return append_t<__half>(p, stream);
-  return p.c.type == kPagedS8 ? append_t<S8>(p, stream) : append_t<E4M3>(p, stream);
 }
 
 cudaError_t paged_attn_plan(PagedAttnParams& p) { return splitk(p, nullptr, nullptr); }

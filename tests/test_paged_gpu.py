@@ -129,7 +129,7 @@ def test_what_8_bit_pages_make_of_special_values(fal, dtype):
 @pytest.mark.parametrize("hq,hkv,d,page,layout", [(8, 2, 128, 16, "bshd"), (16, 1, 64, 64, "bhsd"), (3, 3, 32, 32, "bshd"),
                                                  (20, 1, 96, 16, "bhsd"), (4, 2, 256, 128, "bshd"), (6, 6, 128, 256, "bhsd")])
 @pytest.mark.parametrize("rows,lens", [(1, [1, 15, 16, 17, 255, 256, 257, 0, -1]), (1, [2049]), (1, [700, 9, 4100]),
-                                       (3, [3, 1, 16, 300, 0, -1, 35]), (16, [16, 40, 513, 7]), (130, [130, 200, 1000, 0, 64])])
+                                       (3, [3, 1, 16, 300, 0, -1, 35]), (16, [16, 40, 513, 7]), (130, [130, 200, 1000, 0, 64, -5])])
 def test_attention_over_pages(ext, fal, dtype, hq, hkv, d, page, layout, rows, lens):
     gen = torch.Generator().manual_seed(hq * d + rows)
     cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d)
@@ -144,6 +144,80 @@ def test_attention_over_pages(ext, fal, dtype, hq, hkv, d, page, layout, rows, l
         first = max(rows - max(n, 0), 0)
         assert not o[e, :first].any()  # queries before the first position
     assert ext.device_status() == 0
+
+
+# Many more entries than a block has threads, one of them long; with and without unused ones at the ends.
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("batch,rows", [(129, 1), (300, 1), (257, 3)])
+def test_many_entries(ext, fal, dtype, batch, rows):
+    gen = torch.Generator().manual_seed(batch)
+    hq, hkv, d, page = 4, 2, 64, 16
+    lens = [int(x) for x in torch.randint(0, 50, (batch,), generator=gen)]
+    lens[0], lens[batch // 2], lens[128], lens[-1] = -1, 3000, 77, 0
+    cache = _filled(gen, DTYPES[dtype], lens, page, hkv, d)
+    q = _rows(gen, batch, rows, hq, d)
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens), **cache.on_gpu("bshd")).cpu()
+    for e, n in enumerate(lens):
+        k, v = cache.dense(e, max(n, 0), as_half=False)
+        want, mag = attention(q[e], k, v, 1 / math.sqrt(d))
+        assert_close(o[e], want, mag, n, v.abs().max().item() if n > 0 else 0.0)
+    assert ext.device_status() == 0
+
+
+# Long entries, cut into many parts whose borders fall anywhere; every number of query rows that has a kernel of its own, full and
+# partial; lengths that end in the pages and in the tail.
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hq,hkv,d,rows", [(8, 1, 128, 1), (8, 1, 64, 2), (7, 1, 128, 3), (4, 1, 128, 8), (4, 1, 64, 24), (2, 1, 256, 8),
+                                           (5, 1, 256, 5), (3, 1, 96, 10), (2, 2, 32, 24)])
+def test_long_entries_and_every_number_of_rows(ext, fal, dtype, hq, hkv, d, rows):
+    gen = torch.Generator().manual_seed(d + rows)
+    lens = [9000, 4097, 2500]
+    cache = _filled(gen, DTYPES[dtype], lens, 64, hkv, d)
+    q = _rows(gen, 3, rows, hq, d)
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens), softmax_scale=0.3,
+                                          **cache.on_gpu("bshd")).cpu()
+    for e, n in enumerate(lens):
+        k, v = cache.dense(e, n, as_half=False)
+        want, mag = attention(q[e], k, v, 0.3)
+        assert_close(o[e], want, mag, n, v.abs().max().item())
+    assert ext.device_status() == 0
+
+
+def test_scores_of_every_size_and_order(fal):
+    """The largest score last, first, or the same throughout; scores far above and below what exponentials of 32 bits hold."""
+    hq, hkv, d, page, n = 2, 1, 64, 16, 400
+    for dtype in (torch.float16, torch.int8):
+        for slope in (-0.5, 0.0, 0.5, 4.0):
+            for offset in (0.0, -60.0, 60.0):
+                gen = torch.Generator().manual_seed(1)
+                cache = Cache(gen, dtype, 30, page, hkv, d, 1, 26)
+                cache.reserve(0, n)
+                k = torch.zeros(n, hkv, d)
+                k[:, 0, 0] = (torch.arange(n) - n / 2) * slope / 16 + offset  # (times q's 8: steps of slope / 2)
+                cache.append(0, k.half(), _rows(gen, n, hkv, d))
+                q = torch.zeros(1, 1, hq, d).half()
+                q[..., 0] = 8
+                o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens([n]), softmax_scale=1.0,
+                                                      **cache.on_gpu("bshd")).cpu()
+                kd, vd = cache.dense(0, n, as_half=False)
+                want, mag = attention(q[0], kd, vd, 1.0)
+                assert_close(o[0], want, mag, n, vd.abs().max().item())
+
+
+def test_values_behind_the_length_do_not_matter(fal):
+    """NaN and infinities in the rest of the last page, of other pages and of the tail, for every path."""
+    gen = torch.Generator().manual_seed(14)
+    for dtype in DTYPES:
+        for rows in (1, 5, 24, 40):
+            cache = _filled(gen, DTYPES[dtype], [41, 100], 32, 2, 64)
+            got = cache.on_gpu("bshd")
+            args = dict(block_table=cache.table.cuda(), cache_seqlens=_lens([41, 100]))
+            q = _rows(gen, 2, rows, 4, 64).cuda()
+            o = fal.flash_attn_with_paged_kvcache(q, **args, **got)
+            for n, t in got.items():
+                if dtype == "fp16" or n.endswith("tail"):
+                    t.masked_fill_(t.isnan(), math.inf)  # (the model leaves NaN there)
+            assert torch.equal(fal.flash_attn_with_paged_kvcache(q, **args, **got), o) and not o.isnan().any()
 
 
 def test_a_run_of_steps_as_a_server_makes_them(ext, fal):
