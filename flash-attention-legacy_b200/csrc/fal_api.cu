@@ -1187,7 +1187,8 @@ fal::PagedAttnParams paged_attn_params(const fal_paged_attn_args& a) {
   p.c = paged_cache(a.cache);
   p.q = a.q; p.q_strides = to_rs(&a.q_strides); p.o = a.o;
   p.heads_q = a.heads_q; p.rows = a.rows; p.kernel_dim = kernel_head_dim(a.cache.head_dim);
-  p.part_o = static_cast<float*>(a.workspace);
+  p.cuts = static_cast<int64_t*>(a.workspace);
+  p.part_o = reinterpret_cast<float*>(p.cuts + 2 * static_cast<int64_t>(a.cache.batch));
   p.scale = a.softmax_scale; p.status = a.status;
   return p;
 }
@@ -1214,7 +1215,7 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
     if (e == cudaErrorInvalidValue) return p;  // too many units for one grid: nothing that a workspace helps
     if (e != cudaSuccess) k.slots = kPagedUnknownSlots;
     const int per_cta = fal::paged_rows_per_cta(static_cast<int>(rows), dim);
-    p.total = static_cast<size_t>(k.slots) * per_cta * (dim + 2) * sizeof(float) + 16;
+    p.total = static_cast<size_t>(c.batch) * 2 * sizeof(int64_t) + static_cast<size_t>(k.slots) * per_cta * (dim + 2) * sizeof(float);
     return p;
   }
   const int64_t unit = capacity * c.head_dim * 4;  // K and V

@@ -20,8 +20,8 @@ __device__ __forceinline__ void merge_stats(float& m, float& l, float m2, float 
 // Waits for the grids before this one, then merges n partials into head_dim_real columns at out_row: the i-th has its
 // statistics at ml[index(i)] and its row at po[index(i) * D / 4].
 template <int D, int WARPS, class Index>
-__device__ __forceinline__ void combine_row(int tid, bool row_ok, int n, const float2* ml, const float4* po, Index index, __half* out_row,
-                                            int head_dim_real, float* lse) {
+__device__ __forceinline__ void combine_row(int tid, bool row_ok, int n, const float2* ml, const float4* po, Index index,
+                                            __half* out_row, int head_dim_real, float* lse) {
   static_assert(WARPS == 1 || WARPS * 32 == kCombineThreads, "a row per warp or per block");
   constexpr int kThreads = 32 * WARPS;                       // threads per row
   constexpr int kLanes = D / 4 < kThreads ? D / 4 : kThreads;  // threads per partial row

@@ -291,7 +291,8 @@ bool paged_cache(PyObject* const* args, int64_t batch, int64_t head_dim, PagedTe
     for (const at::Tensor* s : {x.ks, x.vs})
       if (s->size(0) != pages || s->size(1) != heads || !s->is_contiguous()) return false;
     for (const at::Tensor* s : {x.kt, x.vt})
-      if (s->size(0) != batch || s->size(1) != kp.size(1) || s->size(2) != kp.size(2) || s->size(3) != head_dim || !addressable(*s, 8))
+      if (s->size(0) != batch || s->size(1) != kp.size(1) || s->size(2) != kp.size(2) || s->size(3) != head_dim ||
+          !addressable(*s, 8))
         return false;
     if (storage(x.kt) == storage(x.vt)) return false;
     c.k_scales = x.ks->mutable_data_ptr<float>();
@@ -348,8 +349,10 @@ const at::Tensor* paged_rows(PyObject* obj, const PagedTensors& x) {
 fal_strides row_strides(const at::Tensor& t) { return {t.stride(0), t.stride(2), t.stride(1)}; }
 
 // Fills the append's block but for its outputs; q may be null.
-bool paged_append_block(const PagedTensors& x, const at::Tensor* q, const at::Tensor& k, const at::Tensor& v, fal_paged_append_args& a) {
-  if (k.sizes() != v.sizes() || k.size(0) != a.cache.batch || k.size(2) != a.cache.heads_kv || k.size(3) != a.cache.head_dim) return false;
+bool paged_append_block(const PagedTensors& x, const at::Tensor* q, const at::Tensor& k, const at::Tensor& v,
+                        fal_paged_append_args& a) {
+  if (k.sizes() != v.sizes() || k.size(0) != a.cache.batch || k.size(2) != a.cache.heads_kv || k.size(3) != a.cache.head_dim)
+    return false;
   if (q != nullptr) {
     if (q->size(0) != k.size(0) || q->size(1) != k.size(1) || q->size(3) != k.size(3)) return false;
     a.q = q->const_data_ptr();
@@ -427,7 +430,8 @@ PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize
   fal_paged_attn_args r{};
   if (q == nullptr || !paged_cache(args + 3, q->size(0), q->size(3), x, a.cache)) Py_RETURN_NONE;
   q = paged_rows(args[0], x);
-  if (q == nullptr || q->size(2) % a.cache.heads_kv != 0 || !scale_of(args[3 + kPagedArgs], q->size(3), r.softmax_scale)) Py_RETURN_NONE;
+  if (q == nullptr || q->size(2) % a.cache.heads_kv != 0 || !scale_of(args[3 + kPagedArgs], q->size(3), r.softmax_scale))
+    Py_RETURN_NONE;
   const bool appends = args[1] != Py_None;
   if (appends) {
     const at::Tensor* k = paged_rows(args[1], x);

@@ -240,6 +240,7 @@ struct PagedAttnParams {
   const void* q;         // [batch, rows, heads_q, head_dim] fp16 through strides (entry / head / row)
   RowStrides q_strides;
   void* o;               // [batch, rows, heads_q, head_dim] fp16, contiguous
+  int64_t* cuts;         // workspace [batch, 2]: parts of an entry with positions, and the first one's place; in front
   float* part_o;         // workspace [slots, rows per CTA, kernel head_dim]
   float* part_ml;        // workspace [slots, rows per CTA, 2], behind part_o
   int heads_q;

@@ -130,7 +130,9 @@ __device__ __forceinline__ void append_token(const PagedAppendParams& p, int tok
   const bool placed = start >= 0 && pos64 < capacity;  // (start < 0: an unused entry of a padded batch)
   const int pos = placed ? static_cast<int>(pos64) : 0;
   if (thread == 0) {
-    if (i == 0) p.new_lens[b] = start < 0 ? start : static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
+    if (i == 0)
+      p.new_lens[b] =
+          start < 0 ? start : static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
     if (start >= 0 && !placed && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
   }
   if (lane >= lanes) return;  // (head_dim 96)
@@ -352,7 +354,8 @@ cudaError_t append_t(const PagedAppendParams& p, cudaStream_t stream) {
   const int64_t pages = std::is_same<T, __half>::value ? 0 : (p.rows + (int64_t{1} << p.c.page_shift) - 1) >> p.c.page_shift;
   // threads to a head: kSealKept pieces each where that fills warps
   int64_t head_threads = 32;
-  while (head_threads < kAppendThreads && head_threads * kSealKept < (int64_t{p.c.head_dim / 16} << p.c.page_shift)) head_threads *= 2;
+  while (head_threads < kAppendThreads && head_threads * kSealKept < (int64_t{p.c.head_dim / 16} << p.c.page_shift))
+    head_threads *= 2;
   const int64_t at_once = kAppendThreads / head_threads;
   const int64_t page_blocks = pages * ((2 * p.c.heads_kv + at_once - 1) / at_once) * p.c.batch;
   const int64_t blocks = page_blocks + (tokens + 1) / 2;

@@ -27,8 +27,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // product of a 16-key slice is added to the output.  P^T of the scores' layout becomes the second product's operand by
 // movmatrix; its column sums, one more product with ones, are the softmax sum.
 //
-// An (entry, KV head, chunk of 8 NT query rows) is a unit; its keys count in steps of 64, a 16-key slice for each of four
-// warps.  Entries are cut into parts of one length that the GPU works out from all lengths, so that all units together
+// An (entry, KV head, chunk of 8 NT query rows) is a unit; its keys count in steps, one 16-key slice for each of four warps, or
+// two.  Entries are cut into parts of one length that the GPU works out from all lengths, so that all units together
 // make a few CTAs for every place on the GPU, whatever the lengths are; the units of one part are CTAs next to each other,
 // because their rows are next to each other in memory where a page holds all heads of a position.  Parts of a cut entry go
 // to the workspace and a second kernel merges them; a CTA that has all keys of its unit writes the result itself.
@@ -55,7 +55,8 @@ __device__ __forceinline__ void cp_async_16_bytes(uint32_t dst, const void* src,
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // D = A * B + C (fp16 16 x 16 and 16 x 8, fp32)
-__device__ __forceinline__ void mma_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+__device__ __forceinline__ void mma_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                               const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -170,8 +171,8 @@ constexpr float kNoKey = -1e30f;  // further below any score than an exponential
 // A part is as long as makes kPagedWaves CTAs of all units for every place on the GPU (SMs get unequal shares of the memory's
 // bandwidth), but no shorter than kPagedGoodSteps, which a CTA's set-up is small beside, as long as there is a CTA for every
 // place, nor than kPagedMinKeys.  (A length that makes the CTAs fill the places a whole number of times is no better.)
-// us with 1 / 2 / 4 CTAs for every place: 64 entries of 16 000 int8 positions, 8 heads of 128, 421 / 366 / 339, fp16 623 / 604 / 605, 16
-// fp16 - / 167 / 159; parts of 16 against 8 steps: 16 entries of 32 000 int8, 4 heads of 64, 57 / 61; 34 against 17: 16 of 5 000
+// us with 1 / 2 / 4 CTAs for every place: 64 entries of 16 000 int8 positions, 8 heads of 128, 421 / 366 / 339, fp16 623 / 604 /
+// 605, 16 fp16 - / 167 / 159; parts of 16 against 8 steps: 16 entries of 32 000 int8, 4 heads of 64, 57 / 61; 34 against 17: 16 of 5 000
 // e4m3, 16 heads of 256, 109 / 114.
 constexpr int kPagedMinKeys = 256;
 constexpr int kPagedWaves = 4;
@@ -187,10 +188,10 @@ struct PagedCut {
   int64_t group;  // parts of the entries before it
   int64_t slot;   // the same, of those that are cut (their results go to the workspace)
 };
-// Finds entry b, or for b < 0 the one that has part `group` of all entries' parts.  False: there is none.  Called by all threads
-// of a block, each of which looks at batch / kPagedThreads entries in a row.  STEP: keys of a step; heads: units of an entry.
+// Finds the entry that has part `group` of all entries' parts.  False: there is none.  Called by all threads of a block, each
+// of which looks at batch / kPagedThreads entries in a row.  STEP: keys of a step; heads: units of an entry.
 template <int D, int STEP>
-__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, int64_t heads, int64_t group, int b) {
+__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, int64_t heads, int64_t group) {
   const PagedCache& c = p.c;
   const int per = (c.batch + kPagedThreads - 1) / kPagedThreads;
   const int first = threadIdx.x * per, last = min(first + per, c.batch);
@@ -210,12 +211,12 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, con
   for (int e = first; e < last; ++e) mine += parts_of(paged_steps<STEP>(c, paged_len(c, e)));
   uint64_t from = paged_block_sum(sums, mine, all) - mine;
   const int64_t low = static_cast<int64_t>(from & 0xffffffffu), high = low + static_cast<int64_t>(mine & 0xffffffffu);
-  if (b >= 0 ? b >= first && b < last : group >= low && group < high) {
+  if (group >= low && group < high) {
     for (int e = first; e < last; ++e) {
       const int n = paged_len(c, e), steps = paged_steps<STEP>(c, n);
       const uint64_t parts = parts_of(steps);
       const int64_t before = static_cast<int64_t>(from & 0xffffffffu), count = static_cast<int64_t>(parts & 0xffffffffu);
-      if (b >= 0 ? e == b : group >= before && group < before + count)
+      if (group >= before && group < before + count)
         found = PagedCut{e, n, steps, static_cast<int>(count), before, static_cast<int64_t>(from >> 32)};
       from += parts;
     }
@@ -381,7 +382,8 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
         mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], zero);
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-          const uint64_t y = ffma2(pack_f32x2(x[e], x[e + 1]), pack_f32x2(v_scale, v_scale), pack_f32x2(st.o[nt][j][e], st.o[nt][j][e + 1]));
+          const uint64_t y = ffma2(pack_f32x2(x[e], x[e + 1]), pack_f32x2(v_scale, v_scale),
+                                   pack_f32x2(st.o[nt][j][e], st.o[nt][j][e + 1]));
           unpack_f32x2(y, st.o[nt][j][e], st.o[nt][j][e + 1]);
         }
       } else {
@@ -474,8 +476,8 @@ constexpr int kNoSlice = -2147483647;  // in place of a page: beyond the part
 
 // Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
 template <int D, class T, int NT>
-__device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, PagedRing& ring, uint32_t queries,
-                                            int b, int n, int kv_head, int row0, int rows_valid, int step0, int step1,
+__device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
+                                            PagedRing& ring, uint32_t queries, int b, int n, int kv_head, int row0, int rows_valid, int step0, int step1,
                                             PagedState<D, NT, kPagedSlices<D, T, NT>>& st) {
   using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
@@ -567,7 +569,8 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       for (int it = 0; it < Tail::kLoads; ++it) {
         const int r = it * Tail::kCopyRows + lane / Tail::kChunks;
         const bool ok = row + r < tail_end && ch * 8 < c.head_dim;
-        cp_async_16_bytes(ring.base + fill * L::kStageBytes + Tail::place(r, ch), ok ? src + r * s.row + ch * 8 : src, ok ? 16u : 0u);
+        cp_async_16_bytes(ring.base + fill * L::kStageBytes + Tail::place(r, ch), ok ? src + r * s.row + ch * 8 : src,
+                          ok ? 16u : 0u);
       }
       cp_async_commit();
     }
@@ -643,7 +646,9 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       for (int x = rows * (Tile::kBlockRow / 16) + lane; x < kPagedSlice * (Tile::kBlockRow / 16); x += 32)
 #pragma unroll
         for (int block = 0; block < Tile::kBlocks; ++block)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(stage + L::kTensorBytes + block * Tile::kBlockBytes + x * 16), "r"(0) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(stage + L::kTensorBytes + block * Tile::kBlockBytes + x * 16),
+                       "r"(0)
+                       : "memory");
       __syncwarp();
     }
     float s[kH][NT][4];
@@ -681,13 +686,17 @@ template <int D, class T, int NT>
 constexpr int paged_ctas_per_sm() {
   const int by_memory = (227 << 10) / (PagedSmem<D, T, NT>::kBytes + (2 << 10));
   constexpr int kOutput = NT * D;  // floats of a lane's share of the output, times four
-  const int by_registers = kOutput <= 64 ? 5 : kOutput <= 128 && kPagedSlices<D, T, NT> == 1 ? 4 : kOutput == 384 || (kOutput <= 256 && NT < 4) ? 3 : 2;
+  const int by_registers = kOutput <= 64                                        ? 5
+                           : kOutput <= 128 && kPagedSlices<D, T, NT> == 1      ? 4
+                           : kOutput == 384 || (kOutput <= 256 && NT < 4)       ? 3
+                                                                                : 2;
   return by_memory < by_registers ? by_memory : by_registers;
 }
 
 template <int D, class T, int NT>
 __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm<D, T, NT>())
-fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap k_map,
+                        const __grid_constant__ CUtensorMap v_map) {
   using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
   constexpr int kRows = 8 * NT;
@@ -711,9 +720,13 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
   const int chunks = (p.rows * group + kRows - 1) / kRows;
   const unsigned heads = c.heads_kv * chunks;  // units of an entry
   const int unit = blockIdx.x % heads;
-  if (!paged_find<D, kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads, -1)) return;
+  if (!paged_find<D, kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads)) return;
   const int b = cut.entry;
   const int part = static_cast<int>(blockIdx.x / heads - cut.group);
+  if (unit == 0 && part == 0 && threadIdx.x == 0) {  // for the merge
+    p.cuts[2 * b] = cut.parts;
+    p.cuts[2 * b + 1] = cut.slot;
+  }
   const int step0 = static_cast<int>(static_cast<int64_t>(cut.steps) * part / cut.parts);
   const int step1 = static_cast<int>(static_cast<int64_t>(cut.steps) * (part + 1) / cut.parts);
   const int kv_head = unit / chunks;
@@ -722,7 +735,8 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   PagedRing ring{smem_u32(paged_smem) + warp * L::kRingBytes, smem_u32(&barriers[warp][0]), 0u, WaitCtx{&abort_flag, p.status}};
   PagedState<D, NT, kPagedSlices<D, T, NT>> st;
-  paged_piece<D, T, NT>(p, &k_map, &v_map, ring, smem_u32(paged_smem) + L::kQueryOffset, b, cut.n, kv_head, row0, rows_valid, step0, step1, st);
+  paged_piece<D, T, NT>(p, &k_map, &v_map, ring, smem_u32(paged_smem) + L::kQueryOffset, b, cut.n, kv_head, row0, rows_valid,
+                        step0, step1, st);
   __syncthreads();  // the ring becomes the place of the warps' results
 
   // (column pair c of a row is at c ^ (its lane / 2): eight lanes and four rows of a store hit different banks)
@@ -740,8 +754,7 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
             make_float2(st.o[nt][j][x], st.o[nt][j][2 + x]);
       }
       if (g == 0)
-        *reinterpret_cast<float2*>(mml + row * 2) =
-            make_float2(st.m[nt][x], st.l[nt][x]);
+        *reinterpret_cast<float2*>(mml + row * 2) = make_float2(st.m[nt][x], st.l[nt][x]);
     }
   }
   __syncthreads();
@@ -755,7 +768,8 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) {
       const float x = fast_exp2(mml[(w * kRows + r) * 2] - most);
-      const float2 y = *reinterpret_cast<const float2*>(mo + (w * kRows + r) * L::kPitch + (pair ^ paged_merge_mix<D, T>(pair)) * 2);
+      const float2 y =
+          *reinterpret_cast<const float2*>(mo + (w * kRows + r) * L::kPitch + (pair ^ paged_merge_mix<D, T>(pair)) * 2);
       o0 += x * y.x;
       o1 += x * y.y;
       l += x * mml[(w * kRows + r) * 2 + 1];
@@ -763,7 +777,8 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
     if (cut.parts == 1) {
       const float inv = l != 0.f ? 1.f / l : 0.f;  // (0: the row sees no key)
       const int head = kv_head * group + (row0 + r) % group;
-      __half* out = static_cast<__half*>(p.o) + ((static_cast<int64_t>(b) * p.rows + (row0 + r) / group) * p.heads_q + head) * c.head_dim;
+      __half* out =
+          static_cast<__half*>(p.o) + ((static_cast<int64_t>(b) * p.rows + (row0 + r) / group) * p.heads_q + head) * c.head_dim;
       if (2 * pair < c.head_dim) *reinterpret_cast<uint32_t*>(out + 2 * pair) = pack_half2(o0 * inv, o1 * inv);
     } else {
       *reinterpret_cast<float2*>(p.part_o + (slot + r) * D + 2 * pair) = make_float2(o0, o1);
@@ -773,28 +788,23 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
 }
 
 // Merges the parts of the entries that were cut, and writes the zeros of entries without positions.
-template <int D, int NT, int STEP>
+template <int D, int NT>
 __global__ void __launch_bounds__(kCombineThreads) fal_paged_combine_kernel(const PagedAttnParams p) {
-  static_assert(kCombineThreads == kPagedThreads, "a block finds an entry's cut");
   constexpr int kRows = 8 * NT;
-  __shared__ PagedSums sums;
-  __shared__ PagedCut cut;
   const PagedCache& c = p.c;
   const int group = p.heads_q / c.heads_kv;
   const int chunks = (p.rows * group + kRows - 1) / kRows;
   const int heads = c.heads_kv * chunks;
   const int row = blockIdx.x;
-  const int head = row % p.heads_q, token = row / p.heads_q % p.rows;
-  // (the lengths were not written by the grid before, and whatever wrote them ended before that grid let this one start)
-  paged_find<D, STEP>(sums, cut, p, heads, 0, row / p.heads_q / p.rows);
-  if (cut.parts == 1) {
-    grid_dependency_wait();  // (this grid must not end before the one that wrote the result)
-    return;
-  }
+  const int head = row % p.heads_q, token = row / p.heads_q % p.rows, b = row / p.heads_q / p.rows;
+  grid_dependency_wait();
+  const longlong2 cut = *reinterpret_cast<const longlong2*>(p.cuts + 2 * b);
+  const int parts = paged_len(c, b) > 0 ? static_cast<int>(cut.x) : 0;
+  if (parts == 1) return;
   const int in_head = token * group + head % group;  // query row of the KV head
-  const int64_t first = (cut.slot * heads + head / group * chunks + in_head / kRows) * kRows + in_head % kRows;
+  const int64_t first = (cut.y * heads + head / group * chunks + in_head / kRows) * kRows + in_head % kRows;
   auto at = [&](int i) { return first + static_cast<int64_t>(i) * heads * kRows; };
-  combine_row<D, kCombineThreads / 32>(threadIdx.x, true, cut.parts, reinterpret_cast<const float2*>(p.part_ml),
+  combine_row<D, kCombineThreads / 32>(threadIdx.x, true, parts, reinterpret_cast<const float2*>(p.part_ml),
                                        reinterpret_cast<const float4*>(p.part_o), at,
                                        static_cast<__half*>(p.o) + static_cast<int64_t>(row) * c.head_dim, c.head_dim, nullptr);
 }
@@ -827,7 +837,8 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
   if (e != cudaSuccess) return e;
   const int64_t chunks = (static_cast<int64_t>(p.rows) * (p.heads_q / p.c.heads_kv) + 8 * NT - 1) / (8 * NT);
   const int64_t heads = p.c.heads_kv * chunks;
-  // Parts of all entries: one each, and as many more as there are CTAs to make; and no more than kPagedMinKeys make of full entries.
+  // Parts of all entries: one each, and as many more as there are CTAs to make; and no more than kPagedMinKeys make of full
+  // entries.
   constexpr int kStep = kPagedStep<D, T, NT>, kMinSteps = kPagedMinKeys / kStep;
   const int64_t steps = ((static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) + kStep - 1) / kStep + 1;
   const int64_t parts = static_cast<int64_t>(kPagedWaves) * p.resident;
@@ -841,7 +852,7 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
                        PagedSmem<D, T, NT>::kBytes, stream, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
   const unsigned rows = static_cast<unsigned>(p.c.batch) * p.rows * p.heads_q;
-  return launch_dependent(fal_paged_combine_kernel<D, NT, kStep>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
+  return launch_dependent(fal_paged_combine_kernel<D, NT>, dim3(rows), dim3(kCombineThreads), 0, stream, p);
 }
 
 template <int D, class T>
@@ -924,7 +935,8 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
     }
   }
   const int64_t capacity = paged_capacity(c);
-  __half* dst = static_cast<__half*>(is_v ? p.v_out : p.k_out) + ((static_cast<int64_t>(e) * p.heads + hh) * capacity + pos) * c.head_dim + col;
+  __half* dst =
+      static_cast<__half*>(is_v ? p.v_out : p.k_out) + ((static_cast<int64_t>(e) * p.heads + hh) * capacity + pos) * c.head_dim + col;
   reinterpret_cast<uint4*>(dst)[0] = out[0];
   reinterpret_cast<uint4*>(dst)[1] = out[1];
 }
