@@ -191,29 +191,32 @@ struct PagedCut {
 // Finds the entry that has part `group` of all entries' parts.  False: there is none.  Called by all threads of a block, each
 // of which looks at batch / kPagedThreads entries in a row.  STEP: keys of a step; heads: units of an entry.
 template <int D, int STEP>
-__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, int64_t heads, int64_t group) {
+__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, unsigned heads, int64_t group) {
   const PagedCache& c = p.c;
   const int per = (c.batch + kPagedThreads - 1) / kPagedThreads;
   const int first = threadIdx.x * per, last = min(first + per, c.batch);
   if (threadIdx.x == 0) found.entry = -1;  // (seen by all behind the sums' barriers)
+  const int n_first = first < last ? paged_len(c, first) : 0;
+  auto len_of = [&](int e) { return e == first ? n_first : paged_len(c, e); };
   uint64_t total = 0, all;
-  for (int e = first; e < last; ++e) total += paged_steps<STEP>(c, paged_len(c, e));
+  for (int e = first; e < last; ++e) total += paged_steps<STEP>(c, len_of(e));
   paged_block_sum(sums, total, all);
-  const int64_t once = (static_cast<int64_t>(all) * heads + p.resident - 1) / p.resident;
-  const int64_t length = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<int64_t>(kPagedGoodSteps<D>))),
-                             static_cast<int64_t>(kPagedMinKeys / STEP));
+  const uint64_t once = (all * heads + p.resident - 1) / p.resident;
+  const uint64_t wanted = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<uint64_t>(kPagedGoodSteps<D>))),
+                              static_cast<uint64_t>(kPagedMinKeys / STEP));
+  const uint32_t length = static_cast<uint32_t>(min(wanted, uint64_t{1} << 30));  // (no entry has more steps)
   // parts in the low half, parts of cut entries in the high half
   auto parts_of = [&](int steps) {
-    const uint64_t parts = static_cast<uint32_t>((steps + length - 1) / length);
+    const uint64_t parts = (static_cast<uint32_t>(steps) + length - 1) / length;
     return parts | (parts > 1 ? parts << 32 : 0);
   };
   uint64_t mine = 0;
-  for (int e = first; e < last; ++e) mine += parts_of(paged_steps<STEP>(c, paged_len(c, e)));
+  for (int e = first; e < last; ++e) mine += parts_of(paged_steps<STEP>(c, len_of(e)));
   uint64_t from = paged_block_sum(sums, mine, all) - mine;
   const int64_t low = static_cast<int64_t>(from & 0xffffffffu), high = low + static_cast<int64_t>(mine & 0xffffffffu);
   if (group >= low && group < high) {
     for (int e = first; e < last; ++e) {
-      const int n = paged_len(c, e), steps = paged_steps<STEP>(c, n);
+      const int n = len_of(e), steps = paged_steps<STEP>(c, n);
       const uint64_t parts = parts_of(steps);
       const int64_t before = static_cast<int64_t>(from & 0xffffffffu), count = static_cast<int64_t>(parts & 0xffffffffu);
       if (group >= before && group < before + count)
@@ -722,13 +725,14 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
   const int unit = blockIdx.x % heads;
   if (!paged_find<D, kPagedStep<D, T, NT>>(sums, cut, p, heads, blockIdx.x / heads)) return;
   const int b = cut.entry;
-  const int part = static_cast<int>(blockIdx.x / heads - cut.group);
+  const unsigned part = blockIdx.x / heads - static_cast<unsigned>(cut.group);
   if (unit == 0 && part == 0 && threadIdx.x == 0) {  // for the merge
     p.cuts[2 * b] = cut.parts;
     p.cuts[2 * b + 1] = cut.slot;
   }
-  const int step0 = static_cast<int>(static_cast<int64_t>(cut.steps) * part / cut.parts);
-  const int step1 = static_cast<int>(static_cast<int64_t>(cut.steps) * (part + 1) / cut.parts);
+  const unsigned parts = cut.parts, steps = cut.steps, longer = steps % parts;  // the first ones have a step more
+  const int step0 = part * (steps / parts) + min(static_cast<unsigned>(part), longer);
+  const int step1 = step0 + steps / parts + (part < longer ? 1 : 0);
   const int kv_head = unit / chunks;
   const int row0 = unit % chunks * kRows;  // of the KV head's rows * group query rows
   const int rows_valid = min(kRows, p.rows * group - row0);
