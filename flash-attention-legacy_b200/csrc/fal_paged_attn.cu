@@ -172,12 +172,14 @@ constexpr float kNoKey = -1e30f;  // further below any score than an exponential
 // bandwidth), but no shorter than kPagedGoodSteps, which a CTA's set-up is small beside, as long as there is a CTA for every
 // place, nor than kPagedMinKeys.  (A length that makes the CTAs fill the places a whole number of times is no better.)
 // us with 1 / 2 / 4 CTAs for every place: 64 entries of 16 000 int8 positions, 8 heads of 128, 421 / 366 / 339, fp16 623 / 604 /
-// 605, 16 fp16 - / 167 / 159; parts of 16 against 8 steps: 16 entries of 32 000 int8, 4 heads of 64, 57 / 61; 34 against 17: 16 of 5 000
-// e4m3, 16 heads of 256, 109 / 114.
+// 605, 16 fp16 - / 167 / 159.  Parts of 8 / 16 / 32 steps: 16 entries of 32 000 int8, 4 heads of 64, 60 / 56 / 53, 16 of 6 000 with
+// 5 tokens, 8 heads of 64, 57 / 49 / 53; 16 of 16 000 int8, 8 heads of 128, 99 / 104 / -, 20 of 5 000 48 / 59 / - (128 keys to a step);
+// with 16 heads to a KV head 57 / 52 / -, 12 of 2 000 fp16 with 5 tokens 39 / 31 / -, 8 of 6 000 int8 45 / 49 / 49, 30 000 38 / 29 / -;
+// 16 of 5 000 e4m3, 16 heads of 256, 119 / 119 / 110.
 constexpr int kPagedMinKeys = 256;
 constexpr int kPagedWaves = 4;
-template <int D>
-constexpr int kPagedGoodSteps = D == 64 ? 16 : D == 128 ? 8 : 32;
+template <int D, int STEP>
+constexpr int kPagedGoodSteps = D == 256 ? 32 : D == 128 && STEP > 64 ? 8 : 16;
 
 // How an entry is cut.
 struct PagedCut {
@@ -202,7 +204,7 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, con
   for (int e = first; e < last; ++e) total += paged_steps<STEP>(c, len_of(e));
   paged_block_sum(sums, total, all);
   const uint64_t once = (all * heads + p.resident - 1) / p.resident;
-  const uint64_t wanted = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<uint64_t>(kPagedGoodSteps<D>))),
+  const uint64_t wanted = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<uint64_t>(kPagedGoodSteps<D, STEP>))),
                               static_cast<uint64_t>(kPagedMinKeys / STEP));
   const uint32_t length = static_cast<uint32_t>(min(wanted, uint64_t{1} << 30));  // (no entry has more steps)
   // parts in the low half, parts of cut entries in the high half
