@@ -391,7 +391,8 @@ int fwd_batched(const void* q, const void* k, const void* v, void* o, float* lse
                 int seqlen_k, int head_dim, const fal_strides* q_strides,
                 const fal_strides* k_strides, const fal_strides* v_strides,
                 const fal_strides* o_strides, float softmax_scale, int is_causal, int* status,
-                void* stream, void* workspace = nullptr, size_t workspace_bytes = 0) {
+                void* stream, void* workspace = nullptr, size_t workspace_bytes = 0, const float4* key_scales = nullptr,
+                int key_blocks = 0) {
   if (!q || !k || !v || !o || !lse || !q_strides || !k_strides || !v_strides || !o_strides)
     return FAL_ERR_INVALID_ARGUMENT;
   if (batch <= 0 || heads_q <= 0 || heads_kv <= 0 || seqlen_q <= 0 || seqlen_k < 0)
@@ -442,6 +443,8 @@ int fwd_batched(const void* q, const void* k, const void* v, void* o, float* lse
   else p.shift_per_sequence = is_causal == FAL_CAUSAL_BOTTOM_RIGHT ? 1 : 0;
   p.scale = softmax_scale;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.key_scales = key_scales;
+  p.key_blocks = key_blocks;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int kdim = kernel_head_dim(head_dim);
@@ -1197,7 +1200,8 @@ fal::PagedAttnParams paged_attn_params(const fal_paged_attn_args& a) {
 struct PagedPlan {
   bool few_rows;
   int entries, heads;  // many rows: (entry, KV head) pairs whose rows are put in order at a time
-  size_t k_bytes, lse_bytes, split_bytes;
+  int key_blocks;      // of an (entry, KV head), 0 for fp16 pages
+  size_t k_bytes, scale_bytes, lse_bytes, split_bytes;
   size_t total;
 };
 
@@ -1227,9 +1231,11 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
     p.entries = static_cast<int>(e < 1 ? 1 : e < c.batch ? e : c.batch);
   }
   p.k_bytes = static_cast<size_t>(p.entries) * p.heads * capacity * c.head_dim * 2;
+  p.key_blocks = c.dtype != FAL_PAGED_F16 ? static_cast<int>(round_up(capacity, 128) / fal::kPagedBoxRows) : 0;
+  p.scale_bytes = static_cast<size_t>(p.entries) * p.heads * p.key_blocks * sizeof(float4);
   p.lse_bytes = round_up(static_cast<int64_t>(p.entries) * p.heads * group * a.rows * 4, 256);
   p.split_bytes = fal_fwd_kvcache_workspace_bytes(p.entries, p.heads * group, a.rows, static_cast<int>(capacity), c.head_dim);
-  p.total = 2 * p.k_bytes + p.lse_bytes + p.split_bytes;
+  p.total = 2 * p.k_bytes + p.scale_bytes + p.lse_bytes + p.split_bytes;
   return p;
 }
 
@@ -1317,8 +1323,11 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
   g.k_out = ws;
   g.v_out = ws + plan.k_bytes;
   g.status = a->status;
-  float* lse = reinterpret_cast<float*>(ws + 2 * plan.k_bytes);
-  void* split = plan.split_bytes != 0 ? ws + 2 * plan.k_bytes + plan.lse_bytes : nullptr;
+  g.scales_out = plan.key_blocks != 0 ? reinterpret_cast<float4*>(ws + 2 * plan.k_bytes) : nullptr;
+  g.key_blocks = plan.key_blocks;
+  g.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  float* lse = reinterpret_cast<float*>(ws + 2 * plan.k_bytes + plan.scale_bytes);
+  void* split = plan.split_bytes != 0 ? ws + 2 * plan.k_bytes + plan.scale_bytes + plan.lse_bytes : nullptr;
   const fal_strides o_strides = {static_cast<int64_t>(a->rows) * a->heads_q * c.head_dim, c.head_dim,
                                  static_cast<int64_t>(a->heads_q) * c.head_dim};
   for (g.b0 = 0; g.b0 < c.batch; g.b0 += plan.entries) {
@@ -1333,7 +1342,8 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
       __half* o = static_cast<__half*>(a->o) + g.b0 * o_strides.batch + g.h0 * group * o_strides.head;
       rc = fwd_batched(q, g.k_out, g.v_out, o, lse, c.cache_seqlens + g.b0, g.entries, g.heads * group, g.heads, a->rows,
                        capacity, c.head_dim, &a->q_strides, &kv, &kv, &o_strides, a->softmax_scale,
-                       FAL_CAUSAL_BOTTOM_RIGHT, a->status, a->stream, split, plan.split_bytes);
+                       FAL_CAUSAL_BOTTOM_RIGHT, a->status, a->stream, split, plan.split_bytes, g.scales_out,
+                       plan.key_blocks);
       if (rc != FAL_OK) return rc;
     }
   }

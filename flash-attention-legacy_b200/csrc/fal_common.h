@@ -55,6 +55,11 @@ struct FwdParams {
                              // lengths); seqlen_k is then the capacity, and shift_per_sequence applies per entry
   int heaviest_first;  // (shift_per_sequence, seqused_k, at most kOrderedEntries entries) blocks with most keys first
   int kv_splits;     // (seqused_k) CTAs that share a query block's keys, each a range of key tiles; 1: none
+  // Batched causal mode, optional: K and V hold whole numbers or other codes, whose values are theirs times a scale for every 16
+  // keys: [batch, heads_kv, key_blocks] (K's scale x scale_log2, log2 of V's scale, 1 / V's scale, -), as far as the last
+  // key's tile of 128 reaches.
+  const float4* key_scales;
+  int key_blocks;
   float* part_o;     // kv_splits > 1: [split, batch, heads_q, seqlen_q, head_dim] fp32, normalised per split
   float* part_lse;   // [split, batch, heads_q, seqlen_q]
   float scale;       // softmax scale

@@ -69,6 +69,7 @@ enum FwdShape : int {
 constexpr int kTileM = 128;   // query rows per softmax warpgroup
 constexpr int kTileN = 128;   // keys per step
 constexpr float kNegInf = -INFINITY;
+constexpr float kLn2 = 0.6931471805599453f;
 // Skip the O rescale while the running maximum grows by less than 2^8.
 constexpr float kRescaleThreshold = 8.0f;
 
@@ -323,7 +324,10 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
 // alignment); the kernels of the reference's own top-left mask are compiled without it.
 // SPLIT: the keys of a query block are dealt to gridDim.y CTAs.  A kernel of its own: the code costs the others up
 // to 5 % (short rows at head_dim 256 without a mask 12.8 -> 13.3 us, 16 heads x 16 384 of 64 causal 755 -> 791).
-template <int D, bool CAUSAL, bool SHIFTED, int SHAPE, bool SPLIT>
+// SCALED: K and V are codes with a scale for every 16 keys (FwdParams::key_scales).  A code is exact in fp16; its value, rounded,
+// would not be.  K's scale multiplies the scores.  V's is part of the weight: P = 2^(s + log2 v - m), with m the largest
+// such exponent so far, so that P keeps its bits however the scales differ, and the row sums add P / v.
+template <int D, bool CAUSAL, bool SHIFTED, int SHAPE, bool SPLIT, bool SCALED>
 __global__ void __launch_bounds__(FwdSmem<D, SHAPE>::kThreads, FwdSmem<D, SHAPE>::kCtasPerSm)
 fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -332,6 +336,7 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   constexpr int NS = L::kStages;
   constexpr int kSmWarps = L::kSmWarps;
   static_assert(!SPLIT || (SHAPE == kOneTile && (SHIFTED || !CAUSAL)), "a split chunk behind a cache");
+  static_assert(!SCALED || SHIFTED, "codes are those of a cache");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* sgen = smem_raw + (sbase - smem_u32(smem_raw));
@@ -689,7 +694,10 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t tP = kAlt ? tmem_base + lane_addr + 256 + wg * 64
                              : L::kSepP ? tmem_base + lane_addr + L::kPCol + wg * 64 : tS;  // packed fp16 P
     const int nt = kAlt ? ntile[0] : ntile[wg];
-    const float c2 = p.scale_log2;
+    const float c2 = SCALED ? 1.f : p.scale_log2;  // (in key_scales)
+    const float4* key_scales = nullptr;
+    if constexpr (SCALED)
+      key_scales = p.key_scales + (static_cast<int64_t>(wk.batch) * p.heads_kv + wk.kv_head) * p.key_blocks + wk.k_row0 / 16;
     // kAlt: the reference maximum of a row travels between the two threads that own the row (same
     // quarter, same lane, other warpgroup) through xm[row]; named barrier 1 + 2 quarter + w says
     // "warpgroup w has published" (the publisher arrives, the reader syncs; the two strictly alternate).
@@ -751,6 +759,13 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             a = fmaxf(a, __uint_as_float(sr[c][b0 + 15]));
             part[c * 2 + hlf] = a;
           }
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            const float4 x = __ldg(key_scales + j * 8 + b);
+            part[b] = __fmaf_rn(part[b], x.x, x.y);
+          }
+        }
         mx = fmaxf(fmax3(part[0], part[1], part[2]), fmax3(part[3], part[4], part[5]));
         mx = fmax3(mx, part[6], part[7]);
       }
@@ -807,22 +822,40 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
       // P = exp2(s * c2 - m * c2) from the registers, four independent row-sum chains,
       // fp16 P back into TMEM over the first half of S.
-      const uint64_t c2p = pack_f32x2(c2, c2);
-      const uint64_t moffp = pack_f32x2(-moff, -moff);
+      uint64_t c2p = pack_f32x2(c2, c2);
+      uint64_t moffp = pack_f32x2(-moff, -moff);
       uint64_t sum_a = pack_f32x2(0.f, 0.f), sum_b = sum_a;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
+        uint64_t block_a = 0, block_b = 0, inv_v = 0;  // (SCALED: of 16 keys)
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
+          if constexpr (SCALED) {
+            if (i % 16 == 0) {
+              const float4 x = __ldg(key_scales + j * 8 + c * 2 + i / 16);
+              c2p = pack_f32x2(x.x, x.x);
+              moffp = pack_f32x2(x.y - moff, x.y - moff);
+              inv_v = pack_f32x2(x.z, x.z);
+            }
+          }
           const uint64_t x01 = ffma2(pack_f32x2(__uint_as_float(sr[c][i + 0]), __uint_as_float(sr[c][i + 1])),
                                      c2p, moffp);
           const uint64_t x23 = ffma2(pack_f32x2(__uint_as_float(sr[c][i + 2]), __uint_as_float(sr[c][i + 3])),
                                      c2p, moffp);
           const uint64_t p01 = exp2_pair(x01);
           const uint64_t p23 = exp2_pair(x23);
-          sum_a = fadd2(sum_a, p01);
-          sum_b = fadd2(sum_b, p23);
+          if constexpr (SCALED) {
+            block_a = i % 16 == 0 ? p01 : fadd2(block_a, p01);
+            block_b = i % 16 == 0 ? p23 : fadd2(block_b, p23);
+            if (i % 16 == 12) {
+              sum_a = ffma2(block_a, inv_v, sum_a);
+              sum_b = ffma2(block_b, inv_v, sum_b);
+            }
+          } else {
+            sum_a = fadd2(sum_a, p01);
+            sum_b = fadd2(sum_b, p23);
+          }
           float p0, p1, p2, p3;
           unpack_f32x2(p01, p0, p1);
           unpack_f32x2(p23, p2, p3);
@@ -936,7 +969,7 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       }
     }
     if (row_ok && (!kAlt || wg == 0)) {
-      const float lse = (nt > 0 && m_ref != kNegInf) ? m_ref * p.scale + logf(fmaxf(l, 1e-20f))
+      const float lse = (nt > 0 && m_ref != kNegInf) ? m_ref * (SCALED ? kLn2 : p.scale) + logf(fmaxf(l, 1e-20f))
                                                       : kNegInf;
       if (SPLIT && shared) p.part_lse[part_row] = lse;
       else p.lse[wk.lse_base + static_cast<int64_t>(q_local) * p.lse_strides.row] = lse;
@@ -1021,11 +1054,11 @@ __global__ void __launch_bounds__(128) fal_fwd_combine_kernel(const FwdParams p)
     p.lse[b * p.lse_strides.batch + head * p.lse_strides.head + row] = m == kNegInf ? kNegInf : m + logf(fmaxf(sum, 1e-20f));
 }
 
-template <int D, bool CAUSAL, bool SHIFTED, int SHAPE, bool SPLIT = false>
+template <int D, bool CAUSAL, bool SHIFTED, int SHAPE, bool SPLIT = false, bool SCALED = false>
 cudaError_t launch_fwd_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          const CUtensorMap& to, const FwdParams& p, int grid, cudaStream_t stream) {
   using L = FwdSmem<D, SHAPE>;
-  auto kern = fal_fwd_kernel<D, CAUSAL, SHIFTED, SHAPE, SPLIT>;
+  auto kern = fal_fwd_kernel<D, CAUSAL, SHIFTED, SHAPE, SPLIT, SCALED>;
   static DeviceOnce configured;  // one per template instance
   cudaError_t e = configured.run([&] {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAllocBytes);
@@ -1040,6 +1073,14 @@ cudaError_t launch_fwd_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
 template <int D, int SHAPE>
 cudaError_t launch_fwd_d(bool causal, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          const CUtensorMap& to, const FwdParams& p, int grid, cudaStream_t stream) {
+  if (p.key_scales != nullptr) {
+    if (!causal || p.shift_per_sequence == 0) return cudaErrorInvalidValue;  // no such instance
+    if constexpr (SHAPE == kOneTile) {
+      if (p.kv_splits > 1) return launch_fwd_t<D, true, true, SHAPE, true, true>(tq, tk, tv, to, p, grid, stream);
+    }
+    if (p.kv_splits > 1) return cudaErrorInvalidValue;
+    return launch_fwd_t<D, true, true, SHAPE, false, true>(tq, tk, tv, to, p, grid, stream);
+  }
   if constexpr (SHAPE == kOneTile) {
     if (p.kv_splits > 1 && causal && p.shift_per_sequence != 0)
       return launch_fwd_t<D, true, true, SHAPE, true>(tq, tk, tv, to, p, grid, stream);

@@ -259,11 +259,15 @@ cudaError_t paged_attn_plan(PagedAttnParams& p);  // sets p.resident and p.slots
 constexpr int kPagedBoxRows = 16;
 cudaError_t launch_paged_attn(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t stream);
 
-// Entries b0 ... b0 + entries - 1 and KV heads h0 ... h0 + heads - 1 of a paged cache as fp16 rows in order.
+// Entries b0 ... b0 + entries - 1 and KV heads h0 ... h0 + heads - 1 of a paged cache as fp16 rows in order: codes of 8-bit pages
+// as they are, with their scales as FwdParams::key_scales has them.
 struct PagedGatherParams {
   PagedCache c;
   void* k_out;           // [entries, heads, capacity, head_dim]
   void* v_out;
+  float4* scales_out;    // 8-bit pages: [entries, heads, key_blocks]
+  int key_blocks;        // a multiple of 8
+  float scale_log2;      // softmax scale x log2(e)
   int b0, entries, h0, heads;
   int* status;
 };

@@ -888,7 +888,13 @@ cudaError_t splitk(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t str
 // ---------------------------------------------------------------------------
 // Rows in order, for the forward kernel
 // ---------------------------------------------------------------------------
-// Bound by HBM.  A thread takes 16 columns of a row; code x scale is rounded to fp16, which the forward kernel's operands are.
+// Bound by HBM.  A thread takes 16 columns of a row.  Codes stay codes (exact in fp16), a thread for every 16 keys hands their
+// scales to the forward kernel.  (With the values rounded to fp16 the output was 1.5 times as far from 64 bits as the split-K
+// pass's.)  Where a scale is no ordinary positive or negative number, the values are written, and their scale is 1.
+__device__ __forceinline__ bool paged_scale_apart(float scale) {
+  const float a = fabsf(scale);
+  return a >= 0x1p-40f && a <= 0x1p40f;
+}
 template <class T>
 __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGatherParams p) {
   const PagedCache& c = p.c;
@@ -904,6 +910,7 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
   const int col = static_cast<int>(task % pieces) * 16;
   if (pos >= n) return;
   uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  float k_scale = 1.f, v_scale = 1.f;  // that the forward kernel applies
   if (pos >= in_pages) {
     const RowStrides& s = is_v ? c.v_tail_strides : c.k_tail_strides;
     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(is_v ? c.v_tail : c.k_tail) + b * s.batch +
@@ -917,7 +924,11 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
       const int64_t at = page * s.batch + h * s.head + (pos & ((1 << c.page_shift) - 1)) * s.row + col;
       if constexpr (Elem<T>::kScaled) {
         const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(is_v ? c.v_pages : c.k_pages) + at);
-        const float scale = (is_v ? c.v_scales : c.k_scales)[static_cast<int64_t>(page) * c.heads_kv + h];
+        const float scales[2] = {__ldg(c.k_scales + static_cast<int64_t>(page) * c.heads_kv + h),
+                                 __ldg(c.v_scales + static_cast<int64_t>(page) * c.heads_kv + h)};
+        if (paged_scale_apart(scales[0])) k_scale = fabsf(scales[0]);
+        if (paged_scale_apart(scales[1])) v_scale = fabsf(scales[1]);
+        const float scale = paged_scale_apart(scales[is_v]) ? copysignf(1.f, scales[is_v]) : scales[is_v];
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         uint32_t y[8];
 #pragma unroll
@@ -939,6 +950,13 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
     } else if (col == 0 && p.status) {
       atomicCAS(p.status, 0, kDevNoPage);
     }
+  }
+  if (Elem<T>::kScaled && !is_v && col == 0 && (pos & (kPagedBoxRows - 1)) == 0) {
+    float4* to = p.scales_out + (static_cast<int64_t>(e) * p.heads + hh) * p.key_blocks + pos / kPagedBoxRows;
+    // (a product of extremes stays a number that neither infinities nor zeros turn into a NaN)
+    to[0] = make_float4(fminf(fmaxf(k_scale * p.scale_log2, 0x1p-126f), 0x1p100f), log2f(v_scale), 1.f / v_scale, 0.f);
+    if (pos + kPagedBoxRows >= n)  // the rest of the last tile's 128 keys
+      for (int64_t i = 1; ((pos / kPagedBoxRows + i) & 7) != 0; ++i) to[i] = make_float4(p.scale_log2, 0.f, 1.f, 0.f);
   }
   const int64_t capacity = paged_capacity(c);
   __half* dst =

@@ -100,16 +100,16 @@ class Cache:
             x = x if layout == "bshd" else x.transpose(1, 2)
             assert torch.equal(x.cpu(), want.view(kind)), n
 
-    def dense(self, entry, n, as_half):
-        """The rows of an entry as its cache holds them, [n,Hkv,d] in 64 bits; as_half: 8-bit values rounded to fp16."""
+    def dense(self, entry, n):
+        """The rows of an entry as its cache holds them, [n,Hkv,d] in 64 bits."""
         out = []
         for name in ("k", "v"):
             rows = self.rows[name][entry].double().clone()
             if self.dtype != torch.float16:
                 for i in range(n // self.page):
                     at = int(self.table[entry, i])
-                    x = self.tensors[name + "_pages"][at].float().double() * self.tensors[name + "_scales"][at].double()[None, :, None]
-                    rows[i * self.page:(i + 1) * self.page] = x.half().double() if as_half else x
+                    scales = self.tensors[name + "_scales"][at].double()[None, :, None]
+                    rows[i * self.page:(i + 1) * self.page] = self.tensors[name + "_pages"][at].float().double() * scales
             out.append(rows[:n])
         return out
 

@@ -138,7 +138,7 @@ def test_attention_over_pages(ext, fal, dtype, hq, hkv, d, page, layout, rows, l
     o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens),
                                           cache_layout=layout, **cache.on_gpu(layout)).cpu()
     for e, n in enumerate(lens):
-        k, v = cache.dense(e, max(n, 0), as_half=rows > 24)
+        k, v = cache.dense(e, max(n, 0))
         want, mag = attention(q[e], k, v, scale)
         assert_close(o[e], want, mag, n, v.abs().max().item() if n > 0 else 0.0)
         first = max(rows - max(n, 0), 0)
@@ -158,7 +158,7 @@ def test_many_entries(ext, fal, dtype, batch, rows):
     q = _rows(gen, batch, rows, hq, d)
     o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens), **cache.on_gpu("bshd")).cpu()
     for e, n in enumerate(lens):
-        k, v = cache.dense(e, max(n, 0), as_half=False)
+        k, v = cache.dense(e, max(n, 0))
         want, mag = attention(q[e], k, v, 1 / math.sqrt(d))
         assert_close(o[e], want, mag, n, v.abs().max().item() if n > 0 else 0.0)
     assert ext.device_status() == 0
@@ -177,7 +177,7 @@ def test_long_entries_and_every_number_of_rows(ext, fal, dtype, hq, hkv, d, rows
     o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens), softmax_scale=0.3,
                                           **cache.on_gpu("bshd")).cpu()
     for e, n in enumerate(lens):
-        k, v = cache.dense(e, n, as_half=False)
+        k, v = cache.dense(e, n)
         want, mag = attention(q[e], k, v, 0.3)
         assert_close(o[e], want, mag, n, v.abs().max().item())
     assert ext.device_status() == 0
@@ -199,9 +199,37 @@ def test_scores_of_every_size_and_order(fal):
                 q[..., 0] = 8
                 o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens([n]), softmax_scale=1.0,
                                                       **cache.on_gpu("bshd")).cpu()
-                kd, vd = cache.dense(0, n, as_half=False)
+                kd, vd = cache.dense(0, n)
                 want, mag = attention(q[0], kd, vd, 1.0)
                 assert_close(o[0], want, mag, n, vd.abs().max().item())
+
+
+# Pages whose values differ by many powers of two, pages of zeros, of the smallest fp16 numbers and of the largest; each query sees
+# another part of them, and is off by no more than the largest value that it sees allows.
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 7, 24, 25, 130, 400])
+@pytest.mark.parametrize("hq,hkv,d,page", [(4, 2, 128, 16), (2, 2, 64, 32), (2, 1, 256, 16), (3, 1, 96, 64)])
+def test_pages_of_every_size_of_values(ext, fal, dtype, rows, hq, hkv, d, page):
+    gen = torch.Generator().manual_seed(rows + d)
+    n = 411
+    cache = Cache(gen, DTYPES[dtype], n // page + 3, page, hkv, d, 1, n // page + 1)
+    cache.reserve(0, n)
+    pages = n // page + 1
+
+    def sizes(powers):
+        x = torch.tensor(powers)[torch.randint(0, len(powers), (pages, hkv), generator=gen)]
+        return x.repeat_interleave(page, 0)[:n, :, None]
+    k = (_rows(gen, n, hkv, d).float() * sizes([0.0, 2.0 ** -24, 2.0 ** -10, 1.0, 4.0])).half()
+    v = (_rows(gen, n, hkv, d).float() * sizes([0.0, 2.0 ** -22, 2.0 ** -14, 2.0 ** -7, 1.0, 2.0 ** 7, 2.0 ** 12])).half()
+    cache.append(0, k, v)
+    q = _rows(gen, 1, rows, hq, d)
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens([n]),
+                                          **cache.on_gpu("bshd")).cpu()
+    kd, vd = cache.dense(0, n)
+    want, mag = attention(q[0], kd, vd, 1 / math.sqrt(d))
+    seen = vd.abs().amax(dim=2).cummax(dim=0).values[n - rows:].repeat_interleave(hq // hkv, dim=1)[:, :, None]
+    assert_close(o[0], want, mag, n, seen)
+    assert ext.device_status() == 0
 
 
 def test_values_behind_the_length_do_not_matter(fal):
@@ -237,7 +265,7 @@ def test_a_run_of_steps_as_a_server_makes_them(ext, fal):
                                                   rotary_cos=cos.cuda(), rotary_sin=sin.cuda(), **got).cpu()
             for e in range(2):
                 cache.append(e, rotate(k[e, at:at + n], at, cos, sin, False), v[e, at:at + n])
-                kd, vd = cache.dense(e, at + n, as_half=n > 24)
+                kd, vd = cache.dense(e, at + n)
                 want, mag = attention(rotate(q[e, at:at + n], at, cos, sin, False), kd, vd, 1 / math.sqrt(d))
                 assert_close(o[e], want, mag, at + n, vd.abs().max().item())
             at += n
@@ -352,7 +380,7 @@ def test_a_position_without_a_page_counts_as_zeros(ext, fal, dtype, rows):
     o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=table.cuda(), **args).cpu()
     assert ext.device_status() == 3000
     for e, (n, gone) in enumerate(zip(lens, (2, 0))):
-        k, v = cache.dense(e, n, as_half=rows > 24)
+        k, v = cache.dense(e, n)
         k[gone * page:(gone + 1) * page] = 0
         v[gone * page:(gone + 1) * page] = 0
         want, mag = attention(q[e], k, v, 1 / math.sqrt(d))
