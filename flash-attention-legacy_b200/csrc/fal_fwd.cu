@@ -718,6 +718,11 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
     for (int j = kAlt ? wg : 0; j < nt; j += kAlt ? 2 : 1) {
       const int par = kAlt ? (j >> 1) & 1 : j & 1;
+      float2 scales[8];  // (SCALED: fetched while the scores are still being made)
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) scales[b] = __ldg(reinterpret_cast<const float2*>(key_scales + j * 8 + b));
+      }
       mbar_wait(bar(iSReady + wg), par, wctx, kBarSReady + wg);
       tc_fence_after_sync();
       const int kv0 = j * kTileN;
@@ -761,10 +766,7 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           }
         if constexpr (SCALED) {
 #pragma unroll
-          for (int b = 0; b < 8; ++b) {
-            const float4 x = __ldg(key_scales + j * 8 + b);
-            part[b] = __fmaf_rn(part[b], x.x, x.y);
-          }
+          for (int b = 0; b < 8; ++b) part[b] = __fmaf_rn(part[b], scales[b].x, scales[b].y);
         }
         mx = fmaxf(fmax3(part[0], part[1], part[2]), fmax3(part[3], part[4], part[5]));
         mx = fmax3(mx, part[6], part[7]);
@@ -833,10 +835,11 @@ fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         for (int i = 0; i < 32; i += 4) {
           if constexpr (SCALED) {
             if (i % 16 == 0) {
-              const float4 x = __ldg(key_scales + j * 8 + c * 2 + i / 16);
-              c2p = pack_f32x2(x.x, x.x);
-              moffp = pack_f32x2(x.y - moff, x.y - moff);
-              inv_v = pack_f32x2(x.z, x.z);
+              const int b = c * 2 + i / 16;
+              const float from = scales[b].y - moff, v = __ldg(&key_scales[j * 8 + b].z);
+              c2p = pack_f32x2(scales[b].x, scales[b].x);
+              moffp = pack_f32x2(from, from);
+              inv_v = pack_f32x2(v, v);
             }
           }
           const uint64_t x01 = ffma2(pack_f32x2(__uint_as_float(sr[c][i + 0]), __uint_as_float(sr[c][i + 1])),
