@@ -1177,10 +1177,10 @@ int make_paged_map(CUtensorMap* map, const void* base, const fal_paged_cache& c,
 
 // Query tokens up to which the split-K pass takes a call, 8 to 32 (token, head) rows to a CTA that streams the keys for itself.
 // The forward kernel takes as long for one token as for 128, per query head, behind a pass that puts the pages in order.  us,
-// this / that: 8 entries of 6 000 int8 positions, 32 / 8 heads of 128, 17 tokens 115 / 201, 24 129 / 201, 32 171 / 202, 48 244 /
-// 202; one such entry, 17 21.7 / 28.0, 32 35.2 / 28.7; 16 x 1 000, 16 / 16 of 64, 16 34 / 41, 24 44 / 41, 32 53 / 43; 32 x 500 fp16,
-// 8 / 8 of 256, 16 48 / 85, 24 76 / 86; 8 x 6 000 int8, 16 / 16 of 128, 24 91 / 188.
-constexpr int kPagedFewTokens = 24;
+// this / that: 8 entries of 6 000 int8 positions, 32 / 8 heads of 128, 25 tokens 163 / 225, 32 165 / 226, 40 194 / 226, 48 231 /
+// 226, fp16 32 148 / 205, 48 206 / 205; one such entry, 32 27.5 / 29.9, 40 45 / 30; 16 x 1 000, 16 / 16 of 64, 32 46 / 50, 40 59 /
+// 50; 32 x 500 fp16, 8 / 8 of 256, 32 84 / 87, 40 115 / 87; 8 x 6 000 int8, 16 / 16 of 128, 48 125 / 207.
+constexpr int kPagedFewTokens = 32;
 constexpr int64_t kPagedGatherBytes = int64_t{1} << 30;
 
 constexpr int64_t kPagedUnknownSlots = 148 * 24;  // without a GPU to ask
