@@ -23,9 +23,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // page) into a ring of its own.  Fragments are read from shared memory as the lanes' own 16 bytes, without ldmatrix: a
 // contraction may take its terms in any order, so lane t of four takes 16 bytes of a key row that are next to each other,
 // and Q is laid out to match; lane g of eight takes 16 neighbouring bytes of a V row.
-// 8-bit codes become fp16 in registers (exact), the scales enter in 32 bits: K's with the softmax scale, V's where the
-// product of a 16-key slice is added to the output.  P^T of the scores' layout becomes the second product's operand by
-// movmatrix; its column sums, one more product with ones, are the softmax sum.
+// 8-bit codes become fp16 in registers (exact).  The scales enter in 32 bits: K's multiplies the scores, V's is part of the
+// weights, P = 2^(s + log2 v - m) with m near the largest such exponent, so that P keeps its bits however the scales differ; the
+// softmax sum adds P / v, in 32 bits.  P^T of the scores' layout becomes the second product's operand by movmatrix.
 //
 // An (entry, KV head, chunk of 8 NT query rows) is a unit; its keys count in steps, one 16-key slice for each of four warps, or
 // two.  Entries are cut into parts of one length that the GPU works out from all lengths, so that all units together
@@ -239,7 +239,7 @@ struct PagedState {
   uint32_t p[H][NT][2];  // the weights of the slices in hand, as the second product's operand
   float o[NT][D / 16][4];
   float m[NT][2];     // reference of the exponents, log2 domain: at most 8 below the largest score so far; kNoKey before the first
-  float l[NT][2];     // sums of the weights
+  float l[NT][2];     // this lane's keys' share of the softmax sums
   float c2;
   int min_limit;     // first key that some query row does not see
 };
@@ -249,14 +249,18 @@ struct PagedState {
 // entry's first token does not see.
 template <int H, int D, int NT, int HS>
 __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
-                                              const float (&k_scale)[H], int first_limit, int row0, int group) {
+                                              const float (&k_scale)[H], const float (&v_log)[H], int first_limit, int row0,
+                                              int group) {
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     const float f = st.c2 * k_scale[h];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[h][nt][e] *= f;
+      for (int e = 0; e < 4; e += 2) {
+        const uint64_t y = ffma2(pack_f32x2(s[h][nt][e], s[h][nt][e + 1]), pack_f32x2(f, f), pack_f32x2(v_log[h], v_log[h]));
+        unpack_f32x2(y, s[h][nt][e], s[h][nt][e + 1]);
+      }
   }
   if (key0 + H * kPagedSlice > min(st.min_limit, end)) {
 #pragma unroll
@@ -308,21 +312,21 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
     }
   }
 #pragma unroll
-  for (int h = 0; h < H; ++h)
+  for (int h = 0; h < H; ++h) {
+    const float inv = fast_exp2(fmaxf(-v_log[h], -126.f));  // 1 / v (of a NaN: any number)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[h][nt][e] = fast_exp2(s[h][nt][e] - st.m[nt][e & 1]);
+      const uint64_t m = pack_f32x2(-st.m[nt][0], -st.m[nt][1]);
+      const uint64_t p0 = exp2_pair(fadd2(pack_f32x2(s[h][nt][0], s[h][nt][1]), m));
+      const uint64_t p1 = exp2_pair(fadd2(pack_f32x2(s[h][nt][2], s[h][nt][3]), m));
+      unpack_f32x2(p0, s[h][nt][0], s[h][nt][1]);
+      unpack_f32x2(p1, s[h][nt][2], s[h][nt][3]);
       st.p[h][nt][0] = movmatrix(pack_half2(s[h][nt][0], s[h][nt][1]));
       st.p[h][nt][1] = movmatrix(pack_half2(s[h][nt][2], s[h][nt][3]));
-      // sums of the weights as they are rounded, which is what the output is divided by
-      const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-      float sum[4];
-      mma_16816_from(sum, ones, st.p[h][nt][0], st.p[h][nt][1], zero);
-      st.l[nt][0] += sum[0];
-      st.l[nt][1] += sum[1];
+      const uint64_t l = ffma2(fadd2(p0, p1), pack_f32x2(inv, inv), pack_f32x2(st.l[nt][0], st.l[nt][1]));
+      unpack_f32x2(l, st.l[nt][0], st.l[nt][1]);
     }
+  }
 }
 
 // s (+)= the product of 16 keys' columns of one step and Q's.
@@ -376,25 +380,11 @@ __device__ __forceinline__ void paged_scores(PagedState<D, NT, H>& st, float (&s
 
 // O^T += V^T P^T of the h-th slice, of a page; vb: its shared address + v_read.
 template <class T, int D, int NT, int H>
-__device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, uint32_t vb, float v_scale) {
+__device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, uint32_t vb) {
   using Tile = PagedTile<D, T>;
   auto product = [&](int j, const uint32_t (&a)[4]) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      if constexpr (Elem<T>::kScaled) {
-        float x[4];
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_16816_from(x, a, st.p[h][nt][0], st.p[h][nt][1], zero);
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const uint64_t y = ffma2(pack_f32x2(x[e], x[e + 1]), pack_f32x2(v_scale, v_scale),
-                                   pack_f32x2(st.o[nt][j][e], st.o[nt][j][e + 1]));
-          unpack_f32x2(y, st.o[nt][j][e], st.o[nt][j][e + 1]);
-        }
-      } else {
-        mma_16816_add(st.o[nt][j], a, st.p[h][nt][0], st.p[h][nt][1]);
-      }
-    }
+    for (int nt = 0; nt < NT; ++nt) mma_16816_add(st.o[nt][j], a, st.p[h][nt][0], st.p[h][nt][1]);
   };
 #pragma unroll
   for (int block = 0; block < Tile::kBlocks; ++block) {
@@ -446,8 +436,8 @@ __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint
       paged_score_step(st, s[0], a, seg * 4 + k);
     }
   }
-  const float scale[1] = {1.f};
-  paged_weights<1>(st, s, key0, key0 + g, end, scale, first_limit, row0, group);
+  const float k_scale[1] = {1.f}, v_log[1] = {0.f};
+  paged_weights<1>(st, s, key0, key0 + g, end, k_scale, v_log, first_limit, row0, group);
 }
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint32_t base) {
@@ -518,10 +508,12 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
   };
   auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages); };
   auto scale_of = [&](const float* scales, int page) {
-    return kScaled && there(page) ? __ldg(scales + static_cast<int64_t>(page) * c.heads_kv + kv_head) : 0.f;
+    return kScaled && there(page) ? __ldg(scales + static_cast<int64_t>(page) * c.heads_kv + kv_head) : 1.f;
   };
+  // log2 of V's scale; of 0, which a page of zeros has, of a number that is as good
+  auto v_log_of = [&](int page) { return kScaled ? __log2f(scale_of(c.v_scales, page) + 0x1p-100f) : 0.f; };
   int pages = pages_of(0), next_pages = 0;
-  float k_scales = 0.f, v_scales = 0.f, next_k = 0.f, next_v = 0.f, last_k = 0.f, last_v = 0.f;
+  float k_scales = 0.f, v_logs = 0.f, next_k = 0.f, next_v = 0.f, last_k = 0.f, last_v = 0.f;
   uint32_t fill = 0;  // stage that the next loads go to
   auto issue = [&](int i) {
     if (i < turns) {
@@ -529,14 +521,14 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       if (in_batch == 0 && i > 0) {
         pages = next_pages;
         last_k = k_scales;
-        last_v = v_scales;
+        last_v = v_logs;
         k_scales = next_k;
-        v_scales = next_v;
+        v_logs = next_v;
       }
       if (in_batch == kBatch / 8) next_pages = pages_of((i & ~(kBatch - 1)) + kBatch);
       if (kScaled && in_batch == kBatch * 5 / 8) {
         next_k = scale_of(c.k_scales, next_pages);
-        next_v = scale_of(c.v_scales, next_pages);
+        next_v = v_log_of(next_pages);
       }
       int page[kH];
 #pragma unroll
@@ -584,7 +576,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) issue(i);
   k_scales = scale_of(c.k_scales, pages);
-  v_scales = scale_of(c.v_scales, pages);
+  v_logs = v_log_of(pages);
 
   // ---- queries and their limits, under the first loads ----
   auto query = [&](int nt, int ks) {
@@ -633,14 +625,15 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     issue(i + kAhead);
     const uint32_t stage = ring.base + drain * L::kStageBytes;
     const int key0 = first + i * kStep;
-    float k_scale[kH], v_scale[kH];
+    float k_scale[kH], v_log[kH];
     const bool before = (min(i + kAhead, turns - 1) ^ i) >= kBatch;
 #pragma unroll
     for (int h = 0; h < kH; ++h) {
-      k_scale[h] = v_scale[h] = 1.f;
+      k_scale[h] = 1.f;
+      v_log[h] = 0.f;
       if constexpr (kScaled) {
         k_scale[h] = __shfl_sync(0xffffffffu, before ? last_k : k_scales, i * kH + h);
-        v_scale[h] = __shfl_sync(0xffffffffu, before ? last_v : v_scales, i * kH + h);
+        v_log[h] = __shfl_sync(0xffffffffu, before ? last_v : v_logs, i * kH + h);
       }
     }
     mbar_wait(ring.barriers + drain * 8, (ring.phases >> drain) & 1u, ring.wait, kPagedBarrierId);
@@ -659,9 +652,9 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     float s[kH][NT][4];
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_scores<T>(st, s[h], stage + k_read + h * Tile::kSliceBytes);
-    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, first_limit, row0, group);
+    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, v_log, first_limit, row0, group);
 #pragma unroll
-    for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes, v_scale[h]);
+    for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes);
     drain = drain + 1 < L::kStages ? drain + 1 : 0;
     __syncwarp();  // all lanes are done with this stage before it is refilled
   }
@@ -677,6 +670,13 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       __syncwarp();
     }
   }
+  // the lanes' shares of the sums
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) st.l[nt][e] += __shfl_xor_sync(0xffffffffu, st.l[nt][e], off);
 }
 
 // What a pair of columns is exclusive-or'ed with where the warps' results lie: a number of its lane, below the pairs of a lane.
