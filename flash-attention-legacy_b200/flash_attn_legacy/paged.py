@@ -10,7 +10,7 @@ A cache is a set of tensors:
     block_table       int32 [B, pages per entry]: position p of entry b is row p % page of page block_table[b, p // page]
     cache_seqlens     int32 [B]: positions that an entry holds; negative: an unused entry of a padded batch
     and for 8-bit pages
-    k_scales, v_scales  float32 [num_pages, Hkv]: a value is code * scale
+    k_scales, v_scales  float32 [num_pages, Hkv], not negative: a value is code * scale
     k_tail, v_tail    float16 [B, page, Hkv, d] (or [B, Hkv, page, d]): the rows of an entry's last, unfinished page
 
 An 8-bit page is written when its last row arrives, from fp16 rows and with the largest magnitude of each head as its

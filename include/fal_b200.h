@@ -369,7 +369,7 @@ FAL_API int fal_cache_append(const void* k_new, const void* v_new, void* k_cache
  * block_table[b, p / page_size]; an entry holds cache_seqlens[b] positions of pages_per_entry * page_size at most.
  *   dtype FAL_PAGED_F16: pages of fp16 rows.
  *   dtype FAL_PAGED_S8 / FAL_PAGED_E4M3: pages of 8-bit codes, each page and KV head with a scale of its own,
- *   k_scales / v_scales [num_pages, heads_kv] fp32: value = code * scale.  A page is written when it is full:
+ *   k_scales / v_scales [num_pages, heads_kv] fp32, not negative: value = code * scale.  A page is written when it is full:
  *   scale = a / m with the largest magnitude a of its rows of the head, m = 127 / 448, code = x m / a rounded to the
  *   nearest whole number / e4m3 number, ties to even (scale NaN if the page holds an infinity or a NaN).  The rows of an
  *   entry's last, unfinished page are fp16 rows of its tail: position p is row p % page_size of k_tail / v_tail [b].
