@@ -5,10 +5,9 @@
 // 8-bit pages.  A value is rounded to 8 bits once, when its page is full: a = max |x| over the page's rows of a head,
 // scale = a / m and code = round(x m / a), m = 127 (int8, nearest whole number) or 448 (e4m3, nearest such number).  Until
 // then the row waits as fp16 in the entry's tail, so that the cache does not depend on how the rows came in, token by
-// token or as chunks, and no page is rounded again when a larger value arrives.  x m is exact in 32 bits (11 + 7 bits), and
-// its quotient by a within a unit of the last place is on the same side of every rounding border as the exact one, which is on
-// the border or at least 2^-19 of itself away: a border is a number of 8 bits at most, a one of 11, and the difference of the
-// products a whole number.
+// token or as chunks, and no page is rounded again when a larger value arrives.  The codes are those of the exact quotients: one
+// is on a rounding border or at least 2^-19 of itself away, because a border is a number of 8 bits at most, a one of 11, and
+// the difference of x m and border x a a whole number in the units of both.
 #include <algorithm>
 #include <type_traits>
 
@@ -184,24 +183,22 @@ __device__ __forceinline__ void append_token(const PagedAppendParams& p, int tok
   }
 }
 
-// x / a from r, about 1 / a: one step of Newton's method, whose residual is exact in a fused multiply-add.  Within a unit of the
-// last place, and exact where the quotient is a number of 24 bits -- a rounding border of the codes --, which is all that
-// their rounding needs.
-__device__ __forceinline__ float quotient(float x, float a, float r) {
-  const float y = x * r;
-  return y == 0.f ? y : __fmaf_rn(__fmaf_rn(-y, a, x), r, y);  // (a zero keeps its sign)
+// x m / a, near enough for its rounding to a code: x's product with c = m / a is within 2^-22.9 of itself of the quotient.
+// Rounded to 21 bits it is a border of the codes where the quotient is one, and on the quotient's side of every border
+// elsewhere, 2^-20.5 against 2^-19.  (A zero keeps its sign.)
+__device__ __forceinline__ float quotient(float x, float c) {
+  return __uint_as_float((__float_as_uint(__fmul_rn(x, c)) + 4u) & ~7u);
 }
-// The codes of two fp16 values as two bytes; most: the page's largest magnitude, not 0; r: 1 / most.
-__device__ __forceinline__ uint32_t codes_of(const S8*, float2 x, float most, float r) {
-  const int lo = __float2int_rn(quotient(x.x * 127.f, most, r)), hi = __float2int_rn(quotient(x.y * 127.f, most, r));
-  return (lo & 0xff) | ((hi & 0xff) << 8);
+// The codes of four fp16 values as four bytes.  A sum with 1.5 x 2^23 is rounded to a whole number, in the lowest bits.
+__device__ __forceinline__ uint32_t codes_of(const S8*, float2 x, float2 z, float c) {
+  auto whole = [&](float y) { return __float_as_uint(__fadd_rn(quotient(y, c), 12582912.f)); };
+  return __byte_perm(__byte_perm(whole(x.x), whole(x.y), 0x0040), __byte_perm(whole(z.x), whole(z.y), 0x0040), 0x5410);
 }
-__device__ __forceinline__ uint32_t codes_of(const E4M3*, float2 x, float most, float r) {
-  uint16_t out;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-      : "=h"(out)
-      : "f"(quotient(x.y * 448.f, most, r)), "f"(quotient(x.x * 448.f, most, r)));
-  return out;
+__device__ __forceinline__ uint32_t codes_of(const E4M3*, float2 x, float2 z, float c) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(quotient(x.y, c)), "f"(quotient(x.x, c)));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(quotient(z.y, c)), "f"(quotient(z.x, c)));
+  return lo | static_cast<uint32_t>(hi) << 16;
 }
 __device__ __forceinline__ float code_max(const S8*) { return 127.f; }
 __device__ __forceinline__ float code_max(const E4M3*) { return 448.f; }
@@ -275,7 +272,7 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
   const float largest = __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
   const bool finite = most < 0x7c00u;
   const bool some = finite && most != 0;
-  const float inverse = some ? __fdiv_rn(1.f, largest) : 0.f;
+  const float per_value = some ? __fdiv_rn(code_max(static_cast<const T*>(nullptr)), largest) : 0.f;
 
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.num_pages)) {
     if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kDevAppendOverflow);
@@ -287,8 +284,8 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
       if (some) {
         const __half2* y = reinterpret_cast<const __half2*>(&x);
         const T* type = nullptr;
-        w.x = codes_of(type, __half22float2(y[0]), largest, inverse) | codes_of(type, __half22float2(y[1]), largest, inverse) << 16;
-        w.y = codes_of(type, __half22float2(y[2]), largest, inverse) | codes_of(type, __half22float2(y[3]), largest, inverse) << 16;
+        w.x = codes_of(type, __half22float2(y[0]), __half22float2(y[1]), per_value);
+        w.y = codes_of(type, __half22float2(y[2]), __half22float2(y[3]), per_value);
       }
       return w;
     };
