@@ -25,6 +25,17 @@ constexpr int kAppendThreads = 256;
 template <class T>
 constexpr int kAppendBlocks = std::is_same<T, __half>::value ? 5 : 4;
 
+// How a launch is laid out: a grid row per entry, first its page blocks, then its token blocks.
+struct AppendGrid {
+  unsigned page_blocks;   // of an entry
+  unsigned head_groups;   // page blocks of a page
+  int head_threads_log2;  // of a page block, to a head
+  unsigned per_piece;     // 65 536 / pieces of a row, rounded up
+};
+// x / pieces of a row, for x < 65 536 / 6: a multiplication, because divisions were a third of the instructions of a kernel that
+// the integer pipe bounded (13 x 1 027 tokens of 24 / 8 heads of 128, int8, 69.7 us, without them 63.4).
+__device__ __forceinline__ int over_pieces(const AppendGrid& g, int x) { return static_cast<int>(x * g.per_piece >> 16); }
+
 struct Piece {
   int first, second;  // columns of the two pieces
   bool rotated;
@@ -118,13 +129,11 @@ __device__ __forceinline__ const __half* new_row(const void* base, const RowStri
 // Rows of 8-bit caches that finish a page are the page blocks' business, and so are those behind such a page: their places in
 // the tail are read there first.
 constexpr int kTokenThreads = kAppendThreads / 2;
-__device__ __forceinline__ void append_token(const PagedAppendParams& p, int token, int thread) {
-  const int b = token / p.rows;
-  const int i = token % p.rows;
+__device__ __forceinline__ void append_token(const PagedAppendParams& p, const AppendGrid& grid, int b, int i, int thread) {
   const int start = p.c.lens[b];
   const int capacity = paged_capacity(p.c);
   const int pieces = p.c.head_dim / 16;
-  const int lanes = kTokenThreads / pieces, lane = thread / pieces, c = thread % pieces;
+  const int lanes = over_pieces(grid, kTokenThreads), lane = over_pieces(grid, thread), c = thread - lane * pieces;
   const int64_t pos64 = static_cast<int64_t>(start) + i;
   const bool placed = start >= 0 && pos64 < capacity;  // (start < 0: an unused entry of a padded batch)
   const int pos = placed ? static_cast<int>(pos64) : 0;
@@ -175,7 +184,7 @@ __device__ __forceinline__ void append_token(const PagedAppendParams& p, int tok
     const Piece& at = hv < 0 ? turned : plain;
     uint4 a = *reinterpret_cast<const uint4*>(src + at.first), z = *reinterpret_cast<const uint4*>(src + at.second);
     if (at.rotated) append_turn(p, angles, a, z);
-    __half* dst = hk < 0 ? static_cast<__half*>(p.q_out) + (static_cast<int64_t>(token) * p.heads_q + h) * p.c.head_dim
+    __half* dst = hk < 0 ? static_cast<__half*>(p.q_out) + ((static_cast<int64_t>(b) * p.rows + i) * p.heads_q + h) * p.c.head_dim
                          : hv < 0 ? k_to + hk * k_head : v_to + hv * v_head;
     if (!placed) a = z = make_uint4(0, 0, 0, 0);  // (a query without a position)
     *reinterpret_cast<uint4*>(dst + at.first) = a;
@@ -210,7 +219,9 @@ __device__ __forceinline__ float code_max(const E4M3*) { return 448.f; }
 // (256 threads to a head: 4 x 2 987 tokens, pages of 16 x 128, 104 us against 80.)
 constexpr int kSealKept = 2;
 template <class T>
-__device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, int b, int first_head, int index_from, int threads) {
+__device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, const AppendGrid& grid, int b, int first_head,
+                                                  int index_from) {
+  const int threads = 1 << grid.head_threads_log2;
   __shared__ uint32_t warp_most[kAppendThreads / 32];
   const int start = p.c.lens[b];
   const int capacity = paged_capacity(p.c);
@@ -219,9 +230,10 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
   const int end = static_cast<int>(min(static_cast<int64_t>(start) + p.rows, static_cast<int64_t>(capacity)));
   const int index = (start >> shift) + index_from;  // page of the entry
   if (index >= (end >> shift)) return;              // not full
-  const int head = min(first_head + static_cast<int>(threadIdx.x) / threads, 2 * p.c.heads_kv - 1);
-  const bool active = first_head + static_cast<int>(threadIdx.x) / threads == head;
-  const int thread = threadIdx.x % threads;
+  const int wanted = first_head + static_cast<int>(threadIdx.x >> grid.head_threads_log2);
+  const int head = min(wanted, 2 * p.c.heads_kv - 1);
+  const bool active = wanted == head;
+  const int thread = threadIdx.x & (threads - 1);
   const int page = p.c.table[b * p.c.table_stride + index];
   const bool is_v = head >= p.c.heads_kv;
   const int h = is_v ? head - p.c.heads_kv : head;
@@ -231,7 +243,7 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
   const void* src = is_v ? p.v : p.k;
   const RowStrides& ss = is_v ? p.v_new_strides : p.k_new_strides;
   auto load = [&](int task, uint4& a, uint4& z, Piece& at) {
-    const int r = task / pieces, c = task % pieces;
+    const int r = over_pieces(grid, task), c = task - r * pieces;
     const int pos = (index << shift) + r;
     if (pos < start) {
       // (in the pieces that the rotation of a new row takes together, so that one place holds one piece)
@@ -290,7 +302,7 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
       return w;
     };
     auto store = [&](int task, const uint4& a, const uint4& z) {
-      const int r = task / pieces, c = task % pieces;
+      const int r = over_pieces(grid, task), c = task - r * pieces;
       Piece to = append_piece(p, c);
       if (is_v) to = Piece{c * 16, c * 16 + 8, false};
       *reinterpret_cast<uint2*>(out + r * s.row + to.first) = codes(a);
@@ -318,7 +330,7 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
   const int left = active ? end & (page_rows - 1) : 0;  // rows behind the last full page
   const int first = end & ~(page_rows - 1);
   for (int task = thread; task < left * pieces; task += threads) {
-    const int r = task / pieces, c = task % pieces;
+    const int r = over_pieces(grid, task), c = task - r * pieces;
     uint4 x, z;
     append_load(p, new_row(src, ss, b, h, first + r - start), c, !is_v, first + r, x, z, at);
     *reinterpret_cast<uint4*>(tail + r * ts.row + at.first) = x;
@@ -326,40 +338,42 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, in
   }
 }
 
-// One launch: first the page blocks (8-bit caches: heads of K and of V, then page, then entry), then the token blocks.
 template <class T>
 __global__ void __launch_bounds__(kAppendThreads, kAppendBlocks<T>)
-fal_paged_append_kernel(const PagedAppendParams p, unsigned page_blocks, unsigned pages, unsigned head_threads, unsigned tokens) {
+fal_paged_append_kernel(const PagedAppendParams p, const AppendGrid grid) {
   grid_dependency_wait();
   grid_dependency_launch();
+  const int b = blockIdx.y;
   if constexpr (!std::is_same<T, __half>::value) {
-    if (blockIdx.x < page_blocks) {
-      const unsigned at_once = kAppendThreads / head_threads, groups = (2 * p.c.heads_kv + at_once - 1) / at_once;
-      const unsigned which = blockIdx.x / groups;
-      append_page_codes<T>(p, which / pages, blockIdx.x % groups * at_once, which % pages, head_threads);
+    if (blockIdx.x < grid.page_blocks) {  // (page, then heads of K and of V)
+      const unsigned page = blockIdx.x / grid.head_groups, heads = blockIdx.x - page * grid.head_groups;
+      append_page_codes<T>(p, grid, b, static_cast<int>(heads * (kAppendThreads >> grid.head_threads_log2)), static_cast<int>(page));
       return;
     }
   }
-  const unsigned token = (blockIdx.x - page_blocks) * 2 + threadIdx.x / kTokenThreads;
-  if (token < tokens) append_token(p, token, threadIdx.x % kTokenThreads);
+  const unsigned i = (blockIdx.x - grid.page_blocks) * 2 + threadIdx.x / kTokenThreads;
+  if (i < static_cast<unsigned>(p.rows)) append_token(p, grid, b, static_cast<int>(i), threadIdx.x % kTokenThreads);
 }
 
 template <class T>
 cudaError_t append_t(const PagedAppendParams& p, cudaStream_t stream) {
-  const int64_t tokens = static_cast<int64_t>(p.c.batch) * p.rows;
   // pages that one entry can finish
   const int64_t pages = std::is_same<T, __half>::value ? 0 : (p.rows + (int64_t{1} << p.c.page_shift) - 1) >> p.c.page_shift;
+  const int pieces = p.c.head_dim / 16;
+  AppendGrid grid{};
   // threads to a head: kSealKept pieces each where that fills warps
-  int64_t head_threads = 32;
-  while (head_threads < kAppendThreads && head_threads * kSealKept < (int64_t{p.c.head_dim / 16} << p.c.page_shift))
-    head_threads *= 2;
-  const int64_t at_once = kAppendThreads / head_threads;
-  const int64_t page_blocks = pages * ((2 * p.c.heads_kv + at_once - 1) / at_once) * p.c.batch;
-  const int64_t blocks = page_blocks + (tokens + 1) / 2;
-  if (tokens > 0x7fffffff || blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_dependent(fal_paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream, p,
-                          static_cast<unsigned>(page_blocks), static_cast<unsigned>(pages), static_cast<unsigned>(head_threads),
-                          static_cast<unsigned>(tokens));
+  grid.head_threads_log2 = 5;
+  while (1 << grid.head_threads_log2 < kAppendThreads && kSealKept << grid.head_threads_log2 < pieces << p.c.page_shift)
+    ++grid.head_threads_log2;
+  const int64_t at_once = kAppendThreads >> grid.head_threads_log2;
+  grid.head_groups = static_cast<unsigned>((2 * p.c.heads_kv + at_once - 1) / at_once);
+  grid.per_piece = (65536 + pieces - 1) / pieces;
+  const int64_t page_blocks = pages * grid.head_groups;
+  const int64_t blocks = page_blocks + (static_cast<int64_t>(p.rows) + 1) / 2;
+  if (blocks > 0x7fffffff || p.c.batch > 65535) return cudaErrorInvalidValue;
+  grid.page_blocks = static_cast<unsigned>(page_blocks);
+  return launch_dependent(fal_paged_append_kernel<T>, dim3(static_cast<unsigned>(blocks), p.c.batch), dim3(kAppendThreads), 0,
+                          stream, p, grid);
 }
 
 }  // namespace
