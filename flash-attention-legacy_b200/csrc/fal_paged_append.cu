@@ -17,13 +17,13 @@ namespace fal {
 
 namespace {
 
-// Bound by HBM on prompts, by latency for single tokens.  A thread takes 16 columns of a head: the two 8-column pieces
+// Prompts are bound by HBM with fp16 pages (0.90 of a copy's rate), by the integer and floating pipes with 8-bit ones (4 x 1 024
+// tokens of 32 + 8 + 8 heads of 128, int8, 22.9 us, 4.2 TB/s); single tokens by latency.  A thread takes 16 columns of a head: the two 8-column pieces
 // whose columns are rotated with each other, or two neighbouring ones.
 constexpr int kAppendThreads = 256;
-// Blocks per SM: 48 registers a thread, 64 with 8-bit pages.  us on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, 4 / 5 / 6
-// blocks: fp16 64.6 / 60.5 / 65.5; int8, 3 / 4 / 5: 96.9 / 83.1 / 85.2.
-template <class T>
-constexpr int kAppendBlocks = std::is_same<T, __half>::value ? 5 : 4;
+// Blocks per SM: 48 registers a thread.  us with 4 / 5 / 6 blocks on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, fp16: 63.3 / 59.9
+// (5.8 TB/s) / 60.1; with 3 / 4 / 5 on the same in int8, 81.2 / 70.2 / 69.6, on 13 x 1 027 of 24 + 8 + 8, 73.1 / 63.4 / 61.4.
+constexpr int kAppendBlocks = 5;
 
 // How a launch is laid out: a grid row per entry, first its page blocks, then its token blocks.
 struct AppendGrid {
@@ -125,7 +125,7 @@ __device__ __forceinline__ const __half* new_row(const void* base, const RowStri
 }
 
 // Half a token block: one token.  A thread takes one piece of every few heads, so that it fetches its angles once (a thread for
-// every piece of a token's heads, angles and all: 4 x 1 024 tokens of 48 heads of 128, int8, 36 us, against 26).
+// every piece of a token's heads, angles and all, took 36 us where this took 26: 4 x 1 024 tokens of 48 heads of 128, int8).
 // Rows of 8-bit caches that finish a page are the page blocks' business, and so are those behind such a page: their places in
 // the tail are read there first.
 constexpr int kTokenThreads = kAppendThreads / 2;
@@ -216,7 +216,7 @@ __device__ __forceinline__ float code_max(const E4M3*) { return 448.f; }
 // A thread keeps the first kSealKept pieces that it reads (the rows before the new ones from the tail, the others from the
 // call, rotated) and reads further ones, of pages of more than 8 192 values a head, again: once for the largest magnitude, once
 // for the codes.  The first page's block also writes the rows behind the last full page to the tail, once it has read it.
-// (256 threads to a head: 4 x 2 987 tokens, pages of 16 x 128, 104 us against 80.)
+// (256 threads to a head took 104 us where this took 80: 4 x 2 987 tokens, pages of 16 x 128.)
 constexpr int kSealKept = 2;
 template <class T>
 __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, const AppendGrid& grid, int b, int first_head,
@@ -339,7 +339,7 @@ __device__ __forceinline__ void append_page_codes(const PagedAppendParams& p, co
 }
 
 template <class T>
-__global__ void __launch_bounds__(kAppendThreads, kAppendBlocks<T>)
+__global__ void __launch_bounds__(kAppendThreads, kAppendBlocks)
 fal_paged_append_kernel(const PagedAppendParams p, const AppendGrid grid) {
   grid_dependency_wait();
   grid_dependency_launch();
