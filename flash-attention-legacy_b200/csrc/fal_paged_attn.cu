@@ -508,7 +508,8 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
   };
   auto there = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.num_pages); };
   auto scale_of = [&](const float* scales, int page) {
-    return kScaled && there(page) ? __ldg(scales + static_cast<int64_t>(page) * c.heads_kv + kv_head) : 1.f;
+    // (an ordinary load: the append before may still be writing scales while this grid's blocks take their places)
+    return kScaled && there(page) ? scales[static_cast<int64_t>(page) * c.heads_kv + kv_head] : 1.f;
   };
   // log2 of V's scale; of 0, which a page of zeros has, of a number that is as good
   auto v_log_of = [&](int page) { return kScaled ? __log2f(scale_of(c.v_scales, page) + 0x1p-100f) : 0.f; };

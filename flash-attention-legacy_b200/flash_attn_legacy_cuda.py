@@ -906,6 +906,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_sca
                                      softmax_scale, 0, workspace, nbytes, _status_ptr(dev), _raw_stream(dev))
 
     nbytes = _lib.fal_paged_attn_workspace_bytes(args(0, 0))
+    if nbytes == 0:
+        raise RuntimeError("the call has too many query rows for one grid")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     if append is not None:
         q, cache_seqlens = append()
