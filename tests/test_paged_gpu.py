@@ -204,6 +204,25 @@ def test_scores_of_every_size_and_order(fal):
                 assert_close(o[0], want, mag, n, vd.abs().max().item())
 
 
+# Block tables so long that the pages of a part of the entries, or of the KV heads of one entry, are put in order at a time.
+@pytest.mark.parametrize("dtype", ["fp16", "int8"])
+@pytest.mark.parametrize("batch,hq,hkv,d,width", [(70, 4, 2, 64, 128), (2, 8, 8, 128, 2048)])
+def test_many_tokens_behind_long_block_tables(ext, fal, dtype, batch, hq, hkv, d, width):
+    gen = torch.Generator().manual_seed(width)
+    lens = [int(x) for x in torch.randint(0, 300, (batch,), generator=gen)]
+    lens[-1] = 513
+    cache = _filled(gen, DTYPES[dtype], lens, 256, hkv, d)
+    table = torch.full((batch, width), -1, dtype=torch.int32)
+    table[:, :cache.table.shape[1]] = cache.table
+    q = _rows(gen, batch, 33, hq, d)
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=table.cuda(), cache_seqlens=_lens(lens), **cache.on_gpu("bshd")).cpu()
+    for e, n in enumerate(lens):
+        k, v = cache.dense(e, n)
+        want, mag = attention(q[e], k, v, 1 / math.sqrt(d))
+        assert_close(o[e], want, mag, n, v.abs().max().item() if n > 0 else 0.0)
+    assert ext.device_status() == 0
+
+
 # Pages whose values differ by many powers of two, pages of zeros, of the smallest fp16 numbers and of the largest; each query sees
 # another part of them, and is off by no more than the largest value that it sees allows.
 @pytest.mark.parametrize("dtype", ["int8", "e4m3"])
