@@ -247,6 +247,7 @@ struct PagedAttnParams {
   int rows;              // query i sees the keys up to position len - rows + i
   int kernel_dim;        // 64, 128 or 256
   int resident;          // CTAs of the split-K kernel that run at once
+  int even_parts;        // parts of all entries that together are no more than there are places, were all of one length
   int64_t slots;         // CTAs whose results can go to the workspace
   float scale;
   int* status;

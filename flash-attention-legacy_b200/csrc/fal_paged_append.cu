@@ -18,8 +18,8 @@ namespace fal {
 namespace {
 
 // Prompts are bound by HBM with fp16 pages (0.90 of a copy's rate), by the integer and floating pipes with 8-bit ones (4 x 1 024
-// tokens of 32 + 8 + 8 heads of 128, int8, 22.9 us, 4.2 TB/s); single tokens by latency.  A thread takes 16 columns of a head: the two 8-column pieces
-// whose columns are rotated with each other, or two neighbouring ones.
+// tokens of 32 + 8 + 8 heads of 128, int8, 22.9 us, 4.2 TB/s); single tokens by latency.  A thread takes 16 columns of a head:
+// the two 8-column pieces whose columns are rotated with each other, or two neighbouring ones.
 constexpr int kAppendThreads = 256;
 // Blocks per SM: 48 registers a thread.  us with 4 / 5 / 6 blocks on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, fp16: 63.3 / 59.9
 // (5.8 TB/s) / 60.1; with 3 / 4 / 5 on the same in int8, 81.2 / 70.2 / 69.6, on 13 x 1 027 of 24 + 8 + 8, 73.1 / 63.4 / 61.4.

@@ -172,14 +172,20 @@ constexpr float kNoKey = -1e30f;  // further below any score than an exponential
 // bandwidth), but no shorter than kPagedGoodSteps, which a CTA's set-up is small beside, as long as there is a CTA for every
 // place, nor than kPagedMinKeys.  (A length that makes the CTAs fill the places a whole number of times is no better.)
 // us with 1 / 2 / 4 CTAs for every place: 64 entries of 16 000 int8 positions, 8 heads of 128, 421 / 366 / 339, fp16 623 / 604 /
-// 605, 16 fp16 - / 167 / 159.  Parts of 8 / 16 / 32 steps: 16 entries of 32 000 int8, 4 heads of 64, 60 / 56 / 53, 16 of 6 000 with
-// 5 tokens, 8 heads of 64, 57 / 49 / 53; 16 of 16 000 int8, 8 heads of 128, 99 / 104 / -, 20 of 5 000 48 / 59 / - (128 keys to a step);
-// with 16 heads to a KV head 57 / 52 / -, 12 of 2 000 fp16 with 5 tokens 39 / 31 / -, 8 of 6 000 int8 45 / 49 / 49, 30 000 38 / 29 / -;
-// 16 of 5 000 e4m3, 16 heads of 256, 119 / 119 / 110.
+// 605, 16 fp16 - / 167 / 159.  Parts of 8 / 16 / 32 steps: 16 entries of 32 000 int8, 4 heads of 64, 60 / 56 / 53, 16 of 6 000
+// with 5 tokens, 8 heads of 64, 57 / 49 / 53; 16 of 16 000 int8, 8 heads of 128, 99 / 104 / -, 20 of 5 000 48 / 59 / - (128 keys
+// to a step); with 16 heads to a KV head 57 / 52 / -, 12 of 2 000 fp16 with 5 tokens 39 / 31 / -, one of 30 000 int8
+// 38 / 29 / -; 16 of 5 000 e4m3, 16 heads of 256, 119 / 119 / 110.
 constexpr int kPagedMinKeys = 256;
 constexpr int kPagedWaves = 4;
 template <int D, int STEP>
 constexpr int kPagedGoodSteps = D == 256 ? 32 : D == 128 && STEP > 64 ? 8 : 16;
+
+// Where that length would give every place one CTA, a few more CTAs than places, from parts that are not of full length, would
+// take the GPU twice: then the parts are a quarter to a half longer, if those fit.  us without / with that: 8 entries of 6 000
+// int8, 5 tokens, 8 heads of 128, 48.4 / 37.4, of 2 000 28.7 / 23.7; 16 of 3 000, one token, 32.7 / 27.6; 6 of 100 ... 5 000
+// e4m3, 16 heads of 256, 36.1 / 30.5; where it does not help, 8 of 500 ... 12 000 38.5 / 39.2, 4 of 8 000 19.9 / 20.6.
+constexpr int kPagedChooseEntries = 4096;  // (their parts are counted in 16 bits)
 
 // How an entry is cut.
 struct PagedCut {
@@ -193,7 +199,8 @@ struct PagedCut {
 // Finds the entry that has part `group` of all entries' parts.  False: there is none.  Called by all threads of a block, each
 // of which looks at batch / kPagedThreads entries in a row.  STEP: keys of a step; heads: units of an entry.
 template <int D, int STEP>
-__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, unsigned heads, int64_t group) {
+__device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, const PagedAttnParams& p, unsigned heads,
+                                           int64_t group) {
   const PagedCache& c = p.c;
   const int per = (c.batch + kPagedThreads - 1) / kPagedThreads;
   const int first = threadIdx.x * per, last = min(first + per, c.batch);
@@ -204,26 +211,43 @@ __device__ __forceinline__ bool paged_find(PagedSums& sums, PagedCut& found, con
   for (int e = first; e < last; ++e) total += paged_steps<STEP>(c, len_of(e));
   paged_block_sum(sums, total, all);
   const uint64_t once = (all * heads + p.resident - 1) / p.resident;
-  const uint64_t wanted = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, static_cast<uint64_t>(kPagedGoodSteps<D, STEP>))),
-                              static_cast<uint64_t>(kPagedMinKeys / STEP));
-  const uint32_t length = static_cast<uint32_t>(min(wanted, uint64_t{1} << 30));  // (no entry has more steps)
-  // parts in the low half, parts of cut entries in the high half
-  auto parts_of = [&](int steps) {
-    const uint64_t parts = (static_cast<uint32_t>(steps) + length - 1) / length;
-    return parts | (parts > 1 ? parts << 32 : 0);
-  };
+  constexpr uint64_t kGood = kPagedGoodSteps<D, STEP>, kLeast = kPagedMinKeys / STEP;
+  const uint64_t wanted = max(max((once + kPagedWaves - 1) / kPagedWaves, min(once, kGood)), kLeast);
+  uint32_t length = static_cast<uint32_t>(min(wanted, uint64_t{1} << 30));  // (no entry has more steps)
+  // Parts, and parts of cut entries: in halves of 32 bits; with a second length to choose from, in quarters.
+  const bool choose = once > kLeast && once <= kGood && c.batch <= kPagedChooseEntries;
+  const uint32_t even = (static_cast<uint32_t>(all) + p.even_parts - 1) / p.even_parts;  // (to choose, `all` is small)
+  const uint32_t longer = max(length + (length + 3) / 4, min(even, length + (length + 1) / 2));
+  auto parts_of = [&](int steps, uint32_t len) -> uint64_t { return (static_cast<uint32_t>(steps) + len - 1) / len; };
   uint64_t mine = 0;
-  for (int e = first; e < last; ++e) mine += parts_of(paged_steps<STEP>(c, len_of(e)));
+  for (int e = first; e < last; ++e) {
+    const int steps = paged_steps<STEP>(c, len_of(e));
+    const uint64_t parts = parts_of(steps, length);
+    if (choose) {
+      const uint64_t fewer = parts_of(steps, longer);
+      mine += parts | (parts > 1 ? parts << 16 : 0) | fewer << 32 | (fewer > 1 ? fewer << 48 : 0);
+    } else {
+      mine += parts | (parts > 1 ? parts << 32 : 0);
+    }
+  }
   uint64_t from = paged_block_sum(sums, mine, all) - mine;
+  if (choose) {
+    if ((all & 0xffff) * heads > p.resident && (all >> 32 & 0xffff) * heads <= p.resident) {
+      length = longer;
+      from >>= 32;
+      mine >>= 32;
+    }
+    from = (from & 0xffff) | (from & 0xffff0000u) << 16;
+    mine = (mine & 0xffff) | (mine & 0xffff0000u) << 16;
+  }
   const int64_t low = static_cast<int64_t>(from & 0xffffffffu), high = low + static_cast<int64_t>(mine & 0xffffffffu);
   if (group >= low && group < high) {
     for (int e = first; e < last; ++e) {
       const int n = len_of(e), steps = paged_steps<STEP>(c, n);
-      const uint64_t parts = parts_of(steps);
-      const int64_t before = static_cast<int64_t>(from & 0xffffffffu), count = static_cast<int64_t>(parts & 0xffffffffu);
+      const int64_t before = static_cast<int64_t>(from & 0xffffffffu), count = static_cast<int64_t>(parts_of(steps, length));
       if (group >= before && group < before + count)
         found = PagedCut{e, n, steps, static_cast<int>(count), before, static_cast<int64_t>(from >> 32)};
-      from += parts;
+      from += count | (count > 1 ? count << 32 : 0);
     }
   }
   __syncthreads();
@@ -472,7 +496,8 @@ constexpr int kNoSlice = -2147483647;  // in place of a page: beyond the part
 // Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
 template <int D, class T, int NT>
 __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
-                                            PagedRing& ring, uint32_t queries, int b, int n, int kv_head, int row0, int rows_valid, int step0, int step1,
+                                            PagedRing& ring, uint32_t queries, int b, int n, int kv_head, int row0, int rows_valid,
+                                            int step0, int step1,
                                             PagedState<D, NT, kPagedSlices<D, T, NT>>& st) {
   using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
@@ -645,7 +670,8 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       for (int x = rows * (Tile::kBlockRow / 16) + lane; x < kPagedSlice * (Tile::kBlockRow / 16); x += 32)
 #pragma unroll
         for (int block = 0; block < Tile::kBlocks; ++block)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(stage + L::kTensorBytes + block * Tile::kBlockBytes + x * 16),
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};"
+                       ::"r"(stage + L::kTensorBytes + block * Tile::kBlockBytes + x * 16),
                        "r"(0)
                        : "memory");
       __syncwarp();
@@ -844,6 +870,7 @@ cudaError_t splitk_t(PagedAttnParams& p, const CUtensorMap* maps, cudaStream_t s
   if (e != cudaSuccess) return e;
   const int64_t chunks = (static_cast<int64_t>(p.rows) * (p.heads_q / p.c.heads_kv) + 8 * NT - 1) / (8 * NT);
   const int64_t heads = p.c.heads_kv * chunks;
+  p.even_parts = static_cast<int>(p.c.batch * std::max<int64_t>(1, p.resident / (p.c.batch * heads)));
   // Parts of all entries: one each, and as many more as there are CTAs to make; and no more than kPagedMinKeys make of full
   // entries.
   constexpr int kStep = kPagedStep<D, T, NT>, kMinSteps = kPagedMinKeys / kStep;
