@@ -327,6 +327,8 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
 // SCALED: K and V are codes with a scale for every 16 keys (FwdParams::key_scales).  A code is exact in fp16; its value, rounded,
 // would not be.  K's scale multiplies the scores.  V's is part of the weight: P = 2^(s + log2 v - m), with m the largest
 // such exponent so far, so that P keeps its bits however the scales differ, and the row sums add P / v.
+// (512 tokens on 4 x 8 000 int8 positions, 32 / 8 heads of 128: 296 us with the pass that puts the pages in order, 369 when the
+// scales were fetched behind the scores, fp16 pages 281.)
 template <int D, bool CAUSAL, bool SHIFTED, int SHAPE, bool SPLIT, bool SCALED>
 __global__ void __launch_bounds__(FwdSmem<D, SHAPE>::kThreads, FwdSmem<D, SHAPE>::kCtasPerSm)
 fal_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
