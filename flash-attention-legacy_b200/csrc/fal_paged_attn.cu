@@ -536,8 +536,13 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     // (an ordinary load: the append before may still be writing scales while this grid's blocks take their places)
     return kScaled && there(page) ? scales[static_cast<int64_t>(page) * c.heads_kv + kv_head] : 1.f;
   };
-  // log2 of V's scale; of 0, which a page of zeros has, of a number that is as good
-  auto v_log_of = [&](int page) { return kScaled ? __log2f(scale_of(c.v_scales, page) + 0x1p-100f) : 0.f; };
+  // log2 of V's scale; of 0, which a page of zeros has, of a number small enough for its values to be no more than 0 in fp16, but no
+  // smaller: its keys' weights in the softmax sum are those of the exponents v log down from the others', which 2^-126 ends.
+  // (At 2^-100 keys with 2^-20 of the weight of one whose V values are the largest of fp16 were lost.)
+  auto v_log_of = [&](int page) {
+    const float scale = scale_of(c.v_scales, page);
+    return kScaled ? __log2f(scale < 0x1p-60f ? 0x1p-60f : scale) : 0.f;  // (a NaN stays one)
+  };
   int pages = pages_of(0), next_pages = 0;
   float k_scales = 0.f, v_logs = 0.f, next_k = 0.f, next_v = 0.f, last_k = 0.f, last_v = 0.f;
   uint32_t fill = 0;  // stage that the next loads go to
