@@ -1188,6 +1188,7 @@ constexpr int64_t kPagedUnknownSlots = 148 * 24;  // without a GPU to ask
 fal::PagedAttnParams paged_attn_params(const fal_paged_attn_args& a) {
   fal::PagedAttnParams p{};
   p.c = paged_cache(a.cache);
+  p.c.appended = a.appended != 0 ? a.rows : 0;
   p.q = a.q; p.q_strides = to_rs(&a.q_strides); p.o = a.o;
   p.heads_q = a.heads_q; p.rows = a.rows; p.kernel_dim = kernel_head_dim(a.cache.head_dim);
   p.cuts = static_cast<int64_t*>(a.workspace);
@@ -1200,14 +1201,16 @@ fal::PagedAttnParams paged_attn_params(const fal_paged_attn_args& a) {
 struct PagedPlan {
   bool few_rows;
   int entries, heads;  // many rows: (entry, KV head) pairs whose rows are put in order at a time
+  int capacity;        // rows of an (entry, KV head)
   int key_blocks;      // of an (entry, KV head), 0 for fp16 pages
-  size_t k_bytes, scale_bytes, lse_bytes, split_bytes;
+  size_t k_bytes, scale_bytes, lse_bytes, lens_bytes, split_bytes;
   size_t total;
 };
 
 PagedPlan paged_plan(const fal_paged_attn_args& a) {
   const fal_paged_cache& c = a.cache;
-  const int64_t capacity = static_cast<int64_t>(c.pages_per_entry) * c.page_size;
+  // (with room for rows that were appended, all of them beyond the table: paged_gather)
+  const int64_t capacity = static_cast<int64_t>(c.pages_per_entry) * c.page_size + (a.appended != 0 ? a.rows : 0);
   const int group = a.heads_q / c.heads_kv;
   const int64_t rows = static_cast<int64_t>(a.rows) * group;
   const int dim = kernel_head_dim(c.head_dim);
@@ -1230,12 +1233,14 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
     const int64_t e = kPagedGatherBytes / (unit * c.heads_kv);
     p.entries = static_cast<int>(e < 1 ? 1 : e < c.batch ? e : c.batch);
   }
+  p.capacity = static_cast<int>(capacity);
   p.k_bytes = static_cast<size_t>(p.entries) * p.heads * capacity * c.head_dim * 2;
   p.key_blocks = c.dtype != FAL_PAGED_F16 ? static_cast<int>(round_up(capacity, 128) / fal::kPagedBoxRows) : 0;
   p.scale_bytes = static_cast<size_t>(p.entries) * p.heads * p.key_blocks * sizeof(float4);
   p.lse_bytes = round_up(static_cast<int64_t>(p.entries) * p.heads * group * a.rows * 4, 256);
+  p.lens_bytes = a.appended != 0 ? round_up(static_cast<int64_t>(p.entries) * 4, 256) : 0;
   p.split_bytes = fal_fwd_kvcache_workspace_bytes(p.entries, p.heads * group, a.rows, static_cast<int>(capacity), c.head_dim);
-  p.total = 2 * p.k_bytes + p.scale_bytes + p.lse_bytes + p.split_bytes;
+  p.total = 2 * p.k_bytes + p.scale_bytes + p.lse_bytes + p.lens_bytes + p.split_bytes;
   return p;
 }
 
@@ -1246,7 +1251,7 @@ int paged_attn_check(const fal_paged_attn_args& a) {
     return FAL_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15u) != 0 || !paged_strides_ok(a.q_strides, 8))
     return FAL_ERR_INVALID_ARGUMENT;
-  if (static_cast<int64_t>(a.cache.batch) * a.rows * a.heads_q > 0x7fffffff) return FAL_ERR_INVALID_ARGUMENT;
+  if (static_cast<int64_t>(a.cache.batch) * a.rows * a.heads_q > 0x7fffffff || a.rows > (1 << 29)) return FAL_ERR_INVALID_ARGUMENT;
   return FAL_OK;
 }
 
@@ -1289,7 +1294,7 @@ size_t fal_paged_attn_workspace_bytes(const fal_paged_attn_args* a) {
   // (the pointers of the workspace itself and of what the call writes may still be missing)
   if (!a || a->cache.batch <= 0 || a->cache.heads_kv <= 0 || a->cache.page_size <= 0 || a->cache.pages_per_entry <= 0 ||
       static_cast<int64_t>(a->cache.pages_per_entry) * a->cache.page_size > (1 << 30) || a->heads_q < a->cache.heads_kv ||
-      a->rows <= 0 || !head_dim_ok(a->cache.head_dim) || static_cast<int64_t>(a->cache.batch) * a->rows * a->heads_q > 0x7fffffff)
+      a->rows <= 0 || a->rows > (1 << 29) || !head_dim_ok(a->cache.head_dim) || static_cast<int64_t>(a->cache.batch) * a->rows * a->heads_q > 0x7fffffff)
     return 0;
   return paged_plan(*a).total;
 }
@@ -1315,19 +1320,25 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
     return e == cudaSuccess ? FAL_OK : cuda_fail(e);
   }
 
-  const int capacity = c.pages_per_entry * c.page_size;
+  const int capacity = plan.capacity;
   const int group = a->heads_q / c.heads_kv;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   fal::PagedGatherParams g{};
   g.c = paged_cache(c);
+  g.c.appended = a->appended != 0 ? a->rows : 0;
   g.k_out = ws;
   g.v_out = ws + plan.k_bytes;
   g.status = a->status;
   g.scales_out = plan.key_blocks != 0 ? reinterpret_cast<float4*>(ws + 2 * plan.k_bytes) : nullptr;
   g.key_blocks = plan.key_blocks;
   g.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  float* lse = reinterpret_cast<float*>(ws + 2 * plan.k_bytes + plan.scale_bytes);
-  void* split = plan.split_bytes != 0 ? ws + 2 * plan.k_bytes + plan.scale_bytes + plan.lse_bytes : nullptr;
+  g.capacity = capacity;
+  ws += 2 * plan.k_bytes + plan.scale_bytes;
+  float* lse = reinterpret_cast<float*>(ws);
+  ws += plan.lse_bytes;
+  g.lens_out = plan.lens_bytes != 0 ? reinterpret_cast<int32_t*>(ws) : nullptr;
+  ws += plan.lens_bytes;
+  void* split = plan.split_bytes != 0 ? ws : nullptr;
   const fal_strides o_strides = {static_cast<int64_t>(a->rows) * a->heads_q * c.head_dim, c.head_dim,
                                  static_cast<int64_t>(a->heads_q) * c.head_dim};
   for (g.b0 = 0; g.b0 < c.batch; g.b0 += plan.entries) {
@@ -1340,14 +1351,16 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
                               static_cast<int64_t>(capacity) * c.head_dim, c.head_dim};
       const __half* q = static_cast<const __half*>(a->q) + g.b0 * a->q_strides.batch + g.h0 * group * a->q_strides.head;
       __half* o = static_cast<__half*>(a->o) + g.b0 * o_strides.batch + g.h0 * group * o_strides.head;
-      rc = fwd_batched(q, g.k_out, g.v_out, o, lse, c.cache_seqlens + g.b0, g.entries, g.heads * group, g.heads, a->rows,
+      rc = fwd_batched(q, g.k_out, g.v_out, o, lse, g.lens_out != nullptr ? g.lens_out : c.cache_seqlens + g.b0, g.entries, g.heads * group, g.heads, a->rows,
                        capacity, c.head_dim, &a->q_strides, &kv, &kv, &o_strides, a->softmax_scale,
                        FAL_CAUSAL_BOTTOM_RIGHT, a->status, a->stream, split, plan.split_bytes, g.scales_out,
                        plan.key_blocks);
       if (rc != FAL_OK) return rc;
     }
   }
-  return FAL_OK;
+  if (a->appended == 0) return FAL_OK;
+  const cudaError_t e = fal::launch_paged_zero(paged_attn_params(*a), st);
+  return e == cudaSuccess ? FAL_OK : cuda_fail(e);
 }
 
 int fal_set_fwd_variant(int variant) {

@@ -445,6 +445,7 @@ PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize
   r.cache = a.cache;
   r.heads_q = static_cast<int>(q->size(2));
   r.rows = static_cast<int>(q->size(1));
+  r.appended = appends ? 1 : 0;
   r.q = q->const_data_ptr();
   r.q_strides = row_strides(*q);
   a.status = r.status = self->status[dev];
@@ -470,7 +471,6 @@ PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize
         r.q = a.q_out;
         r.q_strides = row_strides(turned);
       }
-      r.cache.cache_seqlens = a.new_seqlens;
       if (!(r.softmax_scale > 0.f)) rc = FAL_ERR_INVALID_ARGUMENT;
       else rc = self->paged_append_run(&a);
       if (rc == 0) paged_written(x);

@@ -212,6 +212,7 @@ struct PagedCache {
   int batch;
   int heads_kv;
   int head_dim;          // the tensors' head_dim
+  int appended;          // attention: rows that were appended to every entry behind lens, as far as they fit
 };
 
 // New rows: q and k rotated by their positions, k and v to their places in the cache.
@@ -244,7 +245,7 @@ struct PagedAttnParams {
   float* part_o;         // workspace [slots, rows per CTA, kernel head_dim]
   float* part_ml;        // workspace [slots, rows per CTA, 2], behind part_o
   int heads_q;
-  int rows;              // query i sees the keys up to position len - rows + i
+  int rows;              // query i sees the keys up to position len - rows + i (c.appended: len + i, none beyond the capacity)
   int kernel_dim;        // 64, 128 or 256
   int resident;          // CTAs of the split-K kernel that run at once
   int even_parts;        // parts of all entries that together are no more than there are places, were all of one length
@@ -266,6 +267,8 @@ struct PagedGatherParams {
   PagedCache c;
   void* k_out;           // [entries, heads, capacity, head_dim]
   void* v_out;
+  int capacity;          // rows of an (entry, head): those of the block table, and c.appended
+  int32_t* lens_out;     // c.appended: [entries], the lengths that tell the tokens' positions, zeros in place of rows beyond the table
   float4* scales_out;    // 8-bit pages: [entries, heads, key_blocks]
   int key_blocks;        // a multiple of 8
   float scale_log2;      // softmax scale x log2(e)
@@ -273,5 +276,7 @@ struct PagedGatherParams {
   int* status;
 };
 cudaError_t launch_paged_gather(const PagedGatherParams& p, cudaStream_t stream);
+// The output rows of tokens that were appended beyond the capacity: zeros.
+cudaError_t launch_paged_zero(const PagedAttnParams& p, cudaStream_t stream);
 
 }  // namespace fal

@@ -14,7 +14,19 @@ struct E4M3 {
 };
 
 __device__ __forceinline__ int paged_capacity(const PagedCache& c) { return c.pages_per_entry << c.page_shift; }
-__device__ __forceinline__ int paged_len(const PagedCache& c, int b) { return min(max(c.lens[b], 0), paged_capacity(c)); }
+// Positions of entry b that attention sees.
+__device__ __forceinline__ int paged_len(const PagedCache& c, int b) {
+  const int length = c.lens[b], capacity = paged_capacity(c);
+  if (length < 0) return 0;
+  const unsigned n = static_cast<unsigned>(min(length, capacity)) + static_cast<unsigned>(c.appended);
+  return static_cast<int>(min(n, static_cast<unsigned>(capacity)));
+}
+// First position that the first of `rows` query tokens of entry b, which has n positions, does not see.  Where rows were appended
+// and may have run over the capacity, n does not tell their positions.
+__device__ __forceinline__ int paged_first_limit(const PagedCache& c, int b, int n, int rows) {
+  if (c.appended != 0 && n == paged_capacity(c)) return min(c.lens[b], n) + 1;
+  return n - rows + 1;
+}
 __device__ __forceinline__ int paged_len_in_pages(const PagedCache& c, int n) {
   return c.type == kPagedF16 ? n : n >> c.page_shift << c.page_shift;
 }

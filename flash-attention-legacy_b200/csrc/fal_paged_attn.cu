@@ -270,11 +270,11 @@ struct PagedState {
 
 // What follows the first product: scores s of this lane's keys key and key + 8 of H slices, from key0 on, for query rows 2 t and
 // 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have; first_limit: first key that the
-// entry's first token does not see.
+// entry's first token does not see; placed: rows whose tokens have a place in the cache.
 template <int H, int D, int NT, int HS>
 __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
-                                              const float (&k_scale)[H], const float (&v_log)[H], int first_limit, int row0,
-                                              int group) {
+                                              const float (&k_scale)[H], const float (&v_log)[H], int first_limit, int placed,
+                                              int row0, int group) {
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     const float f = st.c2 * k_scale[h];
@@ -291,7 +291,8 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int limit = min(end, first_limit + (row0 + nt * 8 + 2 * static_cast<int>(threadIdx.x & 3) + x) / group);
+        const int row = nt * 8 + 2 * static_cast<int>(threadIdx.x & 3) + x;
+        const int limit = row < placed ? min(end, first_limit + (row0 + row) / group) : 0;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           if (key + h * kPagedSlice >= limit) s[h][nt][x] = -INFINITY;
@@ -442,7 +443,7 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
 // The same of a slice of the tail at shared address base; K and V are there one after the other.
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint32_t base, int key0, int end, int first_limit,
-                                                  int row0, int group) {
+                                                  int placed, int row0, int group) {
   using Tail = PagedTailTile<D, T>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float s[1][NT][4];
@@ -461,7 +462,7 @@ __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint
     }
   }
   const float k_scale[1] = {1.f}, v_log[1] = {0.f};
-  paged_weights<1>(st, s, key0, key0 + g, end, k_scale, v_log, first_limit, row0, group);
+  paged_weights<1>(st, s, key0, key0 + g, end, k_scale, v_log, first_limit, placed, row0, group);
 }
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint32_t base) {
@@ -493,11 +494,12 @@ struct PagedRing {
 constexpr int kPagedBarrierId = 60;
 constexpr int kNoSlice = -2147483647;  // in place of a page: beyond the part
 
-// Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
+// Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ..., `placed` of which have a place), this
+// warp's slices of them.
 template <int D, class T, int NT>
 __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
                                             PagedRing& ring, uint32_t queries, int b, int n, int kv_head, int row0, int rows_valid,
-                                            int step0, int step1,
+                                            int first_limit, int placed, int step0, int step1,
                                             PagedState<D, NT, kPagedSlices<D, T, NT>>& st) {
   using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
@@ -646,8 +648,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[nt][j][e] = 0.f;
   }
-  const int first_limit = n - p.rows + 1;
-  st.min_limit = first_limit + row0 / group;
+  st.min_limit = placed < rows_valid ? 0 : first_limit + row0 / group;
   st.c2 = p.scale * kLog2e;
 
   const uint32_t k_read = Tile::k_read(g, t), v_read = L::kTensorBytes + Tile::v_read(g, t);
@@ -684,7 +685,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     float s[kH][NT][4];
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_scores<T>(st, s[h], stage + k_read + h * Tile::kSliceBytes);
-    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, v_log, first_limit, row0, group);
+    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, v_log, first_limit, placed, row0, group);
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes);
     drain = drain + 1 < L::kStages ? drain + 1 : 0;
@@ -696,8 +697,10 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       cp_async_wait<0>();
       __syncwarp();
       const uint32_t stage = ring.base + drain * L::kStageBytes;
-      if ((j & 1) == 0) paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n, first_limit, row0, group);
-      else paged_tail_output<T>(st, stage);
+      if ((j & 1) == 0)
+        paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n, first_limit, placed, row0, group);
+      else
+        paged_tail_output<T>(st, stage);
       drain = drain + 1 < L::kStages ? drain + 1 : 0;
       __syncwarp();
     }
@@ -770,11 +773,14 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
   const int kv_head = unit / chunks;
   const int row0 = unit % chunks * kRows;  // of the KV head's rows * group query rows
   const int rows_valid = min(kRows, p.rows * group - row0);
+  const int first_limit = paged_first_limit(c, b, cut.n, p.rows);
+  // rows of this chunk whose tokens have a place
+  const int placed = min(max(min(paged_capacity(c) + 1 - first_limit, p.rows) * group - row0, 0), rows_valid);
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   PagedRing ring{smem_u32(paged_smem) + warp * L::kRingBytes, smem_u32(&barriers[warp][0]), 0u, WaitCtx{&abort_flag, p.status}};
   PagedState<D, NT, kPagedSlices<D, T, NT>> st;
   paged_piece<D, T, NT>(p, &k_map, &v_map, ring, smem_u32(paged_smem) + L::kQueryOffset, b, cut.n, kv_head, row0, rows_valid,
-                        step0, step1, st);
+                        first_limit, placed, step0, step1, st);
   __syncthreads();  // the ring becomes the place of the warps' results
 
   // (column pair c of a row is at c ^ (its lane / 2): eight lanes and four rows of a store hit different banks)
@@ -812,6 +818,7 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
       o1 += x * y.y;
       l += x * mml[(w * kRows + r) * 2 + 1];
     }
+    if (r >= placed) o0 = o1 = 0.f;  // (weights of 0 throughout, which an infinity among the values would show through)
     if (cut.parts == 1) {
       const float inv = l != 0.f ? 1.f / l : 0.f;  // (0: the row sees no key)
       const int head = kv_head * group + (row0 + r) % group;
@@ -928,6 +935,23 @@ __device__ __forceinline__ bool paged_scale_apart(float scale) {
   const float a = fabsf(scale);
   return a >= 0x1p-40f && a <= 0x1p40f;
 }
+// What the first block of an (entry, head) adds where rows were appended: the forward kernel gets a length that tells the positions of
+// those that did not run over the table, and zeros behind it that only the rows without a place see.
+// (In all blocks, each with its share, the pass took 42 us where this takes 38: 4 x 512 tokens behind 7 000 int8 positions.)
+template <class T>
+__device__ __forceinline__ void paged_gather_over(const PagedGatherParams& p, int e, int hh, bool is_v, int n) {
+  const PagedCache& c = p.c;
+  const int end = n > 0 ? paged_first_limit(c, p.b0 + e, n, c.appended) - 1 + c.appended : 0;
+  if (blockIdx.y == 0 && threadIdx.x == 0) p.lens_out[e] = end;
+  const int64_t head = static_cast<int64_t>(e) * p.heads + hh;
+  uint4* rows = reinterpret_cast<uint4*>(static_cast<__half*>(is_v ? p.v_out : p.k_out) + (head * p.capacity + n) * c.head_dim);
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(end - n) * (c.head_dim / 8); i += 256) rows[i] = make_uint4(0, 0, 0, 0);
+  if (Elem<T>::kScaled && !is_v && end > n) {
+    const int blocks = (end + 127) / 128 * (128 / kPagedBoxRows);  // (n is a whole number of pages)
+    for (int i = n / kPagedBoxRows + threadIdx.x; i < blocks; i += 256)
+      p.scales_out[head * p.key_blocks + i] = make_float4(p.scale_log2, 0.f, 1.f, 0.f);
+  }
+}
 template <class T>
 __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGatherParams p) {
   const PagedCache& c = p.c;
@@ -938,6 +962,7 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
   const int hh = is_v ? blockIdx.y - p.heads : blockIdx.y;
   const int h = p.h0 + hh;
   const int n = paged_len(c, b), in_pages = paged_len_in_pages(c, n);
+  if (c.appended != 0 && blockIdx.x == 0) paged_gather_over<T>(p, e, hh, is_v, n);
   const int64_t task = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t pos = task / pieces;
   const int col = static_cast<int>(task % pieces) * 16;
@@ -991,11 +1016,22 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
     if (pos + kPagedBoxRows >= n)  // the rest of the last tile's 128 keys
       for (int64_t i = 1; ((pos / kPagedBoxRows + i) & 7) != 0; ++i) to[i] = make_float4(p.scale_log2, 0.f, 1.f, 0.f);
   }
-  const int64_t capacity = paged_capacity(c);
   __half* dst =
-      static_cast<__half*>(is_v ? p.v_out : p.k_out) + ((static_cast<int64_t>(e) * p.heads + hh) * capacity + pos) * c.head_dim + col;
+      static_cast<__half*>(is_v ? p.v_out : p.k_out) + ((static_cast<int64_t>(e) * p.heads + hh) * p.capacity + pos) * c.head_dim + col;
   reinterpret_cast<uint4*>(dst)[0] = out[0];
   reinterpret_cast<uint4*>(dst)[1] = out[1];
+}
+
+// Zeros for the tokens of entry blockIdx.x that have no place.  (Rows that the forward kernel left out itself
+// took 1 to 4 % of its other calls: 2 x 200 queries, 16 heads of 256, 44.1 us / 45.2 to 45.7.)
+__global__ void __launch_bounds__(256) fal_paged_zero_kernel(const PagedAttnParams p) {
+  grid_dependency_wait();
+  const int b = blockIdx.x, length = p.c.lens[b], capacity = paged_capacity(p.c);
+  if (length < 0 || length <= capacity - p.rows) return;  // (unused: zeros already)
+  const int64_t token = static_cast<int64_t>(p.heads_q) * p.c.head_dim / 8;  // pieces of 16 bytes
+  uint4* o = static_cast<uint4*>(p.o) + b * p.rows * token;
+  for (int64_t i = (capacity - min(length, capacity)) * token + threadIdx.x; i < p.rows * token; i += 256)
+    o[i] = make_uint4(0, 0, 0, 0);
 }
 
 }  // namespace
@@ -1019,6 +1055,10 @@ cudaError_t launch_paged_gather(const PagedGatherParams& p, cudaStream_t stream)
   else if (p.c.type == kPagedS8) fal_paged_gather_kernel<S8><<<grid, 256, 0, stream>>>(p);
   else fal_paged_gather_kernel<E4M3><<<grid, 256, 0, stream>>>(p);
   return cudaGetLastError();
+}
+
+cudaError_t launch_paged_zero(const PagedAttnParams& p, cudaStream_t stream) {
+  return launch_dependent(fal_paged_zero_kernel, dim3(p.c.batch), dim3(256), 0, stream, p);
 }
 
 }  // namespace fal

@@ -106,7 +106,8 @@ def flash_attn_with_paged_kvcache(
     q [B,L,Hq,d]; returns [B,L,Hq,d].  If k, v ([B,L,Hkv,d]) are given they are first appended at cache_seqlens[b], they and
     q rotated if rotary tables are given (`paged_cache_append`).  Without them the cache holds the new tokens' rows already:
     they are the last L of cache_seqlens[b] positions.  Query i sees everything up to its own position; a query without
-    any gives 0.  What the pages hold behind an entry's length does not matter; a position within it that has no page counts
+    any gives 0, and so does a token that runs over the end of its block table (the device status word is 2000 then; the
+    lengths that `paged_cache_append` returns end there and would not tell where the tokens that fit are).  What the pages hold behind an entry's length does not matter; a position within it that has no page counts
     as a row of zeros and the device status word becomes 3000.  (Between new tokens the mask is a weight of 0: a NaN or an
     infinity in the value row of one of them reaches the earlier ones of the same call.)  Inference only.
 
@@ -131,10 +132,10 @@ def flash_attn_with_paged_kvcache(
         assert v is not None and q.shape[:2] == k.shape[:2], "k, v must be [B, L, H_kv, d]"
 
         def append():
-            turned, lens = paged_cache_append(
+            turned, _ = paged_cache_append(
                 k, v, k_pages, v_pages, block_table, cache_seqlens, q if rotary_cos is not None else None, rotary_cos, rotary_sin,
                 rotary_interleaved, k_scales, v_scales, k_tail, v_tail, cache_layout)
-            return turned if turned is not None else q, lens
+            return turned if turned is not None else q
     else:
         assert v is None and rotary_cos is None and rotary_sin is None, "v and the rotary tables go with k"
     _inference_only(q, k_pages, v_pages, k_tail, v_tail)

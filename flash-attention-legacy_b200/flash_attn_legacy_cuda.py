@@ -880,8 +880,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_sca
                     k_tail=None, v_tail=None, cache_layout="bshd", append=None):
     """q [B,L,Hq,d] against a paged cache that holds its L rows already -> [B,L,Hq,d]; see fal_paged_attn_run in fal_b200.h.
 
-    `append`, if given, is called once everything else has been checked, and returns the queries (of q's shape) and the
-    lengths to go on with.
+    `append`, if given, is called once everything else has been checked: it appends the L rows behind cache_seqlens and
+    returns the queries (of q's shape) to go on with.
     The workspace is allocated per call, so that calls on different streams and captured graphs do not share one.
     """
     _require_cuda_half("q", q, 4)
@@ -903,15 +903,14 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_sca
 
     def args(workspace, nbytes):
         return _PAGED_ATTN_ARGS.pack(*block, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(2), q.stride(1), heads_q, L,
-                                     softmax_scale, 0, workspace, nbytes, _status_ptr(dev), _raw_stream(dev))
+                                     softmax_scale, int(append is not None), workspace, nbytes, _status_ptr(dev), _raw_stream(dev))
 
     nbytes = _lib.fal_paged_attn_workspace_bytes(args(0, 0))
     if nbytes == 0:
         raise RuntimeError("the call has too many query rows for one grid")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     if append is not None:
-        q, cache_seqlens = append()
-        block = (*block[:7], cache_seqlens.data_ptr(), *block[8:])
+        q = append()
     _check(_lib.fal_paged_attn_run(args(ws.data_ptr(), nbytes)))
     return out
 

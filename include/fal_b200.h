@@ -414,7 +414,10 @@ FAL_API int fal_paged_append_run(const fal_paged_append_args* args);
 
 /*
  * Attention of `rows` query tokens per entry over a paged cache that holds their own rows already: query i of entry b
- * sees positions up to cache_seqlens[b] - rows + i.  q [batch, rows, heads_q, head_dim] through strides (entry / head /
+ * sees positions up to cache_seqlens[b] - rows + i.  With `appended` an append of these tokens came before and cache_seqlens
+ * are the lengths before it: query i is at position cache_seqlens[b] + i, sees the positions up to its own, and gives
+ * zeros if that is beyond the capacity (the lengths that the append gave end at the capacity, and no longer tell the
+ * positions of tokens that ran over it); an entry with a negative length is unused and gives zeros.  q [batch, rows, heads_q, head_dim] through strides (entry / head /
  * row), o the same, contiguous.  A query that sees no position gives zeros; a position within the length that has no page
  * counts as a row of zeros and *status becomes 3000.  workspace: fal_paged_attn_workspace_bytes (16-byte aligned, not
  * shared by calls that overlap on the GPU).  Few rows run on a split-K pass over the pages, many on the forward kernel
@@ -427,7 +430,7 @@ typedef struct fal_paged_attn_args {
   fal_strides q_strides;
   int heads_q, rows;
   float softmax_scale;
-  int reserved;
+  int appended;
   void* workspace;
   size_t workspace_bytes;
   int* status;

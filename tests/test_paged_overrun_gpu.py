@@ -1,0 +1,113 @@
+"""GPU: a call whose new tokens run over the end of an entry's block table.  The tokens that fit see what they would see in a
+longer table, those without a place give 0, and the status word reports it."""
+import math
+
+import pytest
+import torch
+
+from paged_reference import assert_close, attention, rotate
+from test_paged_gpu import DTYPES, _filled, _lens, _rows, _tables
+
+pytestmark = pytest.mark.gpu
+
+
+def _run_over(ext, fal, dtype, rows, hq, hkv, d, page, width, lens, rotated, layout, native, monkeypatch):
+    gen = torch.Generator().manual_seed(rows + width)
+    capacity = width * page
+    cache = _filled(gen, DTYPES[dtype], [min(n, capacity) for n in lens], page, hkv, d, extra=rows)
+    cache.table = cache.table[:, :width].contiguous()
+    cos, sin = _tables(capacity, d)
+    got = cache.on_gpu(layout)
+    q, k, v = (_rows(gen, len(lens), rows, h, d) for h in (hq, hkv, hkv))
+    turning = dict(rotary_cos=cos.cuda(), rotary_sin=sin.cuda()) if rotated else {}
+    ext.reset_device_status()
+    if not native:
+        monkeypatch.setattr(ext, "paged_attend_plain", ext._general)
+        monkeypatch.setattr(ext, "paged_append_plain", ext._general)
+    o = fal.flash_attn_with_paged_kvcache(q.cuda(), block_table=cache.table.cuda(), cache_seqlens=_lens(lens), k=k.cuda(), v=v.cuda(),
+                                          cache_layout=layout, **turning, **got).cpu()
+    over = any(n >= 0 and n + rows > capacity for n in lens)
+    assert ext.device_status() == (2000 if over else 0)
+    ext.reset_device_status()
+    for e, n in enumerate(lens):
+        fit = 0 if n < 0 else max(min(rows, capacity - n), 0)
+        assert not o[e, fit:].any()
+        if fit == 0:
+            continue
+        turn = (lambda x: rotate(x[e, :fit], n, cos, sin, False)) if rotated else (lambda x: x[e, :fit])
+        cache.append(e, turn(k), v[e, :fit])
+        kd, vd = cache.dense(e, n + fit)
+        want, mag = attention(turn(q), kd, vd, 1 / math.sqrt(d))
+        assert_close(o[e, :fit], want, mag, n + fit, vd.abs().max().item())
+    cache.check(got, layout)
+
+
+@pytest.fixture()
+def ext():
+    import flash_attn_legacy_cuda as m
+    m.reset_device_status()
+    yield m
+    m.reset_device_status()
+
+
+@pytest.fixture()
+def fal():
+    import flash_attn_legacy as m
+    return m
+
+
+# Entries that run over in the middle, by one, by all but one, that are full or beyond it, unused, that just fit; up to 32 tokens
+# and more, in one tile and several, keys of a block dealt to several thread blocks (2 048 positions), one token.
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("rotated", [True, False])
+@pytest.mark.parametrize("rows,hq,hkv,d,page,width,lens,layout", [
+    (20, 4, 2, 64, 16, 3, [40, 10, -1, 48, 47, 29, 28, 3, 60], "bshd"),
+    (1, 8, 2, 128, 32, 4, [127, 128, 5, -3, 0], "bhsd"),
+    (5, 16, 1, 128, 16, 70, [1117, 1119, 1120, 1115, 600], "bshd"),
+    (32, 2, 1, 256, 16, 5, [60, 48, 49, 80], "bhsd"),
+    (40, 4, 2, 64, 32, 3, [70, 56, 57, 96, -1, 95, 10], "bshd"),
+    (150, 4, 4, 128, 16, 20, [200, 170, 171, 320, 319, 0], "bhsd"),
+    (300, 2, 2, 64, 64, 8, [300, 212, 213, 511, 100], "bshd"),
+    (60, 2, 1, 128, 64, 32, [2030, 1988, 1000, 2048, -1], "bshd"),
+    (70, 2, 2, 256, 128, 3, [350, 384, 20], "bshd")])
+def test_tokens_that_fit_see_their_own_positions(ext, fal, monkeypatch, dtype, native, rotated, rows, hq, hkv, d, page, width, lens, layout):
+    _run_over(ext, fal, dtype, rows, hq, hkv, d, page, width, lens, rotated, layout, native, monkeypatch)
+
+
+@pytest.mark.parametrize("rows", [6, 50])
+def test_tokens_without_a_place_give_zeros_whatever_the_cache_holds(ext, fal, rows):
+    gen = torch.Generator().manual_seed(3)
+    cache = _filled(gen, torch.float16, [30, 2000], 16, 2, 64, extra=rows)
+    cache.table = cache.table[:, :125].contiguous()  # 2 000 positions
+    got = cache.on_gpu("bshd")
+    got["v_pages"][cache.table[1, 0].item(), 3] = math.inf
+    got["v_pages"][cache.table[1, 124].item(), 15] = math.nan
+    q, k, v = (_rows(gen, 2, rows, h, 64).cuda() for h in (4, 2, 2))
+    o = fal.flash_attn_with_paged_kvcache(q, block_table=cache.table.cuda(), cache_seqlens=_lens([30, 2000]), k=k, v=v, **got)
+    assert not o[1].any() and not o[0].isnan().any()
+
+
+def test_a_captured_step_runs_into_the_end_of_its_table(ext, fal):
+    """Lengths moved on inside the graph, beyond the capacity: each replay as the eager call."""
+    gen = torch.Generator().manual_seed(4)
+    cache = _filled(gen, torch.int8, [44, 20], 16, 2, 64, extra=8)
+    cache.table = cache.table[:, :3].contiguous()
+    lens, table = _lens([44, 20]), cache.table.cuda()
+    q, k, v = (_rows(gen, 2, 2, h, 64).cuda() for h in (4, 2, 2))
+    got, eager = cache.on_gpu("bshd"), cache.on_gpu("bshd")
+    fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=lens, k=k, v=v, **{n: t.clone() for n, t in got.items()})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=lens, k=k, v=v, **got)
+        lens += 2
+    lens.copy_(_lens([44, 20]))
+    at = _lens([44, 20])
+    for _ in range(4):
+        graph.replay()
+        want = fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=at, k=k, v=v, **eager)
+        at += 2
+        assert torch.equal(o, want)
+        for n in got:
+            assert torch.equal(got[n].view(torch.uint8), eager[n].view(torch.uint8))
+    assert not o[0].any() and o[1].any()
