@@ -1148,6 +1148,13 @@ fal::PagedCache paged_cache(const fal_paged_cache& c) {
   return p;
 }
 
+// What make_paged_map needs of the strides: positive where they are stepped along, below the 2^40 bytes that a map holds.
+bool paged_map_ok(const fal_paged_cache& c, const fal_strides& s) {
+  const int64_t limit = (int64_t{1} << 40) / (c.dtype == FAL_PAGED_F16 ? 2 : 1);
+  if (s.row >= limit || s.head >= limit || s.batch >= limit) return false;
+  return s.row > 0 && (c.heads_kv == 1 || s.head > 0) && (c.num_pages == 1 || s.batch > 0);
+}
+
 // The pages as [page, head, row, head_dim], boxes as launch_paged_attn wants them.
 int make_paged_map(CUtensorMap* map, const void* base, const fal_paged_cache& c, const fal_strides& s) {
   EncodeTiledFn enc = get_encode_fn();
@@ -1158,7 +1165,6 @@ int make_paged_map(CUtensorMap* map, const void* base, const fal_paged_cache& c,
   const cuuint32_t box_bytes = row_bytes < 128 ? row_bytes : 128;
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
                               static_cast<cuuint64_t>(c.heads_kv), static_cast<cuuint64_t>(c.num_pages)};
-  if (s.row <= 0 || (c.heads_kv > 1 && s.head <= 0) || (c.num_pages > 1 && s.batch <= 0)) return FAL_ERR_INVALID_ARGUMENT;
   // (a dimension of extent 1 is never stepped along: any valid stride will do)
   auto fix = [&](int64_t x) { return static_cast<cuuint64_t>(x > 0 ? x : c.head_dim) * bytes; };
   const cuuint64_t strides[3] = {fix(s.row), fix(s.head), fix(s.batch)};
@@ -1247,6 +1253,8 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
 int paged_attn_check(const fal_paged_attn_args& a) {
   const int rc = paged_check(a.cache);
   if (rc != FAL_OK) return rc;
+  if (a.rows <= kPagedFewTokens && (!paged_map_ok(a.cache, a.cache.k_strides) || !paged_map_ok(a.cache, a.cache.v_strides)))
+    return FAL_ERR_INVALID_ARGUMENT;
   if (!a.q || !a.o || a.rows <= 0 || a.heads_q <= 0 || a.heads_q % a.cache.heads_kv != 0 || !(a.softmax_scale > 0.f))
     return FAL_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15u) != 0 || !paged_strides_ok(a.q_strides, 8))
@@ -1291,11 +1299,8 @@ int fal_paged_append_run(const fal_paged_append_args* a) {
 }
 
 size_t fal_paged_attn_workspace_bytes(const fal_paged_attn_args* a) {
-  // (the pointers of the workspace itself and of what the call writes may still be missing)
-  if (!a || a->cache.batch <= 0 || a->cache.heads_kv <= 0 || a->cache.page_size <= 0 || a->cache.pages_per_entry <= 0 ||
-      static_cast<int64_t>(a->cache.pages_per_entry) * a->cache.page_size > (1 << 30) || a->heads_q < a->cache.heads_kv ||
-      a->rows <= 0 || a->rows > (1 << 29) || !head_dim_ok(a->cache.head_dim) || static_cast<int64_t>(a->cache.batch) * a->rows * a->heads_q > 0x7fffffff)
-    return 0;
+  // Whoever appends rows before the call asks here first: all that the call itself would refuse, but for its workspace.
+  if (!a || paged_attn_check(*a) != FAL_OK) return 0;
   return paged_plan(*a).total;
 }
 

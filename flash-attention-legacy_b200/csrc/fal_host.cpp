@@ -451,6 +451,7 @@ PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize
   a.status = r.status = self->status[dev];
   at::Tensor o;
   int rc = 0;
+  bool appended = false;
   {
     pybind11::gil_scoped_release no_gil;
     at::Tensor lens, turned;
@@ -460,7 +461,7 @@ PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize
     r.workspace_bytes = self->paged_attn_workspace_bytes(&r);
     const at::Tensor ws = at::empty({static_cast<int64_t>(r.workspace_bytes)}, q->options().dtype(at::kByte));
     r.workspace = ws.data_ptr();
-    // (a call that the library refuses must not have appended anything: the general way makes it again)
+    // A call that the library refuses must not have appended anything (the general way makes it again): 0 bytes say so.
     if (r.workspace_bytes == 0) rc = FAL_ERR_INVALID_ARGUMENT;
     if (rc == 0 && appends) {
       lens = at::empty({a.cache.batch}, x.lens->options());
@@ -471,12 +472,14 @@ PyObject* calls_paged_attend(PyObject* self_obj, PyObject* const* args, Py_ssize
         r.q = a.q_out;
         r.q_strides = row_strides(turned);
       }
-      if (!(r.softmax_scale > 0.f)) rc = FAL_ERR_INVALID_ARGUMENT;
-      else rc = self->paged_append_run(&a);
-      if (rc == 0) paged_written(x);
+      rc = self->paged_append_run(&a);
+      appended = rc == 0;
+      if (appended) paged_written(x);
     }
     if (rc == 0) rc = self->paged_attn_run(&r);
   }
+  if (rc != 0 && appended)  // (the rows are in the cache, and appended again they would be rounded with what the tail has become)
+    return PyErr_Format(PyExc_RuntimeError, "flash_attn_legacy_cuda: attention failed behind an append that has been made (error %d)", rc);
   if (rc != 0) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(o));
   END_HANDLE_TH_ERRORS

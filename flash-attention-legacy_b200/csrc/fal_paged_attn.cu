@@ -1050,11 +1050,13 @@ cudaError_t launch_paged_gather(const PagedGatherParams& p, cudaStream_t stream)
   const int64_t tasks = (static_cast<int64_t>(p.c.pages_per_entry) << p.c.page_shift) * (p.c.head_dim / 16);
   const int64_t blocks = (tasks + 255) / 256;
   if (blocks > 0x7fffffff || 2 * p.heads > 65535 || p.entries > 65535) return cudaErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(blocks), 2 * p.heads, p.entries);
-  if (p.c.type == kPagedF16) fal_paged_gather_kernel<__half><<<grid, 256, 0, stream>>>(p);
-  else if (p.c.type == kPagedS8) fal_paged_gather_kernel<S8><<<grid, 256, 0, stream>>>(p);
-  else fal_paged_gather_kernel<E4M3><<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};  // (a launch that returns its own error, and none of another's)
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 2 * p.heads, p.entries);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  if (p.c.type == kPagedF16) return cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<__half>, p);
+  if (p.c.type == kPagedS8) return cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<S8>, p);
+  return cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<E4M3>, p);
 }
 
 cudaError_t launch_paged_zero(const PagedAttnParams& p, cudaStream_t stream) {

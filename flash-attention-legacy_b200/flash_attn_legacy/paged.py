@@ -111,6 +111,9 @@ def flash_attn_with_paged_kvcache(
     as a row of zeros and the device status word becomes 3000.  (Between new tokens the mask is a weight of 0: a NaN or an
     infinity in the value row of one of them reaches the earlier ones of the same call.)  Inference only.
 
+    A call that is refused has not appended anything.  Should a launch fail behind the append, the error says so: the rows are
+    in the cache then, and the same rows are not to be appended again.
+
     Up to 32 tokens run on a split-K pass that reads every page once for up to 32 (token, head) rows of a KV head; more run on
     the forward kernel, over the pages put in order in a workspace as large as the block table allows for (up to
     1 GiB at a time): pass a view of the table's first columns where entries are much shorter than it.

@@ -907,11 +907,14 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_sca
 
     nbytes = _lib.fal_paged_attn_workspace_bytes(args(0, 0))
     if nbytes == 0:
-        raise RuntimeError("the call has too many query rows for one grid")
+        raise RuntimeError("the call has too many query rows for one grid, or strides beyond what the kernels address")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     if append is not None:
         q = append()
-    _check(_lib.fal_paged_attn_run(args(ws.data_ptr(), nbytes)))
+    rc = _lib.fal_paged_attn_run(args(ws.data_ptr(), nbytes))
+    if rc != 0 and append is not None:
+        raise RuntimeError(f"flash_attn_legacy_cuda: attention failed behind an append that has been made (error {rc})")
+    _check(rc)
     return out
 
 

@@ -419,8 +419,8 @@ FAL_API int fal_paged_append_run(const fal_paged_append_args* args);
  * zeros if that is beyond the capacity (the lengths that the append gave end at the capacity, and no longer tell the
  * positions of tokens that ran over it); an entry with a negative length is unused and gives zeros.  q [batch, rows, heads_q, head_dim] through strides (entry / head /
  * row), o the same, contiguous.  A query that sees no position gives zeros; a position within the length that has no page
- * counts as a row of zeros and *status becomes 3000.  workspace: fal_paged_attn_workspace_bytes (16-byte aligned, not
- * shared by calls that overlap on the GPU).  Few rows run on a split-K pass over the pages, many on the forward kernel
+ * counts as a row of zeros and *status becomes 3000.  workspace: fal_paged_attn_workspace_bytes of the same block (0: the
+ * call would be refused; 16-byte aligned, not shared by calls that overlap on the GPU).  Few rows run on a split-K pass over the pages, many on the forward kernel
  * over the rows put in order in the workspace (as many entries and KV heads at a time as 1 GiB holds).
  */
 typedef struct fal_paged_attn_args {
