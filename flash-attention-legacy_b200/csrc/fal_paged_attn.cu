@@ -492,7 +492,7 @@ struct PagedRing {
   WaitCtx wait;
 };
 constexpr int kPagedBarrierId = 60;
-constexpr int kNoSlice = -2147483647;  // in place of a page: beyond the part
+constexpr int kNoSlice = -1;  // in place of a page: beyond the part
 
 // Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ..., `placed` of which have a place), this
 // warp's slices of them.
@@ -575,7 +575,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
         for (int h = 0; h < kH; ++h) {
           const int row = (key0 + h * kPagedSlice) & ((1 << c.page_shift) - 1);
           if (!there(page[h])) {  // (TMA fills a box outside of the tensor with zeros)
-            if (page[h] != kNoSlice && p.status) atomicCAS(p.status, 0, kDevNoPage);
+            if (key0 + h * kPagedSlice < page_end && p.status) atomicCAS(p.status, 0, kDevNoPage);
             page[h] = c.num_pages;
           }
 #pragma unroll
