@@ -21,6 +21,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 import flash_attn_legacy_cuda
 
@@ -28,8 +29,11 @@ from .flash_attn import SUPPORTED_HEAD_DIMS, _kernel_ready
 
 
 def _inference_only(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    tensors = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("paged caches are inference only: call under torch.no_grad() or detach the inputs")
+    if any(unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("paged caches are inference only: they take no forward-mode tangents")
 
 
 def _written(*tensors):
@@ -74,7 +78,7 @@ def paged_cache_append(
     assert q is None or q.dtype == torch.float16, f"Q must be float16, got {q.dtype}"
     d = k.shape[-1]
     assert d in SUPPORTED_HEAD_DIMS, f"head_dim must be 32, 64, 96, 128, or 256, got {d}"
-    _inference_only(q, k, v, k_pages, v_pages, k_tail, v_tail)
+    _inference_only(q, k, v, rotary_cos, rotary_sin, k_pages, v_pages, k_scales, v_scales, k_tail, v_tail)
     out = flash_attn_legacy_cuda.paged_append(
         _kernel_ready(k), _kernel_ready(v), k_pages, v_pages, block_table.to(torch.int32), cache_seqlens.to(torch.int32),
         _kernel_ready(q) if q is not None else None, rotary_cos, rotary_sin, rotary_interleaved,
@@ -141,6 +145,6 @@ def flash_attn_with_paged_kvcache(
             return turned if turned is not None else q
     else:
         assert v is None and rotary_cos is None and rotary_sin is None, "v and the rotary tables go with k"
-    _inference_only(q, k_pages, v_pages, k_tail, v_tail)
+    _inference_only(q, k_pages, v_pages, k_scales, v_scales, k_tail, v_tail)
     return flash_attn_legacy_cuda.paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, softmax_scale, k_scales,
                                                   v_scales, k_tail, v_tail, cache_layout, append)
