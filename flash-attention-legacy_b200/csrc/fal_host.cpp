@@ -13,6 +13,7 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/PythonDispatcherTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -351,6 +352,8 @@ fal_strides row_strides(const at::Tensor& t) { return {t.stride(0), t.stride(2),
 // Fills the append's block but for its outputs; q may be null.
 bool paged_append_block(const PagedTensors& x, const at::Tensor* q, const at::Tensor& k, const at::Tensor& v,
                         fal_paged_append_args& a) {
+  for (const at::Tensor* t : {x.kp, x.vp, x.ks, x.vs, x.kt, x.vt})  // (made in inference mode, written outside of it: refused)
+    if (t != nullptr && t->is_inference() && !c10::InferenceMode::is_enabled()) return false;
   if (k.sizes() != v.sizes() || k.size(0) != a.cache.batch || k.size(2) != a.cache.heads_kv || k.size(3) != a.cache.head_dim)
     return false;
   if (q != nullptr) {

@@ -36,6 +36,11 @@ def _inference_only(*tensors):
         raise RuntimeError("paged caches are inference only: they take no forward-mode tangents")
 
 
+def _writable(*tensors):
+    if not torch.is_inference_mode_enabled() and any(t is not None and t.is_inference() for t in tensors):
+        raise RuntimeError("a paged cache made in inference mode is not to be written outside of it")
+
+
 def _written(*tensors):
     for t in tensors:
         if t is not None and not t.is_inference():
@@ -79,6 +84,7 @@ def paged_cache_append(
     d = k.shape[-1]
     assert d in SUPPORTED_HEAD_DIMS, f"head_dim must be 32, 64, 96, 128, or 256, got {d}"
     _inference_only(q, k, v, rotary_cos, rotary_sin, k_pages, v_pages, k_scales, v_scales, k_tail, v_tail)
+    _writable(k_pages, v_pages, k_scales, v_scales, k_tail, v_tail)
     out = flash_attn_legacy_cuda.paged_append(
         _kernel_ready(k), _kernel_ready(v), k_pages, v_pages, block_table.to(torch.int32), cache_seqlens.to(torch.int32),
         _kernel_ready(q) if q is not None else None, rotary_cos, rotary_sin, rotary_interleaved,
