@@ -69,9 +69,10 @@ def paged_cache_append(
     k, v [B,L,Hkv,d] fp16 go to positions cache_seqlens[b] ... + L - 1 of every entry; `cache_seqlens` itself is not
     modified.  With rotary_cos / rotary_sin ([positions, rotary_dim / 2], fp32 or fp16, positions for the whole block table)
     the first rotary_dim columns of k, and of q [B,L,Hq,d] if given, are rotated: columns i and i + rotary_dim / 2 together,
-    or 2 i and 2 i + 1 with `rotary_interleaved`.  Rows without a place (an entry that is full, a table entry that names no
-    page) are dropped, their queries become 0, and the device status word 2000.  Pages that new rows go to must not be
-    shared between entries.
+    or 2 i and 2 i + 1 with `rotary_interleaved`.  Rows without a place are dropped and the device status word becomes 2000:
+    those behind the end of the block table, whose queries become 0 (as those of unused entries do), and those whose table
+    entry names no page (with 8-bit pages the whole page, when it is full), whose queries are rotated like any other.  The new
+    lengths end at the end of the table.  Pages that new rows go to must not be shared between entries.
     """
     # the ordinary call in one native function; None: any other
     out = flash_attn_legacy_cuda.paged_append_plain(k, v, k_pages, v_pages, block_table, cache_seqlens, rotary_cos, rotary_sin,

@@ -396,8 +396,9 @@ typedef struct fal_paged_cache {
  * are rotated by their position on the way, pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if rotary_interleaved,
  * in 32 bits, rounded once; q_out [batch, rows, heads_q, head_dim] is contiguous.  q (and q_out, heads_q) is optional.
  * new_seqlens[b] = cache_seqlens[b] + rows, the capacity at most.  An entry with a negative length is unused: nothing
- * of it is stored and its length stays.  A row without a place (beyond the capacity, or without a page) is dropped, its
- * query is 0, and *status becomes 2000.  Two entries must not share the page that new rows go to.
+ * of it is stored, its length stays and its queries are 0.  A row beyond the capacity is dropped and its query is 0; a row
+ * whose table entry names no page is dropped too (8-bit pages: with the page, when that would be written) and its query
+ * is rotated like any other.  *status becomes 2000 for both.  Two entries must not share the page that new rows go to.
  */
 typedef struct fal_paged_append_args {
   fal_paged_cache cache;
