@@ -1245,7 +1245,13 @@ PagedPlan paged_plan(const fal_paged_attn_args& a) {
   p.scale_bytes = static_cast<size_t>(p.entries) * p.heads * p.key_blocks * sizeof(float4);
   p.lse_bytes = round_up(static_cast<int64_t>(p.entries) * p.heads * group * a.rows * 4, 256);
   p.lens_bytes = a.appended != 0 ? round_up(static_cast<int64_t>(p.entries) * 4, 256) : 0;
-  p.split_bytes = fal_fwd_kvcache_workspace_bytes(p.entries, p.heads * group, a.rows, static_cast<int>(capacity), c.head_dim);
+  // (the entries or heads that are left for the last launch are fewer, and their keys are dealt to more CTAs: 33 entries of 32 768
+  // positions, 4 / 2 heads of 128, int8, 64 tokens 947 us / 759 so, fp16, 400 tokens 1 310 / 1 157)
+  for (const int e : {p.entries, c.batch % p.entries})
+    for (const int h : {p.heads, c.heads_kv % p.heads}) {
+      const size_t bytes = fal_fwd_kvcache_workspace_bytes(e, h * group, a.rows, static_cast<int>(capacity), c.head_dim);
+      if (bytes > p.split_bytes) p.split_bytes = bytes;
+    }
   p.total = 2 * p.k_bytes + p.scale_bytes + p.lse_bytes + p.lens_bytes + p.split_bytes;
   return p;
 }
