@@ -937,7 +937,8 @@ __device__ __forceinline__ bool paged_scale_apart(float scale) {
 }
 // What the first block of an (entry, head) adds where rows were appended: the forward kernel gets a length that tells the positions of
 // those that did not run over the table, and zeros behind it that only the rows without a place see.
-// (In all blocks, each with its share, the pass took 42 us where this takes 38: 4 x 512 tokens behind 7 000 int8 positions.)
+// (In all blocks, each with its share, the pass took 42 us where this takes 38: 4 x 512 tokens behind 7 000 int8 positions; asked of
+// calls that append nothing too, 64 tokens on 32 x 32 768 of 2 heads took 725 us where they take 722.)
 template <class T>
 __device__ __forceinline__ void paged_gather_over(const PagedGatherParams& p, int e, int hh, bool is_v, int n) {
   const PagedCache& c = p.c;
@@ -952,7 +953,7 @@ __device__ __forceinline__ void paged_gather_over(const PagedGatherParams& p, in
       p.scales_out[head * p.key_blocks + i] = make_float4(p.scale_log2, 0.f, 1.f, 0.f);
   }
 }
-template <class T>
+template <class T, bool APPENDED>
 __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGatherParams p) {
   const PagedCache& c = p.c;
   const int pieces = c.head_dim / 16;
@@ -962,7 +963,9 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
   const int hh = is_v ? blockIdx.y - p.heads : blockIdx.y;
   const int h = p.h0 + hh;
   const int n = paged_len(c, b), in_pages = paged_len_in_pages(c, n);
-  if (c.appended != 0 && blockIdx.x == 0) paged_gather_over<T>(p, e, hh, is_v, n);
+  if constexpr (APPENDED) {
+    if (blockIdx.x == 0) paged_gather_over<T>(p, e, hh, is_v, n);
+  }
   const int64_t task = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t pos = task / pieces;
   const int col = static_cast<int>(task % pieces) * 16;
@@ -1022,6 +1025,12 @@ __global__ void __launch_bounds__(256) fal_paged_gather_kernel(const PagedGather
   reinterpret_cast<uint4*>(dst)[1] = out[1];
 }
 
+template <class T>
+cudaError_t gather_t(const cudaLaunchConfig_t& cfg, const PagedGatherParams& p) {
+  return p.c.appended != 0 ? cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<T, true>, p)
+                           : cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<T, false>, p);
+}
+
 // Zeros for the tokens of entry blockIdx.x that have no place.  (Rows that the forward kernel left out itself
 // took 1 to 4 % of its other calls: 2 x 200 queries, 16 heads of 256, 44.1 us / 45.2 to 45.7.)
 __global__ void __launch_bounds__(256) fal_paged_zero_kernel(const PagedAttnParams p) {
@@ -1054,9 +1063,8 @@ cudaError_t launch_paged_gather(const PagedGatherParams& p, cudaStream_t stream)
   cfg.gridDim = dim3(static_cast<unsigned>(blocks), 2 * p.heads, p.entries);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
-  if (p.c.type == kPagedF16) return cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<__half>, p);
-  if (p.c.type == kPagedS8) return cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<S8>, p);
-  return cudaLaunchKernelEx(&cfg, fal_paged_gather_kernel<E4M3>, p);
+  if (p.c.type == kPagedF16) return gather_t<__half>(cfg, p);
+  return p.c.type == kPagedS8 ? gather_t<S8>(cfg, p) : gather_t<E4M3>(cfg, p);
 }
 
 cudaError_t launch_paged_zero(const PagedAttnParams& p, cudaStream_t stream) {
