@@ -88,26 +88,31 @@ def test_tokens_without_a_place_give_zeros_whatever_the_cache_holds(ext, fal, ro
     assert not o[1].any() and not o[0].isnan().any()
 
 
-def test_a_captured_step_runs_into_the_end_of_its_table(ext, fal):
+@pytest.mark.parametrize("rows", [2, 40])
+def test_captured_steps_run_into_the_end_of_their_table(ext, fal, rows):
     """Lengths moved on inside the graph, beyond the capacity: each replay as the eager call."""
     gen = torch.Generator().manual_seed(4)
-    cache = _filled(gen, torch.int8, [44, 20], 16, 2, 64, extra=8)
-    cache.table = cache.table[:, :3].contiguous()
-    lens, table = _lens([44, 20]), cache.table.cuda()
-    q, k, v = (_rows(gen, 2, 2, h, 64).cuda() for h in (4, 2, 2))
+    width = rows // 4 + 4
+    room = 2 * rows - rows // 2
+    lens = [width * 16 - room, 20]
+    cache = _filled(gen, torch.int8, lens, 16, 2, 64, extra=4 * rows)
+    cache.table = cache.table[:, :width].contiguous()
+    at, table = _lens(lens), cache.table.cuda()
+    q, k, v = (_rows(gen, 2, rows, h, 64).cuda() for h in (4, 2, 2))
     got, eager = cache.on_gpu("bshd"), cache.on_gpu("bshd")
-    fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=lens, k=k, v=v, **{n: t.clone() for n, t in got.items()})
+    inside = at.clone()
+    fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=at, k=k, v=v, **{n: t.clone() for n, t in got.items()})
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        o = fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=lens, k=k, v=v, **got)
-        lens += 2
-    lens.copy_(_lens([44, 20]))
-    at = _lens([44, 20])
+        o = fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=inside, k=k, v=v, **got)
+        inside += rows
+    dropped = []
     for _ in range(4):
         graph.replay()
         want = fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=at, k=k, v=v, **eager)
-        at += 2
+        at += rows
         assert torch.equal(o, want)
         for n in got:
             assert torch.equal(got[n].view(torch.uint8), eager[n].view(torch.uint8))
-    assert not o[0].any() and o[1].any()
+        dropped.append(int((o[0] == 0).all(dim=-1).all(dim=-1).sum()))
+    assert dropped == [min(max((i + 1) * rows - room, 0), rows) for i in range(4)] and dropped[0] == 0 and dropped[-1] == rows
