@@ -1362,7 +1362,8 @@ int fal_paged_attn_run(const fal_paged_attn_args* a) {
                               static_cast<int64_t>(capacity) * c.head_dim, c.head_dim};
       const __half* q = static_cast<const __half*>(a->q) + g.b0 * a->q_strides.batch + g.h0 * group * a->q_strides.head;
       __half* o = static_cast<__half*>(a->o) + g.b0 * o_strides.batch + g.h0 * group * o_strides.head;
-      rc = fwd_batched(q, g.k_out, g.v_out, o, lse, g.lens_out != nullptr ? g.lens_out : c.cache_seqlens + g.b0, g.entries, g.heads * group, g.heads, a->rows,
+      const int32_t* lens = g.lens_out != nullptr ? g.lens_out : c.cache_seqlens + g.b0;
+      rc = fwd_batched(q, g.k_out, g.v_out, o, lse, lens, g.entries, g.heads * group, g.heads, a->rows,
                        capacity, c.head_dim, &a->q_strides, &kv, &kv, &o_strides, a->softmax_scale,
                        FAL_CAUSAL_BOTTOM_RIGHT, a->status, a->stream, split, plan.split_bytes, g.scales_out,
                        plan.key_blocks);

@@ -396,7 +396,8 @@ fal_decode_combine_kernel(const DecodeParams p) {
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + static_cast<int64_t>(bh) * p.splits;
   const float4* po = reinterpret_cast<const float4*>(p.part_o) + static_cast<int64_t>(bh) * p.splits * (D / 4);
   __half* out_row = static_cast<__half*>(p.o) + static_cast<int64_t>(bh) * p.head_dim_real;
-  combine_row<D, WARPS>(tid, row_ok, n, ml, po, [](int i) { return static_cast<int64_t>(i); }, out_row, p.head_dim_real, p.lse != nullptr ? p.lse + bh : nullptr);
+  combine_row<D, WARPS>(tid, row_ok, n, ml, po, [](int i) { return static_cast<int64_t>(i); }, out_row, p.head_dim_real,
+                        p.lse != nullptr ? p.lse + bh : nullptr);
 }
 
 // ---------------------------------------------------------------------------

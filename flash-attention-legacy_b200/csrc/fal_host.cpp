@@ -311,7 +311,8 @@ bool paged_cache(PyObject* const* args, int64_t batch, int64_t head_dim, PagedTe
     if (table_type != at::kFloat && table_type != at::kHalf) return false;
     x.cos = plain(args[kCos], table_type, 2);
     x.sin = plain(args[kSin], table_type, 2);
-    if (!x.cos || !x.sin || tracked(*x.cos) || tracked(*x.sin) || !x.cos->is_contiguous() || !x.sin->is_contiguous() || x.cos->sizes() != x.sin->sizes() ||
+    if (!x.cos || !x.sin || tracked(*x.cos) || tracked(*x.sin) || !x.cos->is_contiguous() || !x.sin->is_contiguous() ||
+        x.cos->sizes() != x.sin->sizes() ||
         !fits_int({x.cos->size(0)}) || x.cos->size(1) > head_dim || x.cos->size(0) < width * page)
       return false;
     x.rotary_dim = static_cast<int>(2 * x.cos->size(1));

@@ -189,8 +189,8 @@ cudaError_t decode_static_scratch(float** ptr);
 cudaError_t launch_decode_splitk(const DecodeParams& p, cudaStream_t stream);
 cudaError_t launch_decode_combine(const DecodeParams& p, cudaStream_t stream);
 
-// Paged caches (fal_paged_append.cu, fal_paged_attn.cu): position p of entry b is row p % page of page table[b, p / page].  8-bit pages hold codes
-// with one fp32 scale per page and KV head; the rows of an entry's last, unfinished page are fp16 rows of its tail.
+// Paged caches (fal_paged_append.cu, fal_paged_attn.cu): position p of entry b is row p % page of page table[b, p / page].  8-bit
+// pages hold codes with one fp32 scale per page and KV head; the rows of an entry's last, unfinished page are fp16 rows of its tail.
 constexpr int kPagedMostRows = 256;  // of a page
 enum PagedType : int { kPagedF16 = 0, kPagedS8 = 1, kPagedE4M3 = 2 };
 struct PagedCache {

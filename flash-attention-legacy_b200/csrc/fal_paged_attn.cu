@@ -51,9 +51,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void cp_async_16_bytes(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 // D = A * B + C (fp16 16 x 16 and 16 x 8, fp32)
 __device__ __forceinline__ void mma_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                                const float (&c)[4]) {
@@ -599,8 +596,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       for (int it = 0; it < Tail::kLoads; ++it) {
         const int r = it * Tail::kCopyRows + lane / Tail::kChunks;
         const bool ok = row + r < tail_end && ch * 8 < c.head_dim;
-        cp_async_16_bytes(ring.base + fill * L::kStageBytes + Tail::place(r, ch), ok ? src + r * s.row + ch * 8 : src,
-                          ok ? 16u : 0u);
+        cp_async_16_zfill(ring.base + fill * L::kStageBytes + Tail::place(r, ch), ok ? src + r * s.row + ch * 8 : src, ok);
       }
       cp_async_commit();
     }
