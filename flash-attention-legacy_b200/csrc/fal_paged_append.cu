@@ -21,7 +21,8 @@ namespace {
 // tokens of 32 + 8 + 8 heads of 128, int8, 22.9 us, 4.2 TB/s); single tokens by latency.  A thread takes 16 columns of a head:
 // the two 8-column pieces whose columns are rotated with each other, or two neighbouring ones.
 constexpr int kAppendThreads = 256;
-// Blocks per SM: 48 registers a thread.  us with 4 / 5 / 6 blocks on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, fp16: 63.3 / 59.9
+// Blocks per SM: 48 registers a thread, at which the kernels of 8-bit pages store 192 bytes a thread and load 124 that four blocks
+// would leave in registers (fp16 pages: 8).  us with 4 / 5 / 6 blocks on 4 x 2 987 tokens of 40 + 8 + 8 heads of 128, fp16: 63.3 / 59.9
 // (5.8 TB/s) / 60.1; with 3 / 4 / 5 on the same in int8, 81.2 / 70.2 / 69.6, on 13 x 1 027 of 24 + 8 + 8, 73.1 / 63.4 / 61.4.
 constexpr int kAppendBlocks = 5;
 

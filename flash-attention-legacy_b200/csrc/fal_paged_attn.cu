@@ -25,7 +25,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // and Q is laid out to match; lane g of eight takes 16 neighbouring bytes of a V row.
 // 8-bit codes become fp16 in registers (exact).  The scales enter in 32 bits: K's multiplies the scores, V's is part of the
 // weights, P = 2^(s + log2 v - m) with m near the largest such exponent, so that P keeps its bits however the scales differ; the
-// softmax sum adds P / v, in 32 bits.  P^T of the scores' layout becomes the second product's operand by movmatrix.
+// softmax sum adds P / v, in 32 bits.  P is rounded to fp16 for the second product (2^-11 of each weight; P in two fp16 parts would
+// be twice the products), which adds 1.9e-4 to the 2.1e-4 of rounding the output.  P^T of the scores' layout becomes the second product's operand by movmatrix.
 //
 // An (entry, KV head, chunk of 8 NT query rows) is a unit; its keys count in steps, one 16-key slice for each of four warps, or
 // two.  Entries are cut into parts of one length that the GPU works out from all lengths, so that all units together
