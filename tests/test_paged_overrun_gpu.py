@@ -116,3 +116,44 @@ def test_captured_steps_run_into_the_end_of_their_table(ext, fal, rows):
             assert torch.equal(got[n].view(torch.uint8), eager[n].view(torch.uint8))
         dropped.append(int((o[0] == 0).all(dim=-1).all(dim=-1).sum()))
     assert dropped == [min(max((i + 1) * rows - room, 0), rows) for i in range(4)] and dropped[0] == 0 and dropped[-1] == rows
+
+
+# Tables so long that the entries, or the KV heads of one, are put in order a few at a time: as each of them alone.
+@pytest.mark.parametrize("dtype", ["fp16", "int8"])
+@pytest.mark.parametrize("hq,hkv,d,width,ends", [(4, 2, 64, 2048, [-30, None, -7, 5000, 0, -40, 600]), (8, 4, 128, 4096, [-30, None, 300])])
+def test_entries_a_few_at_a_time(ext, fal, dtype, hq, hkv, d, width, ends):
+    gen = torch.Generator().manual_seed(width)
+    page, rows, pool = 256, 40, 24
+    capacity, batch = page * width, len(ends)
+    lens = torch.tensor([-2 if n is None else n + capacity if n <= 0 else n for n in ends], dtype=torch.int32).cuda()
+    # every position has a page, most of them several times; the pages that new rows go to are an entry's own
+    table = torch.randint(0, pool, (batch, width), generator=gen, dtype=torch.int32)
+    for e, n in enumerate(lens.tolist()):
+        if n >= 0:
+            for i in range(n // page, min(n // page + 2, width)):
+                table[e, i] = pool + 2 * e + i % 2
+    table = table.cuda()
+    shape = (pool + 2 * batch, page, hkv, d)
+    caches = {}
+    for n in ("k", "v"):
+        x = _rows(gen, *shape).cuda()
+        if dtype == "fp16":
+            caches[n + "_pages"] = x
+        else:
+            caches[n + "_pages"] = (x.float() * 28).clamp(-127, 127).to(torch.int8)
+            caches[n + "_scales"] = (torch.rand(shape[0], hkv, generator=gen) / 50 + 0.01).cuda()
+            caches[n + "_tail"] = _rows(gen, batch, page, hkv, d).cuda()
+    q, k, v = (_rows(gen, batch, rows, h, d).cuda() for h in (hq, hkv, hkv))
+    start = {n: t.clone() for n, t in caches.items()}
+    o = fal.flash_attn_with_paged_kvcache(q, block_table=table, cache_seqlens=lens, k=k, v=v, softmax_scale=0.5, **caches)
+    assert ext.device_status() == 2000
+    for e in range(batch):
+        one = slice(e, e + 1)
+        alone = {n: (t[one].clone() if n.endswith("tail") else t.clone()) for n, t in start.items()}
+        used = max(min(int(lens[e]) + rows + page - 1, capacity) // page, 1)  # (a table no longer than the entry needs)
+        want = fal.flash_attn_with_paged_kvcache(q[one], block_table=table[one, :used], cache_seqlens=lens[one], k=k[one], v=v[one],
+                                                 softmax_scale=0.5, **alone)
+        # each: its output's rounding and its weights', 2^-11 of values below 6 each
+        assert float((o[one].double() - want.double()).abs().max()) <= 2 * 2 * 2.0 ** -11 * 6
+        placed = 0 if ends[e] is None else min(rows, capacity - int(lens[e]))
+        assert not o[e, placed:].any() and bool(o[e, :placed].any(dim=-1).all())
