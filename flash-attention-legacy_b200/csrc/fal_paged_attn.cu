@@ -268,10 +268,10 @@ struct PagedState {
 
 // What follows the first product: scores s of this lane's keys key and key + 8 of H slices, from key0 on, for query rows 2 t and
 // 2 t + 1 of every eight become weights.  end: of the keys that the slices are to have; first_limit: first key that the
-// entry's first token does not see; placed: rows whose tokens have a place in the cache.
+// entry's first token does not see; a token whose own would be beyond the capacity has no place and sees none.
 template <int H, int D, int NT, int HS>
 __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (&s)[H][NT][4], int key0, int key, int end,
-                                              const float (&k_scale)[H], const float (&v_log)[H], int first_limit, int placed,
+                                              const float (&k_scale)[H], const float (&v_log)[H], int first_limit, int capacity,
                                               int row0, int group) {
 #pragma unroll
   for (int h = 0; h < H; ++h) {
@@ -289,8 +289,8 @@ __device__ __forceinline__ void paged_weights(PagedState<D, NT, HS>& st, float (
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int row = nt * 8 + 2 * static_cast<int>(threadIdx.x & 3) + x;
-        const int limit = row < placed ? min(end, first_limit + (row0 + row) / group) : 0;
+        const int sees = first_limit + (row0 + nt * 8 + 2 * static_cast<int>(threadIdx.x & 3) + x) / group;
+        const int limit = sees > capacity ? 0 : min(end, sees);
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           if (key + h * kPagedSlice >= limit) s[h][nt][x] = -INFINITY;
@@ -441,7 +441,7 @@ __device__ __forceinline__ void paged_output(PagedState<D, NT, H>& st, int h, ui
 // The same of a slice of the tail at shared address base; K and V are there one after the other.
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint32_t base, int key0, int end, int first_limit,
-                                                  int placed, int row0, int group) {
+                                                  int capacity, int row0, int group) {
   using Tail = PagedTailTile<D, T>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float s[1][NT][4];
@@ -460,7 +460,7 @@ __device__ __forceinline__ void paged_tail_scores(PagedState<D, NT, H>& st, uint
     }
   }
   const float k_scale[1] = {1.f}, v_log[1] = {0.f};
-  paged_weights<1>(st, s, key0, key0 + g, end, k_scale, v_log, first_limit, placed, row0, group);
+  paged_weights<1>(st, s, key0, key0 + g, end, k_scale, v_log, first_limit, capacity, row0, group);
 }
 template <class T, int D, int NT, int H>
 __device__ __forceinline__ void paged_tail_output(PagedState<D, NT, H>& st, uint32_t base) {
@@ -492,12 +492,11 @@ struct PagedRing {
 constexpr int kPagedBarrierId = 60;
 constexpr int kNoSlice = -1;  // in place of a page: beyond the part
 
-// Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ..., `placed` of which have a place), this
-// warp's slices of them.
+// Steps step0 ... step1 - 1 of the unit (entry b of n positions, KV head, query rows row0 ...), this warp's slices of them.
 template <int D, class T, int NT>
 __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
                                             PagedRing& ring, uint32_t queries, int b, int n, int kv_head, int row0, int rows_valid,
-                                            int first_limit, int placed, int step0, int step1,
+                                            int first_limit, int step0, int step1,
                                             PagedState<D, NT, kPagedSlices<D, T, NT>>& st) {
   using L = PagedSmem<D, T, NT>;
   using Tile = PagedTile<D, T>;
@@ -645,7 +644,8 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[nt][j][e] = 0.f;
   }
-  st.min_limit = placed < rows_valid ? 0 : first_limit + row0 / group;
+  const int capacity = paged_capacity(c);
+  st.min_limit = first_limit + (row0 + rows_valid - 1) / group > capacity ? 0 : first_limit + row0 / group;
   st.c2 = p.scale * kLog2e;
 
   const uint32_t k_read = Tile::k_read(g, t), v_read = L::kTensorBytes + Tile::v_read(g, t);
@@ -682,7 +682,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
     float s[kH][NT][4];
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_scores<T>(st, s[h], stage + k_read + h * Tile::kSliceBytes);
-    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, v_log, first_limit, placed, row0, group);
+    paged_weights<kH>(st, s, key0, key0 + Tile::key_of(g), page_end, k_scale, v_log, first_limit, capacity, row0, group);
 #pragma unroll
     for (int h = 0; h < kH; ++h) paged_output<T>(st, h, stage + v_read + h * Tile::kSliceBytes);
     drain = drain + 1 < L::kStages ? drain + 1 : 0;
@@ -695,7 +695,7 @@ __device__ __forceinline__ void paged_piece(const PagedAttnParams& p, const CUte
       __syncwarp();
       const uint32_t stage = ring.base + drain * L::kStageBytes;
       if ((j & 1) == 0)
-        paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n, first_limit, placed, row0, group);
+        paged_tail_scores<T>(st, stage, in_pages + tail_first + (j >> 1) * kTailStep, n, first_limit, capacity, row0, group);
       else
         paged_tail_output<T>(st, stage);
       drain = drain + 1 < L::kStages ? drain + 1 : 0;
@@ -771,13 +771,11 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
   const int row0 = unit % chunks * kRows;  // of the KV head's rows * group query rows
   const int rows_valid = min(kRows, p.rows * group - row0);
   const int first_limit = paged_first_limit(c, b, cut.n, p.rows);
-  // rows of this chunk whose tokens have a place
-  const int placed = min(max(min(paged_capacity(c) + 1 - first_limit, p.rows) * group - row0, 0), rows_valid);
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   PagedRing ring{smem_u32(paged_smem) + warp * L::kRingBytes, smem_u32(&barriers[warp][0]), 0u, WaitCtx{&abort_flag, p.status}};
   PagedState<D, NT, kPagedSlices<D, T, NT>> st;
   paged_piece<D, T, NT>(p, &k_map, &v_map, ring, smem_u32(paged_smem) + L::kQueryOffset, b, cut.n, kv_head, row0, rows_valid,
-                        first_limit, placed, step0, step1, st);
+                        first_limit, step0, step1, st);
   __syncthreads();  // the ring becomes the place of the warps' results
 
   // (column pair c of a row is at c ^ (its lane / 2): eight lanes and four rows of a store hit different banks)
@@ -799,6 +797,8 @@ fal_paged_splitk_kernel(const PagedAttnParams p, const __grid_constant__ CUtenso
     }
   }
   __syncthreads();
+  // rows of this chunk whose tokens have a place
+  const int placed = min(max(min(paged_capacity(c) + 1 - first_limit, p.rows) * group - row0, 0), rows_valid);
   const int64_t slot = ((cut.slot + part) * heads + unit) * kRows;
   for (int idx = threadIdx.x; idx < rows_valid * (D / 2); idx += kPagedThreads) {
     const int r = idx / (D / 2), pair = idx % (D / 2);
